@@ -1,0 +1,766 @@
+// Kernels around the 8-bit format of fp8.cuh: quantising rows (plain, grouped by expert, or scattered to the expert
+// layout of the MoE layer), quantising weights with their transposed copy, dequantising, and SwiGLU that keeps its
+// inputs in 8 bits for the backward pass.  All are bound by HBM traffic: one pass over the data, 128-bit reads, every
+// value read once and written once; the block maximum lives in registers between the two.
+//
+// Row kernels: a warp takes 512 columns of a row (one scale word); 8 lanes share a block of 128 columns, so the block
+// maximum is three shuffles and every load instruction of the 8 lanes covers 128 contiguous bytes.
+#include "fp8.cuh"
+
+namespace fmab {
+
+constexpr int kQThreads = 256;
+constexpr int kQWarps = kQThreads / 32;
+
+template <typename T>
+struct LaneBlock {                                    // a lane's 16 of the block's 128 columns
+    static constexpr int V = Elem<T>::kPerVec;        // columns per 128-bit access
+    static constexpr int N = 16 / V;                  // accesses
+    // column (inside the block) of access j for the lane's place s = lane % 8
+    __device__ static __forceinline__ int column(int s, int j) { return j * 8 * V + s * V; }
+};
+
+__device__ __forceinline__ uint32_t max_over_8_lanes(uint32_t v) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// Reads the lane's 16 values of columns [col0, cols); columns beyond are zero.
+template <typename T>
+__device__ __forceinline__ void load_lane_block(const T* row, int col0, int cols, int s, float* x) {
+    using B = LaneBlock<T>;
+#pragma unroll
+    for (int j = 0; j < B::N; ++j) {
+        const int c = col0 + B::column(s, j);
+        const uint4 v = c < cols ? ld_stream_16(row + c) : make_uint4(0, 0, 0, 0);
+        Elem<T>::unpack(v, x + j * B::V);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_lane_block(T* row, int col0, int cols, int s, const float* x) {
+    using B = LaneBlock<T>;
+#pragma unroll
+    for (int j = 0; j < B::N; ++j) {
+        const int c = col0 + B::column(s, j);
+        if (c < cols) st_global_16(row + c, Elem<T>::pack(x + j * B::V));
+    }
+}
+// The lane's 16 bytes to / from the value row (pitch columns, of which those from `cols` on are zero).
+template <typename T>
+__device__ __forceinline__ void store_lane_bytes(uint8_t* row, int col0, int pitch, int s, const uint32_t* w) {
+    using B = LaneBlock<T>;
+#pragma unroll
+    for (int j = 0; j < B::N; ++j) {
+        const int c = col0 + B::column(s, j);
+        if (c >= pitch) continue;
+        if (B::V == 8)
+            *reinterpret_cast<uint2*>(row + c) = make_uint2(w[2 * j], w[2 * j + 1]);
+        else
+            *reinterpret_cast<uint32_t*>(row + c) = w[j];
+    }
+}
+template <typename T>
+__device__ __forceinline__ void load_lane_bytes(const uint8_t* row, int col0, int pitch, int s, uint32_t* w) {
+    using B = LaneBlock<T>;
+#pragma unroll
+    for (int j = 0; j < B::N; ++j) {
+        const int c = col0 + B::column(s, j);
+        if (B::V == 8) {
+            const uint2 v = c < pitch ? *reinterpret_cast<const uint2*>(row + c) : make_uint2(0, 0);
+            w[2 * j] = v.x;
+            w[2 * j + 1] = v.y;
+        } else {
+            w[j] = c < pitch ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
+        }
+    }
+}
+// Scale byte of the 8 lanes' block and its 16 packed values per lane; returns the warp's scale word (all lanes).
+__device__ __forceinline__ uint32_t quantize_lane_block(const float* x, uint32_t* w) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, fp8_magnitude(x[i]));
+    const uint32_t byte = fp8_scale_byte(max_over_8_lanes(m));
+    const float inverse = fp8_inverse(byte);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = fp8_pack4(x + 4 * i, inverse);
+    uint32_t word = byte << (8 * ((threadIdx.x & 31) >> 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    word |= __shfl_xor_sync(0xffffffffu, word, 16);
+    return word;
+}
+
+// Where a source row goes.  rows: to itself.  groups: rows of expert e are consecutive in the source
+// ([offsets[e], offsets[e+1])) and start at pad_offsets[e] in the layout.  slots: source row t goes to the k rows
+// row_of_slot[t*k ..] of the MoE layer's layout.
+constexpr int TO_ROWS = 0, TO_GROUPS = 1, TO_SLOTS = 2;
+struct QuantRows {
+    const void* x;
+    void* copy;               // groups: the rows themselves in the padded layout too, or null
+    uint8_t* values;
+    uint8_t* scales;
+    const int32_t* offsets;
+    const int32_t* pad_offsets;
+    const int32_t* row_of_slot;
+    const int32_t* slot_of_row;
+    int64_t x_pitch;
+    int64_t rows;             // source rows
+    int64_t row_blocks;       // blocks that quantise; the others zero the padding rows
+    int64_t layout_rows;
+    int64_t row_tiles;        // scale tiles per quad
+    int32_t cols, pitch, quads, n_groups, k;
+};
+
+// Largest e with offsets[e] <= row (empty experts are skipped: of equal offsets the last one counts).
+__device__ __forceinline__ int group_of_row(const int32_t* offsets, int n, int32_t row) {
+    int lo = 0, hi = n;  // offsets[lo] <= row < offsets[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(offsets + mid) <= row) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// Padding rows of the layout below its used end: zero values, zero copies.
+template <typename T, int TO>
+__device__ void zero_padding_rows(const QuantRows& p, int64_t first_row, int64_t step) {
+    const int lane = threadIdx.x & 31;
+    const int64_t used = min(static_cast<int64_t>(p.pad_offsets[p.n_groups]), p.layout_rows);
+    for (int64_t row = first_row; row < used; row += step) {
+        bool token;
+        if (TO == TO_SLOTS) {
+            token = p.slot_of_row[row] >= 0;
+        } else {
+            const int e = group_of_row(p.pad_offsets, p.n_groups, static_cast<int32_t>(row));
+            token = row - p.pad_offsets[e] < p.offsets[e + 1] - p.offsets[e];
+        }
+        if (token) continue;
+        for (int c = lane * 16; c < p.pitch; c += 512)
+            st_global_16(p.values + row * p.pitch + c, make_uint4(0, 0, 0, 0));
+        for (int q = lane; q < p.quads; q += 32)
+            *reinterpret_cast<uint32_t*>(p.scales + fp8_scale_word(row, q, p.row_tiles)) = 0x01010101u * FP8_SCALE_ONE;
+        if (TO == TO_GROUPS && p.copy != nullptr) {
+            constexpr int V = Elem<T>::kPerVec;
+            for (int c = lane * V; c < p.cols; c += 32 * V)
+                st_global_16(static_cast<T*>(p.copy) + row * p.cols + c, make_uint4(0, 0, 0, 0));
+        }
+    }
+}
+
+template <typename T, int TO>
+__global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRows p) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
+    if (TO != TO_ROWS && blockIdx.x >= p.row_blocks) {
+        zero_padding_rows<T, TO>(p, (blockIdx.x - p.row_blocks) * kQWarps + warp,
+                                 (static_cast<int64_t>(gridDim.x) - p.row_blocks) * kQWarps);
+        return;
+    }
+    const int64_t n_items = p.rows * p.quads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQWarps + warp; i < n_items; i += p.row_blocks * kQWarps) {
+        const int64_t row = i / p.quads;
+        const int q = static_cast<int>(i - row * p.quads);
+        const int col0 = q * FP8_QUAD + (lane >> 3) * FP8_BLOCK;
+        float x[16];
+        load_lane_block<T>(static_cast<const T*>(p.x) + row * p.x_pitch, col0, p.cols, s, x);
+        uint32_t w[4];
+        const uint32_t word = quantize_lane_block(x, w);
+        const int copies = TO == TO_SLOTS ? p.k : 1;
+        for (int j = 0; j < copies; ++j) {
+            int64_t to = row;
+            if (TO == TO_SLOTS) {
+                to = __ldg(p.row_of_slot + row * p.k + j);
+            } else if (TO == TO_GROUPS) {
+                if (row >= __ldg(p.offsets + p.n_groups)) break;  // a row of no expert
+                const int e = group_of_row(p.offsets, p.n_groups, static_cast<int32_t>(row));
+                to = __ldg(p.pad_offsets + e) + (row - __ldg(p.offsets + e));
+            }
+            if (TO != TO_ROWS && (to < 0 || to >= p.layout_rows)) continue;
+            store_lane_bytes<T>(p.values + to * p.pitch, col0, p.pitch, s, w);
+            if (lane == 0) *reinterpret_cast<uint32_t*>(p.scales + fp8_scale_word(to, q, p.row_tiles)) = word;
+            if (TO == TO_GROUPS && p.copy != nullptr)
+                store_lane_block<T>(static_cast<T*>(p.copy) + to * p.cols, col0, p.cols, s, x);
+        }
+    }
+}
+
+// ---- weights ---------------------------------------------------------------------------------------
+// One CTA per block of 128 x 128.  A thread holds 8 rows x 8 columns: its rows leave as 8-byte pieces, and the 8 x 8
+// bytes transposed in registers go through shared memory into the transposed copy, whose rows also leave whole.
+__device__ __forceinline__ void transpose_4x4(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+    const uint32_t ab_lo = __byte_perm(a, b, 0x5140), ab_hi = __byte_perm(a, b, 0x7362);
+    const uint32_t cd_lo = __byte_perm(c, d, 0x5140), cd_hi = __byte_perm(c, d, 0x7362);
+    a = __byte_perm(ab_lo, cd_lo, 0x5410);
+    b = __byte_perm(ab_lo, cd_lo, 0x7632);
+    c = __byte_perm(ab_hi, cd_hi, 0x5410);
+    d = __byte_perm(ab_hi, cd_hi, 0x7632);
+}
+
+struct QuantWeight {
+    const void* w;
+    uint8_t *values, *scales, *values_t, *scales_t;
+    int32_t E, N, K, pitch, pitch_t;  // pitch_t: of the transposed copy [E, K, pitch_t]
+    int32_t n_blocks, k_blocks;       // per expert
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_weight_kernel(const QuantWeight p) {
+    __shared__ uint32_t warp_max[8];
+    __shared__ __align__(16) uint8_t turned[FP8_BLOCK][FP8_BLOCK + 16];
+    constexpr int V = Elem<T>::kPerVec;
+    const int tid = threadIdx.x;
+    const int kb = blockIdx.x % p.k_blocks;
+    const int nb = blockIdx.x / p.k_blocks;
+    const int e = blockIdx.y;
+    const int r0 = nb * FP8_BLOCK + (tid >> 4) * 8, c0 = kb * FP8_BLOCK + (tid & 15) * 8;
+    const T* src = static_cast<const T*>(p.w) + (static_cast<int64_t>(e) * p.N + r0) * p.K + c0;
+    uint4 raw[8][8 / V];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8 / V; ++j)
+            raw[i][j] = (r0 + i < p.N && c0 < p.K) ? ld_stream_16(src + static_cast<int64_t>(i) * p.K + j * V) : make_uint4(0, 0, 0, 0);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8 / V; ++j) {
+            float x[V];
+            Elem<T>::unpack(raw[i][j], x);
+#pragma unroll
+            for (int v = 0; v < V; ++v) m = max(m, fp8_magnitude(x[v]));
+        }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((tid & 31) == 0) warp_max[tid >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, warp_max[i]);
+    const uint32_t byte = fp8_scale_byte(m);
+    const float inverse = fp8_inverse(byte);
+    uint32_t lo[8], hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8 / V; ++j) Elem<T>::unpack(raw[i][j], x + j * V);
+        lo[i] = fp8_pack4(x, inverse);
+        hi[i] = fp8_pack4(x + 4, inverse);
+        if (r0 + i < p.N && c0 < p.pitch)
+            *reinterpret_cast<uint2*>(p.values + (static_cast<int64_t>(e) * p.N + r0 + i) * p.pitch + c0) = make_uint2(lo[i], hi[i]);
+    }
+    if (tid < FP8_BLOCK)
+        p.scales[fp8_scale_word((static_cast<int64_t>(e) * p.n_blocks + nb) * FP8_BLOCK + tid, kb >> 2,
+                                static_cast<int64_t>(p.E) * p.n_blocks) + (kb & 3)] = static_cast<uint8_t>(byte);
+    if (p.values_t == nullptr) return;
+    if (tid < FP8_BLOCK)
+        p.scales_t[fp8_scale_word((static_cast<int64_t>(e) * p.k_blocks + kb) * FP8_BLOCK + tid, nb >> 2,
+                                  static_cast<int64_t>(p.E) * p.k_blocks) + (nb & 3)] = static_cast<uint8_t>(byte);
+    transpose_4x4(lo[0], lo[1], lo[2], lo[3]);  // lo[j] = rows 0-3 of column j
+    transpose_4x4(lo[4], lo[5], lo[6], lo[7]);  // lo[4 + j] = rows 4-7 of column j
+    transpose_4x4(hi[0], hi[1], hi[2], hi[3]);
+    transpose_4x4(hi[4], hi[5], hi[6], hi[7]);
+    const int tc = (tid & 15) * 8, tr = (tid >> 4) * 8;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        *reinterpret_cast<uint2*>(&turned[tc + j][tr]) = make_uint2(lo[j], lo[4 + j]);
+        *reinterpret_cast<uint2*>(&turned[tc + 4 + j][tr]) = make_uint2(hi[j], hi[4 + j]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int piece = i * 256 + tid, col = piece >> 3, at = (piece & 7) * 16;
+        const int k = kb * FP8_BLOCK + col, n = nb * FP8_BLOCK + at;
+        if (k < p.K && n < p.pitch_t)
+            st_global_16(p.values_t + (static_cast<int64_t>(e) * p.K + k) * p.pitch_t + n,
+                         *reinterpret_cast<const uint4*>(&turned[col][at]));
+    }
+}
+
+// ---- back to 16 or 32 bits -------------------------------------------------------------------------
+// Rounds once; what a rounding up to e4m3 lifted above the type's range comes back as its largest finite value.
+template <typename T>
+__device__ __forceinline__ float finite_in(float x);
+template <>
+__device__ __forceinline__ float finite_in<float>(float x) { return fabsf(x) > 3.402823466e38f ? copysignf(3.402823466e38f, x) : x; }
+template <>
+__device__ __forceinline__ float finite_in<__nv_bfloat16>(float x) { return fabsf(x) > 3.389531390e38f ? copysignf(3.389531390e38f, x) : x; }
+template <>
+__device__ __forceinline__ float finite_in<__half>(float x) { return fabsf(x) > 65504.f ? copysignf(65504.f, x) : x; }
+
+struct Dequant {
+    const uint8_t *values, *scales;
+    void* out;
+    const int32_t* rows_used;  // rows from here on are left alone; null: all rows
+    int64_t rows, row_tiles;   // rows over the whole batch
+    int32_t rows_per, tiles_per, cols, pitch, quads;  // of one matrix of the batch
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kQThreads) dequantize_rows_kernel(const Dequant p) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
+    const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
+    const int64_t n_items = rows * p.quads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQWarps + warp; i < n_items; i += static_cast<int64_t>(gridDim.x) * kQWarps) {
+        const int64_t row = i / p.quads;
+        const int q = static_cast<int>(i - row * p.quads);
+        const int64_t b = row / p.rows_per;
+        const int64_t scale_row = b * p.tiles_per * FP8_TILE_ROWS + (row - b * p.rows_per);
+        const int col0 = q * FP8_QUAD + (lane >> 3) * FP8_BLOCK;
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(p.scales + fp8_scale_word(scale_row, q, p.row_tiles));
+        const float factor = fp8_factor((word >> (8 * (lane >> 3))) & 0xffu);
+        uint32_t w[4];
+        float x[16];
+        load_lane_bytes<T>(p.values + row * p.pitch, col0, p.pitch, s, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fp8_unpack4(w[j], factor, x + 4 * j);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = finite_in<T>(x[j]);
+        store_lane_block<T>(static_cast<T*>(p.out) + row * p.cols, col0, p.cols, s, x);
+    }
+}
+
+// ---- SwiGLU with 8-bit checkpoints -----------------------------------------------------------------
+// forward:  out = up * gate * sigmoid(gate) from the inputs as they came; up and gate are kept in 8 bits, and, for the
+// next 8-bit product, out as well.  backward: from the kept values,
+//   d_up = d * silu(gate),  d_gate = d * up * (s + silu(gate) * (1 - s)),  s = sigmoid(gate).
+// Next to the 16-bit SwiGLU the forward pass writes 2 bytes more per element and the backward reads 2 fewer; what
+// stays alive between the two is half as large.  16-bit results take the approximate exponential and reciprocal
+// (two units in the last place of fp32), fp32 results the full ones.
+template <typename T>
+__device__ __forceinline__ float sigmoid_for(float x) { return sigmoid_clamped_fast(x); }
+template <>
+__device__ __forceinline__ float sigmoid_for<float>(float x) { return sigmoid_clamped(x); }
+
+struct SwigluFp8 {
+    const void *gate, *up, *dy;
+    void *out, *gate_grad, *up_grad;
+    int64_t gate_pitch, up_pitch, dy_pitch, out_pitch, gate_grad_pitch, up_grad_pitch;
+    uint8_t *gate8, *gate_scales, *up8, *up_scales, *out8, *out_scales;
+    const int32_t* rows_used;
+    int64_t rows, row_tiles;
+    int32_t cols, pitch, quads;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kQThreads) swiglu_fp8_forward_kernel(const SwigluFp8 p) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
+    const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
+    const int64_t n_items = rows * p.quads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQWarps + warp; i < n_items; i += static_cast<int64_t>(gridDim.x) * kQWarps) {
+        const int64_t row = i / p.quads;
+        const int q = static_cast<int>(i - row * p.quads);
+        const int col0 = q * FP8_QUAD + (lane >> 3) * FP8_BLOCK;
+        const int64_t scale_at = fp8_scale_word(row, q, p.row_tiles);
+        float g[16], u[16];
+        load_lane_block<T>(static_cast<const T*>(p.gate) + row * p.gate_pitch, col0, p.cols, s, g);
+        load_lane_block<T>(static_cast<const T*>(p.up) + row * p.up_pitch, col0, p.cols, s, u);
+        uint32_t w[4];
+        if (p.gate8 != nullptr) {
+            const uint32_t word = quantize_lane_block(g, w);
+            store_lane_bytes<T>(p.gate8 + row * p.pitch, col0, p.pitch, s, w);
+            if (lane == 0) *reinterpret_cast<uint32_t*>(p.gate_scales + scale_at) = word;
+        }
+        if (p.up8 != nullptr) {
+            const uint32_t word = quantize_lane_block(u, w);
+            store_lane_bytes<T>(p.up8 + row * p.pitch, col0, p.pitch, s, w);
+            if (lane == 0) *reinterpret_cast<uint32_t*>(p.up_scales + scale_at) = word;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) u[j] = u[j] * g[j] * sigmoid_for<T>(g[j]);
+        if (p.out != nullptr) store_lane_block<T>(static_cast<T*>(p.out) + row * p.out_pitch, col0, p.cols, s, u);
+        if (p.out8 != nullptr) {  // from the rounded values: what a separate quantisation of `out` gives
+#pragma unroll
+            for (int j = 0; j < 16; ++j) u[j] = Elem<T>::round(u[j]);
+            const uint32_t word = quantize_lane_block(u, w);
+            store_lane_bytes<T>(p.out8 + row * p.pitch, col0, p.pitch, s, w);
+            if (lane == 0) *reinterpret_cast<uint32_t*>(p.out_scales + scale_at) = word;
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kQThreads) swiglu_fp8_backward_kernel(const SwigluFp8 p) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
+    const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
+    const int64_t n_items = rows * p.quads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQWarps + warp; i < n_items; i += static_cast<int64_t>(gridDim.x) * kQWarps) {
+        const int64_t row = i / p.quads;
+        const int q = static_cast<int>(i - row * p.quads);
+        const int col0 = q * FP8_QUAD + (lane >> 3) * FP8_BLOCK;
+        const int64_t scale_at = fp8_scale_word(row, q, p.row_tiles);
+        uint32_t wg[4], wu[4];
+        float d[16], g[16], u[16];
+        load_lane_bytes<T>(p.gate8 + row * p.pitch, col0, p.pitch, s, wg);
+        load_lane_bytes<T>(p.up8 + row * p.pitch, col0, p.pitch, s, wu);
+        load_lane_block<T>(static_cast<const T*>(p.dy) + row * p.dy_pitch, col0, p.cols, s, d);
+        const int shift = 8 * (lane >> 3);
+        const float fg = fp8_factor((*reinterpret_cast<const uint32_t*>(p.gate_scales + scale_at) >> shift) & 0xffu);
+        const float fu = fp8_factor((*reinterpret_cast<const uint32_t*>(p.up_scales + scale_at) >> shift) & 0xffu);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            fp8_unpack4(wg[j], fg, g + 4 * j);
+            fp8_unpack4(wu[j], fu, u + 4 * j);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float sg = sigmoid_for<T>(g[j]);
+            const float silu = g[j] * sg;
+            const float dg = d[j] * u[j] * (sg + silu * (1.f - sg));
+            u[j] = d[j] * silu;
+            g[j] = dg;
+        }
+        store_lane_block<T>(static_cast<T*>(p.gate_grad) + row * p.gate_grad_pitch, col0, p.cols, s, g);
+        store_lane_block<T>(static_cast<T*>(p.up_grad) + row * p.up_grad_pitch, col0, p.cols, s, u);
+    }
+}
+
+// ---- maps of rows that are grouped by expert without alignment -------------------------------------
+// One block.  offsets[e] = first source row of expert e, limited to the rows there are (a count that overshoots is cut
+// off, never followed); pad_offsets[e] = first row of e in the 256-aligned layout; per 128-row tile of the layout the
+// expert, the first source row and the number of source rows.  Source rows behind the last expert's are a group of
+// their own with expert -2: the product writes zeros for them.  Tiles behind the last used one have expert -1.
+constexpr int kMapThreads = 1024;
+struct GroupMaps {
+    const void* counts;
+    int32_t *offsets, *pad_offsets, *tile_expert, *tile_row, *tile_rows;
+    int64_t rows;
+    int32_t index_bytes, E, n_tiles;
+};
+
+__global__ void __launch_bounds__(kMapThreads) group_maps_kernel(const GroupMaps p) {
+    __shared__ int32_t off[1024 + 2], pad[1024 + 3];
+    __shared__ long long scan[kMapThreads];
+    const int t = threadIdx.x;
+    long long c = 0;
+    if (t < p.E) {
+        c = p.index_bytes == 8 ? static_cast<const long long*>(p.counts)[t]
+                               : static_cast<long long>(static_cast<const int32_t*>(p.counts)[t]);
+        c = c < 0 ? 0 : (c > p.rows ? p.rows : c);
+    }
+    scan[t] = c;
+    __syncthreads();
+    for (int d = 1; d < kMapThreads; d <<= 1) {
+        const long long add = t >= d ? scan[t - d] : 0;
+        __syncthreads();
+        scan[t] += add;
+        __syncthreads();
+    }
+    // group E: the rows of no expert
+    if (t < p.E) off[t + 1] = static_cast<int32_t>(min(scan[t], static_cast<long long>(p.rows)));
+    if (t == 0) off[0] = 0;
+    __syncthreads();
+    const int n = p.E;  // groups 0..n-1 are experts, n is the rest
+    long long tiles = 0;
+    if (t < n) tiles = (off[t + 1] - off[t] + 255) / 256;
+    scan[t] = tiles;
+    __syncthreads();
+    for (int d = 1; d < kMapThreads; d <<= 1) {
+        const long long add = t >= d ? scan[t - d] : 0;
+        __syncthreads();
+        scan[t] += add;
+        __syncthreads();
+    }
+    if (t < n) pad[t + 1] = static_cast<int32_t>(scan[t] * 256);
+    if (t == 0) pad[0] = 0;
+    __syncthreads();
+    const int32_t rest = static_cast<int32_t>(p.rows) - off[n];
+    if (t == 0) pad[n + 1] = pad[n] + (rest + 255) / 256 * 256;
+    __syncthreads();
+    if (t <= n) {
+        p.offsets[t] = off[t];
+        p.pad_offsets[t] = pad[t];
+    }
+    if (t == 0) p.pad_offsets[n + 1] = pad[n + 1];
+    for (int i = t; i < p.n_tiles; i += kMapThreads) {
+        const int32_t row = i * 128;
+        int32_t e = -1, first = 0, count = 0;
+        if (row < pad[n + 1]) {
+            int lo = 0, hi = n + 1;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (pad[mid] <= row) lo = mid; else hi = mid;
+            }
+            const int32_t inside = row - pad[lo];
+            const int32_t size = lo < n ? off[lo + 1] - off[lo] : rest;
+            first = off[lo] + inside;
+            count = max(0, min(128, size - inside));
+            e = lo < n ? lo : -2;
+        }
+        p.tile_expert[i] = e;
+        p.tile_row[i] = first;
+        p.tile_rows[i] = count;
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------
+static int64_t row_grid(int64_t items) {
+    const int64_t want = (items + kQWarps - 1) / kQWarps;
+    const int64_t cap = static_cast<int64_t>(sm_count()) * 64;
+    return want < 1 ? 1 : (want > cap ? cap : want);
+}
+
+static int check_rows_cols(int32_t dtype, int64_t rows, int64_t cols) {
+    FMAB_REQUIRE(known_dtype(dtype), FMA_B200_ERR_UNSUPPORTED, "dtype %d", dtype);
+    FMAB_REQUIRE(rows >= 0 && rows < (1LL << 31), FMA_B200_ERR_BAD_ARG, "rows=%lld not in [0, 2^31)", (long long)rows);
+    FMAB_REQUIRE(cols >= 8 && cols % 8 == 0 && cols < (1LL << 30), FMA_B200_ERR_BAD_ARG,
+                 "cols=%lld must be a positive multiple of 8 below 2^30", (long long)cols);
+    return FMA_B200_OK;
+}
+static int check_pitch(const char* what, int32_t dtype, int64_t pitch, int64_t cols) {
+    FMAB_REQUIRE(pitch >= cols && pitch % elems_per_16_bytes(dtype) == 0, FMA_B200_ERR_BAD_ARG,
+                 "%s: row pitch %lld is below the width or not a multiple of 16 bytes", what, (long long)pitch);
+    return FMA_B200_OK;
+}
+
+template <int TO>
+static int launch_quantize(QuantRows& p, int32_t dtype, int64_t extra_rows, cudaStream_t s) {
+    p.row_blocks = row_grid(p.rows * p.quads);
+    int64_t grid = p.row_blocks;
+    if (TO != TO_ROWS) grid += row_grid(extra_rows);
+    dispatch_dtype(dtype, [&](auto tag) {
+        quantize_rows_kernel<decltype(tag), TO><<<static_cast<unsigned>(grid), kQThreads, 0, s>>>(p);
+    });
+    return check_launch("fp8_quantize");
+}
+
+static int fill_quantize(QuantRows& p, const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols,
+                         int64_t layout_rows, void* values, void* scales) {
+    if (int rc = check_rows_cols(dtype, rows, cols)) return rc;
+    if (int rc = check_rows_cols(dtype, layout_rows, cols)) return rc;
+    if (int rc = check_pitch("x", dtype, x_pitch, cols)) return rc;
+    memset(&p, 0, sizeof(p));
+    p.x = x;
+    p.x_pitch = x_pitch;
+    p.rows = rows;
+    p.layout_rows = layout_rows;
+    p.row_tiles = fp8_row_tiles(layout_rows);
+    p.cols = static_cast<int32_t>(cols);
+    p.pitch = static_cast<int32_t>(fp8_pitch(cols));
+    p.quads = static_cast<int32_t>(fp8_quads(cols));
+    p.values = static_cast<uint8_t*>(values);
+    p.scales = static_cast<uint8_t*>(scales);
+    if (rows == 0) return FMA_B200_OK;
+    FMAB_REQUIRE(x && values && scales, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    FMAB_REQUIRE(aligned16(x) && aligned16(values) && aligned16(scales), FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
+    return FMA_B200_OK;
+}
+
+}  // namespace fmab
+
+extern "C" {
+
+int64_t fma_b200_fp8_scale_bytes(int64_t rows, int64_t cols) {
+    if (rows < 0 || cols < 0) return 0;
+    return fmab::fp8_quads(cols) * fmab::fp8_row_tiles(rows) * fmab::FP8_TILE_BYTES;
+}
+
+int fma_b200_fp8_quantize_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols, void* values,
+                               void* scales, void* stream) {
+    using namespace fmab;
+    QuantRows p;
+    if (int rc = fill_quantize(p, x, x_pitch, dtype, rows, cols, rows, values, scales)) return rc;
+    if (rows == 0) return FMA_B200_OK;
+    return launch_quantize<TO_ROWS>(p, dtype, 0, static_cast<cudaStream_t>(stream));
+}
+
+int fma_b200_fp8_quantize_groups(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols,
+                                 const int32_t* offsets, const int32_t* pad_offsets, int32_t E, int64_t layout_rows,
+                                 void* values, void* scales, void* copy, void* stream) {
+    using namespace fmab;
+    QuantRows p;
+    if (int rc = fill_quantize(p, x, x_pitch, dtype, rows, cols, layout_rows, values, scales)) return rc;
+    FMAB_REQUIRE(E >= 1 && E <= 1024, FMA_B200_ERR_BAD_ARG, "E=%d not in [1,1024]", E);
+    if (rows == 0) return FMA_B200_OK;
+    FMAB_REQUIRE(offsets && pad_offsets, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    FMAB_REQUIRE(aligned16(copy), FMA_B200_ERR_BAD_ARG, "copy is not 16-byte aligned");
+    p.copy = copy;
+    p.offsets = offsets;
+    p.pad_offsets = pad_offsets;
+    p.n_groups = E;
+    return launch_quantize<TO_GROUPS>(p, dtype, E * 64LL, static_cast<cudaStream_t>(stream));
+}
+
+int fma_b200_fp8_quantize_scatter(const void* x, int32_t dtype, int64_t T, int64_t cols, int32_t k,
+                                  const int32_t* row_of_slot, const int32_t* slot_of_row, const int32_t* pad_offsets,
+                                  int32_t E, int64_t layout_rows, void* values, void* scales, void* stream) {
+    using namespace fmab;
+    QuantRows p;
+    if (int rc = fill_quantize(p, x, cols, dtype, T, cols, layout_rows, values, scales)) return rc;
+    FMAB_REQUIRE(E >= 1 && k >= 1, FMA_B200_ERR_BAD_ARG, "E=%d, k=%d", E, k);
+    if (T == 0) return FMA_B200_OK;
+    FMAB_REQUIRE(row_of_slot && slot_of_row && pad_offsets, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    p.row_of_slot = row_of_slot;
+    p.slot_of_row = slot_of_row;
+    p.pad_offsets = pad_offsets;
+    p.n_groups = E;
+    p.k = k;
+    return launch_quantize<TO_SLOTS>(p, dtype, E * 64LL, static_cast<cudaStream_t>(stream));
+}
+
+int fma_b200_fp8_quantize_weight(const void* w, int32_t dtype, int32_t E, int32_t N, int32_t K, void* values,
+                                 void* scales, void* values_t, void* scales_t, void* stream) {
+    using namespace fmab;
+    if (int rc = check_rows_cols(dtype, N, K)) return rc;
+    FMAB_REQUIRE(E >= 1 && E <= 1024, FMA_B200_ERR_BAD_ARG, "E=%d not in [1,1024]", E);
+    FMAB_REQUIRE(N >= 8 && N % 8 == 0, FMA_B200_ERR_BAD_ARG, "N=%d must be a positive multiple of 8", N);
+    FMAB_REQUIRE(static_cast<int64_t>(E) * N < (1LL << 31) - 1024 && static_cast<int64_t>(E) * K < (1LL << 31) - 1024,
+                 FMA_B200_ERR_BAD_ARG, "E*N or E*K overflows");
+    FMAB_REQUIRE(w && values && scales && (values_t == nullptr) == (scales_t == nullptr), FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    FMAB_REQUIRE(aligned16(w) && aligned16(values) && aligned16(scales) && aligned16(values_t) && aligned16(scales_t),
+                 FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
+    QuantWeight p;
+    p.w = w;
+    p.values = static_cast<uint8_t*>(values);
+    p.scales = static_cast<uint8_t*>(scales);
+    p.values_t = static_cast<uint8_t*>(values_t);
+    p.scales_t = static_cast<uint8_t*>(scales_t);
+    p.E = E;
+    p.N = N;
+    p.K = K;
+    p.pitch = static_cast<int32_t>(fp8_pitch(K));
+    p.pitch_t = static_cast<int32_t>(fp8_pitch(N));
+    p.n_blocks = (N + FP8_BLOCK - 1) / FP8_BLOCK;
+    p.k_blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+    FMAB_REQUIRE(static_cast<int64_t>(p.n_blocks) * p.k_blocks < (1LL << 31), FMA_B200_ERR_BAD_ARG, "N*K overflows");
+    const dim3 grid(static_cast<unsigned>(p.n_blocks * p.k_blocks), static_cast<unsigned>(E));
+    dispatch_dtype(dtype, [&](auto tag) {
+        quantize_weight_kernel<decltype(tag)><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    });
+    return check_launch("fp8_quantize_weight");
+}
+
+int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batch, int64_t rows, int64_t cols,
+                            const int32_t* rows_used, void* out, int32_t dtype, void* stream) {
+    using namespace fmab;
+    if (int rc = check_rows_cols(dtype, rows, cols)) return rc;
+    FMAB_REQUIRE(batch >= 1 && batch * rows < (1LL << 31), FMA_B200_ERR_BAD_ARG, "batch=%d", batch);
+    if (rows == 0) return FMA_B200_OK;
+    FMAB_REQUIRE(values && scales && out, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    FMAB_REQUIRE(aligned16(values) && aligned16(scales) && aligned16(out), FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
+    Dequant p;
+    p.values = static_cast<const uint8_t*>(values);
+    p.scales = static_cast<const uint8_t*>(scales);
+    p.out = out;
+    p.rows_used = rows_used;
+    p.rows = batch * rows;
+    p.rows_per = static_cast<int32_t>(rows);
+    p.tiles_per = static_cast<int32_t>(fp8_row_tiles(rows));
+    p.row_tiles = static_cast<int64_t>(batch) * p.tiles_per;
+    p.cols = static_cast<int32_t>(cols);
+    p.pitch = static_cast<int32_t>(fp8_pitch(cols));
+    p.quads = static_cast<int32_t>(fp8_quads(cols));
+    dispatch_dtype(dtype, [&](auto tag) {
+        dequantize_rows_kernel<decltype(tag)><<<static_cast<unsigned>(row_grid(p.rows * p.quads)), kQThreads, 0,
+                                                static_cast<cudaStream_t>(stream)>>>(p);
+    });
+    return check_launch("fp8_dequantize");
+}
+
+int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, int64_t rows, int64_t layout_rows,
+                            int32_t* offsets, int32_t* pad_offsets, int32_t* tile_expert, int32_t* tile_row,
+                            int32_t* tile_rows, void* stream) {
+    using namespace fmab;
+    FMAB_REQUIRE(index_bytes == 4 || index_bytes == 8, FMA_B200_ERR_UNSUPPORTED, "index_bytes=%d", index_bytes);
+    FMAB_REQUIRE(E >= 1 && E <= kMapThreads, FMA_B200_ERR_BAD_ARG, "E=%d not in [1,1024]", E);
+    FMAB_REQUIRE(rows >= 0 && layout_rows % 256 == 0 && layout_rows < (1LL << 31) &&
+                     layout_rows >= (rows + 255) / 256 * 256 + 256LL * (E < rows ? E : rows),
+                 FMA_B200_ERR_BAD_ARG, "layout_rows=%lld is too small for %lld rows of %d experts", (long long)layout_rows,
+                 (long long)rows, E);
+    FMAB_REQUIRE(counts && offsets && pad_offsets && tile_expert && tile_row && tile_rows, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    GroupMaps p;
+    p.counts = counts;
+    p.index_bytes = index_bytes;
+    p.E = E;
+    p.rows = rows;
+    p.n_tiles = static_cast<int32_t>(layout_rows / 128);
+    p.offsets = offsets;
+    p.pad_offsets = pad_offsets;
+    p.tile_expert = tile_expert;
+    p.tile_row = tile_row;
+    p.tile_rows = tile_rows;
+    group_maps_kernel<<<1, kMapThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return check_launch("fp8_group_maps");
+}
+
+int fma_b200_swiglu_fp8_forward(const void* gate, int64_t gate_pitch, const void* up, int64_t up_pitch, void* out,
+                                int64_t out_pitch, int32_t dtype, int64_t rows, int64_t cols, const int32_t* rows_used,
+                                void* gate8, void* gate_scales, void* up8, void* up_scales, void* out8, void* out_scales,
+                                void* stream) {
+    using namespace fmab;
+    if (int rc = check_rows_cols(dtype, rows, cols)) return rc;
+    if (int rc = check_pitch("gate", dtype, gate_pitch, cols)) return rc;
+    if (int rc = check_pitch("up", dtype, up_pitch, cols)) return rc;
+    if (out != nullptr)
+        if (int rc = check_pitch("out", dtype, out_pitch, cols)) return rc;
+    FMAB_REQUIRE((gate8 == nullptr) == (gate_scales == nullptr) && (up8 == nullptr) == (up_scales == nullptr) &&
+                     (out8 == nullptr) == (out_scales == nullptr),
+                 FMA_B200_ERR_BAD_ARG, "8-bit values and their scales come together");
+    if (rows == 0) return FMA_B200_OK;
+    FMAB_REQUIRE(gate && up, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    const void* all[9] = {gate, up, out, gate8, gate_scales, up8, up_scales, out8, out_scales};
+    for (const void* ptr : all) FMAB_REQUIRE(aligned16(ptr), FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
+    SwigluFp8 p;
+    memset(&p, 0, sizeof(p));
+    p.gate = gate;
+    p.up = up;
+    p.out = out;
+    p.gate_pitch = gate_pitch;
+    p.up_pitch = up_pitch;
+    p.out_pitch = out_pitch;
+    p.gate8 = static_cast<uint8_t*>(gate8);
+    p.gate_scales = static_cast<uint8_t*>(gate_scales);
+    p.up8 = static_cast<uint8_t*>(up8);
+    p.up_scales = static_cast<uint8_t*>(up_scales);
+    p.out8 = static_cast<uint8_t*>(out8);
+    p.out_scales = static_cast<uint8_t*>(out_scales);
+    p.rows_used = rows_used;
+    p.rows = rows;
+    p.row_tiles = fp8_row_tiles(rows);
+    p.cols = static_cast<int32_t>(cols);
+    p.pitch = static_cast<int32_t>(fp8_pitch(cols));
+    p.quads = static_cast<int32_t>(fp8_quads(cols));
+    dispatch_dtype(dtype, [&](auto tag) {
+        swiglu_fp8_forward_kernel<decltype(tag)><<<static_cast<unsigned>(row_grid(rows * p.quads)), kQThreads, 0,
+                                                   static_cast<cudaStream_t>(stream)>>>(p);
+    });
+    return check_launch("swiglu_fp8_forward");
+}
+
+int fma_b200_swiglu_fp8_backward(const void* gate8, const void* gate_scales, const void* up8, const void* up_scales,
+                                 const void* dy, int64_t dy_pitch, void* gate_grad, int64_t gate_grad_pitch,
+                                 void* up_grad, int64_t up_grad_pitch, int32_t dtype, int64_t rows, int64_t cols,
+                                 const int32_t* rows_used, void* stream) {
+    using namespace fmab;
+    if (int rc = check_rows_cols(dtype, rows, cols)) return rc;
+    if (int rc = check_pitch("dy", dtype, dy_pitch, cols)) return rc;
+    if (int rc = check_pitch("gate_grad", dtype, gate_grad_pitch, cols)) return rc;
+    if (int rc = check_pitch("up_grad", dtype, up_grad_pitch, cols)) return rc;
+    if (rows == 0) return FMA_B200_OK;
+    const void* all[7] = {gate8, gate_scales, up8, up_scales, dy, gate_grad, up_grad};
+    for (const void* ptr : all)
+        FMAB_REQUIRE(ptr != nullptr && aligned16(ptr), FMA_B200_ERR_BAD_ARG, "pointer NULL or not 16-byte aligned");
+    SwigluFp8 p;
+    memset(&p, 0, sizeof(p));
+    p.dy = dy;
+    p.dy_pitch = dy_pitch;
+    p.gate_grad = gate_grad;
+    p.gate_grad_pitch = gate_grad_pitch;
+    p.up_grad = up_grad;
+    p.up_grad_pitch = up_grad_pitch;
+    p.gate8 = static_cast<uint8_t*>(const_cast<void*>(gate8));
+    p.gate_scales = static_cast<uint8_t*>(const_cast<void*>(gate_scales));
+    p.up8 = static_cast<uint8_t*>(const_cast<void*>(up8));
+    p.up_scales = static_cast<uint8_t*>(const_cast<void*>(up_scales));
+    p.rows_used = rows_used;
+    p.rows = rows;
+    p.row_tiles = fp8_row_tiles(rows);
+    p.cols = static_cast<int32_t>(cols);
+    p.pitch = static_cast<int32_t>(fp8_pitch(cols));
+    p.quads = static_cast<int32_t>(fp8_quads(cols));
+    dispatch_dtype(dtype, [&](auto tag) {
+        swiglu_fp8_backward_kernel<decltype(tag)><<<static_cast<unsigned>(row_grid(rows * p.quads)), kQThreads, 0,
+                                                    static_cast<cudaStream_t>(stream)>>>(p);
+    });
+    return check_launch("swiglu_fp8_backward");
+}
+
+}  // extern "C"

@@ -111,6 +111,17 @@ int fma_b200_moe_gemm_wgrad(const void* dY, const void* X, void* dW, int32_t dty
     return simt_wgrad(dY, X, dW, rows_cap, E, OUT, IN, seg_offsets, n_seg, s);
 }
 
+int fma_b200_linear_wgrad(const void* dY, const void* X, void* dW, int32_t dtype, int64_t rows, int32_t E, int32_t OUT,
+                          int32_t IN, const int32_t* seg_offsets, void* stream) {
+    using namespace fmab;
+    FMAB_REQUIRE(dtype == FMA_B200_BF16 || dtype == FMA_B200_F16, FMA_B200_ERR_UNSUPPORTED, "dtype %d", dtype);
+    FMAB_REQUIRE(rows >= 1, FMA_B200_ERR_BAD_ARG, "rows=%lld", (long long)rows);
+    if (int rc = check_layer_gemm(dtype, (rows + 127) / 128 * 128, E, OUT, IN)) return rc;
+    FMAB_REQUIRE(dW && seg_offsets && dY && X, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    FMAB_REQUIRE(aligned16(dY) && aligned16(X) && aligned16(dW), FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
+    return tc2_wgrad(dY, X, dW, rows, E, OUT, IN, seg_offsets, 1, dtype == FMA_B200_F16, static_cast<cudaStream_t>(stream));
+}
+
 int fma_b200_moe_gemm_forward_swiglu(const void* X, const void* W, void* pre, void* act, int32_t dtype,
                                      int64_t rows_cap, int32_t E, int32_t I, int32_t IN, const int32_t* mtile_expert,
                                      int32_t row_align, void* stream) {

@@ -8,7 +8,21 @@ C ABI (see include/fma_b200.h); there is no Triton, eager-PyTorch or CPU fallbac
 from . import _native
 from .kernel_backend import KernelBackend
 from .modules import Experts, ExpertParallelMoE, MoE, shard_expert_state_dict, unshard_expert_state_dicts
-from .ops import continuous_count, grouped_gemm, pack_sequence, swiglu, swiglu_packed, unpack_sequence
+from .ops import (
+    Fp8Blocks,
+    Fp8Weight,
+    continuous_count,
+    grouped_gemm,
+    grouped_linear_fp8,
+    linear_fp8,
+    pack_sequence,
+    quantize_fp8,
+    quantize_fp8_weight,
+    swiglu,
+    swiglu_fp8_checkpoint,
+    swiglu_packed,
+    unpack_sequence,
+)
 from .utils import ceil_divide, ensure_contiguous, set_seed
 
 __all__ = [
@@ -24,6 +38,13 @@ __all__ = [
     "swiglu_packed",
     "pack_sequence",
     "unpack_sequence",
+    "Fp8Blocks",
+    "Fp8Weight",
+    "quantize_fp8",
+    "quantize_fp8_weight",
+    "linear_fp8",
+    "grouped_linear_fp8",
+    "swiglu_fp8_checkpoint",
     "ensure_contiguous",
     "set_seed",
     "ceil_divide",

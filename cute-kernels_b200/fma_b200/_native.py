@@ -77,8 +77,28 @@ SIGNATURES: dict[str, tuple] = {
     "fma_b200_moe_gemm_wgrad": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _I32, _P]),
     "fma_b200_moe_gemm_forward_swiglu": (ctypes.c_int, [_P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _I32, _P]),
     "fma_b200_moe_gemm_dgrad_swiglu": (ctypes.c_int, [_P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _I32, _P]),
+    "fma_b200_linear_wgrad": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P]),
     "fma_b200_grouped_gemm_workspace_bytes": (_I64, [_I32, _I64]),
     "fma_b200_grouped_gemm": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P, _I64, _P]),
+    "fma_b200_fp8_scale_bytes": (_I64, [_I64, _I64]),
+    "fma_b200_fp8_quantize_rows": (ctypes.c_int, [_P, _I64, _I32, _I64, _I64, _P, _P, _P]),
+    "fma_b200_fp8_quantize_groups": (ctypes.c_int, [_P, _I64, _I32, _I64, _I64, _P, _P, _I32, _I64, _P, _P, _P, _P]),
+    "fma_b200_fp8_quantize_scatter": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _P, _P, _P, _I32, _I64, _P, _P, _P]),
+    "fma_b200_fp8_quantize_weight": (ctypes.c_int, [_P, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P]),
+    "fma_b200_fp8_dequantize": (ctypes.c_int, [_P, _P, _I32, _I64, _I64, _P, _P, _I32, _P]),
+    "fma_b200_fp8_group_maps": (ctypes.c_int, [_P, _I32, _I32, _I64, _I64, _P, _P, _P, _P, _P, _P]),
+    "fma_b200_fp8_gemm": (
+        ctypes.c_int,
+        [_P, _P, _I64, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _P, _P],
+    ),
+    "fma_b200_swiglu_fp8_forward": (
+        ctypes.c_int,
+        [_P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P],
+    ),
+    "fma_b200_swiglu_fp8_backward": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _P, _P],
+    ),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -111,6 +131,7 @@ KERNELS_PER_CALL = {
     "fma_b200_moe_sort": 3, "fma_b200_moe_sort_routed": 2, "fma_b200_device_status": 0, "fma_b200_device_status_peek": 0, "fma_b200_set_sm_limit": 0, "fma_b200_peer_buffer_create": 0,
     "fma_b200_peer_buffer_open": 0, "fma_b200_peer_buffer_close": 0, "fma_b200_peer_buffer_destroy": 0,
     "fma_b200_peer_copy": 0,
+    "fma_b200_linear_wgrad": 2,
     "fma_b200_moe_gemm_wgrad": 2,  # expert order + GEMM for the 16-bit types (one kernel for fp32)
 }  # fmt: skip
 launch_count = 0  # kernels launched through this binding since import (a plain counter for benchmarks)

@@ -358,6 +358,13 @@ int fma_b200_moe_gemm_dgrad(const void* dY, const void* W, void* dX, int32_t dty
 int fma_b200_moe_gemm_wgrad(const void* dY, const void* X, void* dW, int32_t dtype, int64_t rows_cap, int32_t E,
                             int32_t OUT, int32_t IN, const int32_t* seg_offsets, int32_t n_seg, void* stream);
 /*
+ * fma_b200_moe_gemm_wgrad (16-bit types, one segment per expert) for any number of rows: dY and X end at `rows`, and
+ * seg_offsets [E+1] at the rows that count; a plain linear map is E = 1 with {0, rows}.  With several experts each
+ * segment starts on a multiple of 64 rows and its padding rows are zero.
+ */
+int fma_b200_linear_wgrad(const void* dY, const void* X, void* dW, int32_t dtype, int64_t rows, int32_t E, int32_t OUT,
+                          int32_t IN, const int32_t* seg_offsets, void* stream);
+/*
  * Up projection with SwiGLU in the epilogue: W is [E, 2*I, IN] with rows 0..I-1 = up and
  * I..2I-1 = gate (the chunk order of swiglu_packed, fma/ops/swiglu/__init__.py:153).
  * Writes pre[p, 0:2I] = X.W^T rounded to dtype (kept for backward) and
@@ -396,6 +403,80 @@ int64_t fma_b200_grouped_gemm_workspace_bytes(int32_t n_groups, int64_t total_mt
 int fma_b200_grouped_gemm(const void* A, const void* B, void* D, const uint32_t* M, const uint32_t* N,
                           const uint32_t* K, int32_t n_groups, int32_t a_transposed, int32_t b_transposed,
                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ======================================================================= */
+/* 8-bit operands and checkpoints                                            */
+/* ======================================================================= */
+/*
+ * No counterpart in the reference (it has no 8-bit types).  A tensor [rows, cols] is held as e4m3 values
+ * [rows, pitch], pitch = cols rounded up to 16 (the columns from cols on are zero), and one scale 2^e per block of
+ * 128 columns of a row, or of 128 x 128 for weights: e is the smallest integer with amax <= 448 * 2^e over the
+ * block's finite elements (0 for a block of zeros, kept in [-127, 127]), a value is e4m3(x * 2^-e) rounded to
+ * nearest even.  Infinities and NaN become NaN.  Scales are bytes e + 127 in tiles of 512 bytes, one tile per 128
+ * rows and 512 columns, tile (q, t) at (q * ceil(rows/128) + t) * 512 and inside it the byte of (row, k-block b) at
+ * (row % 32) * 16 + (row / 32 % 4) * 4 + b % 4; fma_b200_fp8_scale_bytes(rows, cols) is the size of the array.
+ * cols is a multiple of 8, pitches are in elements and whole multiples of 16 bytes, pointers 16-byte aligned.
+ *
+ * quantize_rows      x [rows, cols] (row pitch x_pitch) -> values, scales, blocks of 1 x 128
+ * quantize_groups    the same for rows that are grouped by expert without alignment: source rows
+ *                    [offsets[e], offsets[e+1]) go to layout rows pad_offsets[e].. ; the padding rows below
+ *                    pad_offsets[E] become zeros; source rows from offsets[E] on are left out.  copy (may be NULL)
+ *                    receives the rows themselves, unquantised, in the same layout [layout_rows, cols].
+ * quantize_scatter   token t goes to the k rows row_of_slot[t*k..] of the layout of fma_b200_moe_sort (negative:
+ *                    nowhere), padding rows below pad_offsets[E] become zeros: fma_b200_moe_scatter in 8 bits
+ * quantize_weight    w [E, N, K] -> values [E, N, pitch(K)] and scales of 128 x 128 blocks; with values_t also the
+ *                    transposed copy [E, K, pitch(N)].  Scale tiles count ceil(N/128) (transposed: ceil(K/128))
+ *                    row tiles per expert, so their size is scale_bytes(E * ceil(N/128) * 128, K)
+ * dequantize         batch matrices [rows, cols] with 1 x 128 or 128 x 128 blocks -> out, contiguous; what a rounding
+ *                    to e4m3 lifted above the type's range becomes its largest finite value.  rows_used (device,
+ *                    may be NULL): rows from *rows_used on are not touched.
+ */
+int64_t fma_b200_fp8_scale_bytes(int64_t rows, int64_t cols);
+int fma_b200_fp8_quantize_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols, void* values,
+                               void* scales, void* stream);
+int fma_b200_fp8_quantize_groups(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols,
+                                 const int32_t* offsets, const int32_t* pad_offsets, int32_t E, int64_t layout_rows,
+                                 void* values, void* scales, void* copy, void* stream);
+int fma_b200_fp8_quantize_scatter(const void* x, int32_t dtype, int64_t T, int64_t cols, int32_t k,
+                                  const int32_t* row_of_slot, const int32_t* slot_of_row, const int32_t* pad_offsets,
+                                  int32_t E, int64_t layout_rows, void* values, void* scales, void* stream);
+int fma_b200_fp8_quantize_weight(const void* w, int32_t dtype, int32_t E, int32_t N, int32_t K, void* values,
+                                 void* scales, void* values_t, void* scales_t, void* stream);
+int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batch, int64_t rows, int64_t cols,
+                            const int32_t* rows_used, void* out, int32_t dtype, void* stream);
+/*
+ * Maps for rows grouped by expert without alignment: counts [E] (4- or 8-byte integers on the device) rows per
+ * expert, rows = rows there are.  Writes offsets[E+1] (running sums, cut off at `rows`), pad_offsets[E+2] (first row of
+ * each expert in a layout aligned to 256 rows; entry E+1 is the end with the rows of no expert), and for every
+ * 128-row tile of the layout its expert (-1 unused, -2 rows behind the last expert's), first source row and number
+ * of source rows.  layout_rows is a multiple of 256, at least round_up(rows, 256) + 256 * min(E, rows).
+ */
+int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, int64_t rows, int64_t layout_rows,
+                            int32_t* offsets, int32_t* pad_offsets, int32_t* tile_expert, int32_t* tile_row,
+                            int32_t* tile_rows, void* stream);
+/*
+ * out[r, :] = a[r, :] . w[e(r)]^T for 8-bit a [layout_rows, K] (1 x 128 blocks) and w [E, N, K] (128 x 128 blocks),
+ * fp32 sums, out bfloat16 or half with row pitch N.  tile_expert / tile_row / tile_rows as from group_maps (or the
+ * mtile_expert of fma_b200_moe_sort with NULL, NULL); all NULL: one expert, row for row.  Tiles of expert -2 get
+ * zeros.  rows_used (device, may be NULL): layout rows in use.  N and K are multiples of 8.
+ */
+int fma_b200_fp8_gemm(const void* a, const void* a_scales, int64_t layout_rows, const void* w, const void* w_scales,
+                      int32_t E, int32_t N, int32_t K, void* out, int32_t dtype, int64_t out_rows,
+                      const int32_t* tile_expert, const int32_t* tile_row, const int32_t* tile_rows,
+                      const int32_t* rows_used, void* stream);
+/*
+ * SwiGLU that keeps its inputs in 8 bits.  forward: out as fma_b200_swiglu_forward (may be NULL), and with gate8 / up8
+ * / out8 (each may be NULL) the 8-bit form of gate, up and the rounded out in 1 x 128 blocks.  backward:
+ * fma_b200_swiglu_backward on the values that gate8 and up8 stand for.
+ */
+int fma_b200_swiglu_fp8_forward(const void* gate, int64_t gate_pitch, const void* up, int64_t up_pitch, void* out,
+                                int64_t out_pitch, int32_t dtype, int64_t rows, int64_t cols, const int32_t* rows_used,
+                                void* gate8, void* gate_scales, void* up8, void* up_scales, void* out8, void* out_scales,
+                                void* stream);
+int fma_b200_swiglu_fp8_backward(const void* gate8, const void* gate_scales, const void* up8, const void* up_scales,
+                                 const void* dy, int64_t dy_pitch, void* gate_grad, int64_t gate_grad_pitch,
+                                 void* up_grad, int64_t up_grad_pitch, int32_t dtype, int64_t rows, int64_t cols,
+                                 const int32_t* rows_used, void* stream);
 
 /* ======================================================================= */
 /* peer-memory transport of the expert-parallel layer                        */
