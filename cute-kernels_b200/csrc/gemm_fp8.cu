@@ -6,14 +6,27 @@
 //
 // The instruction wants one scale per 32 columns and row; it picks one of the four bytes of a 32-bit tensor-memory
 // word by an index in its descriptor.  With one scale per 128 columns the four bytes hold four consecutive k-blocks:
-// all four MMAs of k-block b use byte b % 4, so scales enter shared memory and tensor memory once per 512 columns
-// (512 bytes per 128 rows) and are never replicated along k.
+// all four MMAs of k-block b use byte b % 4, so scales enter tensor memory once per 512 columns (512 bytes per 128
+// rows) and are never replicated along k.
 //
 // Structure as in gemm_tc2.cu: cluster of two CTAs, one persistent pair per two SMs, warp 0 = TMA producer, warp 1 of
-// the leader = MMA issuer, warps 2-9 = epilogue.  What bounds it is the traffic from L2 to the SMs (an 8-bit MMA
-// consumes its operands in half the time of a 16-bit one), so the pair tile is as wide as tensor memory allows next to
-// the scales: 256 rows x 384 columns (a 256-column and a 128-column accumulator), 80 KB of operands per 25 MFLOP
-// instead of 64 KB per 17 MFLOP with 256 x 256.
+// the leader = MMA issuer, warps 2-9 = epilogue; and warps 10-13 bring the scales from global memory straight into
+// tensor memory (16 bytes per lane are the four rows whose words its lane holds).
+//
+// What bounds it is the tensor pipe, and what the pipe loses it loses to its command stream rather than to loads (the
+// loads alone run at 3.5 PFLOP/s worth of operands).  Measured at 8192 x 4096 x 14336, one change after the other:
+//   scales copied from shared memory with tcgen05.cp, which drains the pipe around it, two accumulators of 256 and 128
+//   columns so that the operands are read least often, no overlap of the epilogue        486 us  1.98 PFLOP/s
+//   one 256 x 256 accumulator (128-column MMAs run below the rate of 256-column ones)     444 us  2.17
+//   scales through tcgen05.st, overlapping accumulators                                    436 us  2.21
+//   one commit for both CTAs' barriers instead of two                                      418 us  2.30
+//   the whole warp walks the loop and an elected lane issues                               365 us  2.64
+//   ring stages of 256 columns: eight MMAs per wait and commit instead of four             324 us  2.97
+// The library's 8-bit product without block scales takes 322 us on the same GPU.
+//
+// The pair tile is 256 rows x up to 256 columns.  Two 256-column accumulators and the scales do not fit into the 512
+// columns of tensor memory, so the accumulators overlap by 32 columns: the epilogue reads the overlap first and hands
+// it back at once, and the next tile's main loop starts while the rest is still being read and stored.
 #include "fp8.cuh"
 #include "gemm_pair.cuh"
 
@@ -21,33 +34,29 @@ namespace fmab {
 
 constexpr int BK8 = 128;                          // reduction elements per stage = one 128-byte swizzle row
 constexpr int UMMA_K8 = 32;
-constexpr int F8_THREADS = 320;
 constexpr int F8_EPI_WARPS = 8;
+constexpr int F8_SCALE_WARPS = 4;
+constexpr int F8_THREADS = 32 * (2 + F8_EPI_WARPS + F8_SCALE_WARPS);
+constexpr int F8_TILE_N = 256;                    // widest tile
 constexpr int F8_A_BYTES = 128 * BK8;             // this CTA's 128 rows
-constexpr int F8_SCALE_SLOT = 2048;               // per stage: 512 bytes for A, 512 per 128 columns for B
-constexpr int F8_PATCH_BYTES = 32 * 128;
+constexpr int F8_B_BYTES = F8_TILE_N / 2 * BK8;   // its half of the tile's columns
+constexpr int F8_STAGE_KB = 2;                    // k-blocks per ring stage
+constexpr int F8_STAGE_BYTES = F8_STAGE_KB * (F8_A_BYTES + F8_B_BYTES);
+constexpr int F8_STAGES = 3;
+constexpr int F8_PATCH_BYTES = 32 * 64;  // 32 rows x 32 columns of 16 bits per epilogue warp
+constexpr size_t F8_SMEM = static_cast<size_t>(F8_STAGES) * F8_STAGE_BYTES + F8_EPI_WARPS * F8_PATCH_BYTES + 1024;
 constexpr int F8_SUPER = 8;                       // pair m-tiles walked together (operand reuse in L2)
-
-// PARTS accumulators: 256 columns, and with two parts 128 more.
-template <int PARTS>
-struct F8Tile {
-    static constexpr int N = PARTS == 2 ? 384 : 256;
-    static constexpr int B_BYTES = N / 2 * BK8;   // this CTA's half of every part
-    static constexpr int STAGE_BYTES = F8_A_BYTES + B_BYTES;
-    static constexpr int STAGES = PARTS == 2 ? 4 : 5;
-    static constexpr int SCALE_TILES = N / 128;
-    static constexpr int SCALE_BYTES = 512 * (1 + SCALE_TILES);
-    static constexpr size_t SMEM = static_cast<size_t>(STAGES) * (STAGE_BYTES + F8_SCALE_SLOT) +
-                                   F8_EPI_WARPS * F8_PATCH_BYTES + 1024;
-};
-constexpr int F8_SCALE_COL = 384;                 // tensor-memory column of the first scale buffer
-constexpr int F8_SCALE_COLS = 16;                 // A: 4 columns, B: 4 per 128 columns
-// A scale buffer is written again four 512-column groups later.  The MMAs that read it last have completed by then:
-// the copy follows a wait for a refilled ring stage (at most 5 k-blocks back) or for an empty accumulator.
-constexpr int F8_SCALE_BUFFERS = 4;
+// tensor memory: accumulator 0 in columns 0-255, accumulator 1 in 224-479, two scale buffers of 12 columns (A: 4,
+// B: 8) from 480 on
+constexpr int F8_ACC1_COL = 224;
+constexpr int F8_SCALE_COL = 480;
+constexpr int F8_SCALE_COLS = 16;
+constexpr int F8_SCALE_BUFFERS = 2;
 
 struct GemmFp8Params {
-    CUtensorMap map_a, map_b0, map_b1, map_sa, map_sb;
+    CUtensorMap map_a, map_b;
+    const uint8_t* a_scales;
+    const uint8_t* b_scales;
     void* out;
     const int32_t* tile_expert;  // per 128-row tile: expert, -1 = unused, -2 = rows of no expert (zeros); null: one expert
     const int32_t* tile_row;     // per 128-row tile: first output row; null: tile * 128
@@ -55,32 +64,32 @@ struct GemmFp8Params {
     const int32_t* rows_used;    // rows of the layout in use (device); null: layout_rows
     int32_t* status;
     int64_t out_rows;
-    int64_t ldd;
     int64_t layout_rows;
     int32_t n_cols, k_blocks, n_ntiles;
-    int32_t b_rows;              // rows of w per expert
-    int32_t sa_tiles;            // scale tiles per quad of A, and of w; of w per expert
-    int32_t sb_tiles, sb_tiles_expert;
+    int32_t tile_n;              // columns per tile: a multiple of 16, at most 256
+    int32_t a_tiles;             // scale tiles per quad of a
+    int32_t b_tiles, b_tiles_expert;  // scale tiles per quad of w, and of one expert
     int32_t f16;
 };
 
-__device__ __forceinline__ uint64_t f8_operand_desc(uint32_t addr) {  // K-major, 128-byte swizzle
-    return make_smem_desc<false>(addr);
-}
-// 32 rows x 16 bytes without swizzle: 8-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t f8_scale_desc(uint32_t addr) {
-    return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (8ull << 16) | (8ull << 32) | (1ull << 46);
-}
-__device__ __forceinline__ void tc_copy_scales_pair(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
+// Issued by one elected lane of a converged warp.
 __device__ __forceinline__ void tc_mma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                                uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+// One commit that arrives on the barrier at this offset in both CTAs.
+__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+        ::"r"(bar), "h"(static_cast<uint16_t>(3))
         : "memory");
 }
 // M = 256, e4m3 operands, ue8m0 scales; scale_byte = which byte of the scale words.
@@ -88,17 +97,20 @@ __device__ __forceinline__ uint32_t f8_instr_desc(int n, uint32_t scale_byte) {
     return (scale_byte << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(256 >> 4) << 24) |
            (scale_byte << 29);
 }
+__device__ __forceinline__ void tc_store_4(uint32_t taddr, uint4 v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                 : "memory");
+}
 
 struct F8PairTile {
     int32_t expert;
     int32_t a_row;       // this CTA's first row of A
     int32_t n0;
-    int32_t parts;       // parts with columns
     int32_t rows;        // output rows of this CTA
     int64_t out_row;
 };
 
-template <int PARTS>
 __device__ __forceinline__ bool f8_decode(const GemmFp8Params& p, int tile, int n_pairs_m, uint32_t rank, F8PairTile& t) {
     const int per_super = F8_SUPER * p.n_ntiles;
     const int super = tile / per_super;
@@ -111,24 +123,21 @@ __device__ __forceinline__ bool f8_decode(const GemmFp8Params& p, int tile, int 
     t.expert = p.tile_expert != nullptr ? __ldg(p.tile_expert + 2 * pm) : 0;
     if (t.expert == -1) return false;
     t.a_row = mt * 128;
-    t.n0 = nt * F8Tile<PARTS>::N;
-    t.parts = (PARTS == 2 && t.n0 + 256 < p.n_cols) ? 2 : 1;
+    t.n0 = nt * p.tile_n;
     t.out_row = p.tile_row != nullptr ? __ldg(p.tile_row + mt) : static_cast<int64_t>(mt) * 128;
     const int64_t left = p.tile_rows != nullptr ? __ldg(p.tile_rows + mt) : p.out_rows - t.out_row;
     t.rows = static_cast<int32_t>(left < 0 ? 0 : (left > 128 ? 128 : left));
     return true;
 }
 
-template <int PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8_THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
-    using Tile = F8Tile<PARTS>;
-    constexpr int STAGES = Tile::STAGES;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[STAGES];      // used in the leader only
-    __shared__ __align__(8) uint64_t empty_bar[STAGES];     // each CTA waits on its own copy
-    __shared__ __align__(8) uint64_t acc_full_bar[PARTS];   // each CTA waits on its own copy
-    __shared__ __align__(8) uint64_t acc_empty_bar[PARTS];  // used in the leader only
+    __shared__ __align__(8) uint64_t full_bar[F8_STAGES];            // used in the leader only
+    __shared__ __align__(8) uint64_t empty_bar[F8_STAGES];           // each CTA waits on its own copy
+    __shared__ __align__(8) uint64_t acc_full_bar[2];                // each CTA waits on its own copy
+    __shared__ __align__(8) uint64_t acc_empty_bar;                  // used in the leader only
+    __shared__ __align__(8) uint64_t scale_full_bar[F8_SCALE_BUFFERS];  // used in the leader only
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
 
@@ -137,19 +146,18 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t scale_ring = ring + STAGES * Tile::STAGE_BYTES;
-    const uint32_t patches = scale_ring + STAGES * F8_SCALE_SLOT;
+    const uint32_t patches = ring + F8_STAGES * F8_STAGE_BYTES;
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < F8_STAGES; ++s) {
             mbar_init(smem_u32(&full_bar[s]), 1);
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
-        for (int b = 0; b < PARTS; ++b) {
-            mbar_init(smem_u32(&acc_full_bar[b]), 1);
-            mbar_init(smem_u32(&acc_empty_bar[b]), 2 * F8_EPI_WARPS);  // every epilogue warp of both CTAs
-        }
+        mbar_init(smem_u32(&acc_full_bar[0]), 1);
+        mbar_init(smem_u32(&acc_full_bar[1]), 1);
+        mbar_init(smem_u32(&acc_empty_bar), 2 * F8_EPI_WARPS);  // every epilogue warp of both CTAs
+        for (int b = 0; b < F8_SCALE_BUFFERS; ++b) mbar_init(smem_u32(&scale_full_bar[b]), 2 * F8_SCALE_WARPS);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -178,33 +186,26 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
             int stage = 0;
             uint32_t phase = 0;
             bool alive = true;
+            const uint32_t kb_bytes = F8_A_BYTES + p.tile_n / 2 * BK8;
             for (int tile = pair_id; tile < total_tiles && alive; tile += n_pairs) {
                 F8PairTile t;
-                if (!f8_decode<PARTS>(p, tile, n_pairs_m, rank, t) || t.expert < 0) continue;
-                const int b_row = t.expert * p.b_rows + t.n0;
-                const int sb_tile = t.expert * p.sb_tiles_expert + t.n0 / 128;
-                const uint32_t operand_bytes = F8_A_BYTES + (t.parts == 2 ? Tile::B_BYTES : 128 * BK8);
-                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                if (!f8_decode(p, tile, n_pairs_m, rank, t) || t.expert < 0) continue;
+                const int b_row = t.expert * p.n_cols + t.n0 + static_cast<int>(rank) * (p.tile_n / 2);
+                for (int kb = 0; kb < p.k_blocks; kb += F8_STAGE_KB) {
                     if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_ptr, p.status)) {
                         alive = false;
                         break;
                     }
-                    const bool scales = (kb & 3) == 0;
+                    const int n_kb = min(F8_STAGE_KB, p.k_blocks - kb);
                     const uint32_t leader_bar = map_to_rank(smem_u32(&full_bar[stage]), 0);
-                    const uint32_t sa = ring + stage * Tile::STAGE_BYTES;
-                    const uint32_t sb = sa + F8_A_BYTES;
-                    if (leader)
-                        mbar_arrive_expect_tx(smem_u32(&full_bar[stage]), 2 * (operand_bytes + (scales ? Tile::SCALE_BYTES : 0)));
-                    if (scales) {
-                        const uint32_t ss = scale_ring + stage * F8_SCALE_SLOT;
-                        tma_load_2d_pair(ss, &p.map_sa, leader_bar, 0, (kb >> 2) * p.sa_tiles + t.a_row / 128);
-                        tma_load_2d_pair(ss + 512, &p.map_sb, leader_bar, 0, (kb >> 2) * p.sb_tiles + sb_tile);
+                    const uint32_t sa = ring + stage * F8_STAGE_BYTES;
+                    const uint32_t sb = sa + F8_STAGE_KB * F8_A_BYTES;
+                    if (leader) mbar_arrive_expect_tx(smem_u32(&full_bar[stage]), 2 * n_kb * kb_bytes);
+                    for (int j = 0; j < n_kb; ++j) {
+                        tma_load_2d_pair(sa + j * F8_A_BYTES, &p.map_a, leader_bar, (kb + j) * BK8, t.a_row);
+                        tma_load_2d_pair(sb + j * F8_B_BYTES, &p.map_b, leader_bar, (kb + j) * BK8, b_row);
                     }
-                    tma_load_2d_pair(sa, &p.map_a, leader_bar, kb * BK8, t.a_row);
-                    tma_load_2d_pair(sb, &p.map_b0, leader_bar, kb * BK8, b_row + static_cast<int>(rank) * 128);
-                    if (t.parts == 2)
-                        tma_load_2d_pair(sb + 128 * BK8, &p.map_b1, leader_bar, kb * BK8, b_row + 256 + static_cast<int>(rank) * 64);
-                    if (++stage == STAGES) {
+                    if (++stage == F8_STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
@@ -216,140 +217,164 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
         }
     } else if (warp == 1) {
         // ------------------------------ MMA issuer (leader CTA only) ------------------------------
-        if (leader && lane == 0) {
+        // The whole warp walks the loop and one elected lane issues: descriptors then live in uniform registers.
+        if (leader) {
             int stage = 0;
             uint32_t phase = 0;
-            uint32_t acc_phase = 0;
-            uint32_t part1_phase = 0;
-            int group = 0;  // 512-column groups so far: scale buffer
+            uint32_t sbuf = 0, sphase = 0;
+            uint32_t n_done = 0;  // tiles so far: accumulator n_done % 2
             bool alive = true;
             for (int tile = pair_id; tile < total_tiles && alive; tile += n_pairs) {
                 F8PairTile t;
-                if (!f8_decode<PARTS>(p, tile, n_pairs_m, rank, t) || t.expert < 0) continue;
-                uint32_t scales = 0;
-                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                if (!f8_decode(p, tile, n_pairs_m, rank, t) || t.expert < 0) continue;
+                // the epilogues have read the columns that this accumulator shares with the previous one
+                if (n_done > 0 && !mbar_wait(smem_u32(&acc_empty_bar), (n_done - 1) & 1u, abort_ptr, p.status)) break;
+                tc_fence_after();
+                const uint32_t acc = tmem_base + (n_done & 1u) * F8_ACC1_COL;
+                for (int kb = 0; kb < p.k_blocks; kb += F8_STAGE_KB) {
+                    if ((kb & 3) == 0 && !mbar_wait(smem_u32(&scale_full_bar[sbuf]), sphase, abort_ptr, p.status)) {
+                        alive = false;
+                        break;
+                    }
                     if (!mbar_wait(smem_u32(&full_bar[stage]), phase, abort_ptr, p.status)) {
                         alive = false;
                         break;
                     }
                     tc_fence_after();
-                    if (kb == 0) {
-                        if (!mbar_wait(smem_u32(&acc_empty_bar[0]), acc_phase ^ 1u, abort_ptr, p.status)) {
-                            alive = false;
-                            break;
-                        }
-                        tc_fence_after();
-                    }
-                    if ((kb & 3) == 0) {
-                        scales = tmem_base + F8_SCALE_COL + (group % F8_SCALE_BUFFERS) * F8_SCALE_COLS;
-                        ++group;
-                        const uint32_t ss = scale_ring + stage * F8_SCALE_SLOT;
+                    const uint32_t scales = tmem_base + F8_SCALE_COL + sbuf * F8_SCALE_COLS;
+                    const uint32_t sa = ring + stage * F8_STAGE_BYTES;
+                    const uint64_t a_desc = make_smem_desc<false>(sa);
+                    const uint64_t b_desc = make_smem_desc<false>(sa + F8_STAGE_KB * F8_A_BYTES);
 #pragma unroll
-                        for (int i = 0; i < 1 + Tile::SCALE_TILES; ++i)
-                            tc_copy_scales_pair(scales + 4 * i, f8_scale_desc(ss + 512 * i));
-                    }
-                    const uint32_t sa = ring + stage * Tile::STAGE_BYTES;
-                    const uint64_t a_desc = f8_operand_desc(sa);
-                    const uint64_t b_desc = f8_operand_desc(sa + F8_A_BYTES);
-                    const uint32_t byte = kb & 3;
-#pragma unroll
-                    for (int ks = 0; ks < BK8 / UMMA_K8; ++ks)
-                        tc_mma_f8_pair(tmem_base, a_desc + ks * (UMMA_K8 >> 4), b_desc + ks * (UMMA_K8 >> 4),
-                                       f8_instr_desc(256, byte), scales, scales + 4, (kb | ks) != 0);
-                    const bool last = kb == p.k_blocks - 1;
-                    if (last && t.parts == 2) tc_commit_pair(smem_u32(&acc_full_bar[0]));
-                    if (PARTS == 2 && t.parts == 2) {
-                        if (kb == 0) {
-                            if (!mbar_wait(smem_u32(&acc_empty_bar[PARTS - 1]), part1_phase ^ 1u, abort_ptr, p.status)) {
-                                alive = false;
-                                break;
-                            }
-                            tc_fence_after();
-                        }
-                        const uint64_t b1_desc = f8_operand_desc(sa + F8_A_BYTES + 128 * BK8);
+                    for (int j = 0; j < F8_STAGE_KB; ++j) {
+                        if (kb + j >= p.k_blocks) continue;
+                        const uint32_t idesc = f8_instr_desc(p.tile_n, (kb + j) & 3);
 #pragma unroll
                         for (int ks = 0; ks < BK8 / UMMA_K8; ++ks)
-                            tc_mma_f8_pair(tmem_base + 256, a_desc + ks * (UMMA_K8 >> 4), b1_desc + ks * (UMMA_K8 >> 4),
-                                           f8_instr_desc(128, byte), scales, scales + 12, (kb | ks) != 0);
+                            tc_mma_f8_pair(acc, a_desc + (j * F8_A_BYTES + ks * UMMA_K8) / 16,
+                                           b_desc + (j * F8_B_BYTES + ks * UMMA_K8) / 16, idesc, scales, scales + 4,
+                                           (kb | j | ks) != 0);
                     }
-                    tc_commit_pair(smem_u32(&empty_bar[stage]));
-                    // the accumulator that is finished last is published last: no signal of this tile is outstanding
-                    // once the epilogues have seen it
-                    if (last) tc_commit_pair(smem_u32(&acc_full_bar[t.parts - 1]));
-                    if (++stage == STAGES) {
+                    tc_commit_both(smem_u32(&empty_bar[stage]));
+                    if ((kb & 3) == 4 - F8_STAGE_KB || kb + F8_STAGE_KB >= p.k_blocks) {
+                        if (++sbuf == F8_SCALE_BUFFERS) {
+                            sbuf = 0;
+                            sphase ^= 1u;
+                        }
+                    }
+                    if (++stage == F8_STAGES) {
                         stage = 0;
                         phase ^= 1u;
                     }
                 }
-                acc_phase ^= 1u;
-                if (t.parts == 2) part1_phase ^= 1u;
+                // published last: once the epilogues have seen it no other signal of the tile is outstanding
+                if (alive) tc_commit_both(smem_u32(&acc_full_bar[n_done & 1u]));
+                ++n_done;
             }
         }
-    } else {
+    } else if (warp < 2 + F8_EPI_WARPS) {
         // ------------------------------ epilogue (both CTAs) ------------------------------
         const int quad = warp & 3;               // tensor-memory lanes this warp may read
-        const int half = (warp - 2) >> 2;        // half of a part's columns
+        const int half = (warp - 2) >> 2;        // columns 0-127 or 128-255 of the tile
         const uint32_t patch = patches + (warp - 2) * F8_PATCH_BYTES;
         const bool f16 = p.f16 != 0;
         uint16_t* const out = static_cast<uint16_t*>(p.out);
-        uint32_t acc_phase[2] = {0, 0};
+        uint32_t n_done = 0;
+        for (int tile = pair_id; tile < total_tiles; tile += n_pairs) {
+            F8PairTile t;
+            if (!f8_decode(p, tile, n_pairs_m, rank, t)) continue;
+            const uint32_t acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + (n_done & 1u) * F8_ACC1_COL;
+            // the 32 columns of the overlap come first: the last ones of accumulator 0, the first ones of 1
+            const bool backwards = half == 1 && (n_done & 1u) == 0;
+            if (t.expert >= 0) {
+                if (!mbar_wait(smem_u32(&acc_full_bar[n_done & 1u]), (n_done >> 1) & 1u, abort_ptr, p.status)) break;
+                tc_fence_after();
+            }
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                const int c0 = half * 128 + (backwards ? 3 - i : i) * 32;
+                float v[32];
+                if (t.expert >= 0) {
+                    if (c0 < p.tile_n) tc_load_32(acc + c0, v);  // columns from tile_n on are never stored
+                    if (i == 0) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_rank(smem_u32(&acc_empty_bar), 0));
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                }
+                if (c0 >= p.tile_n) continue;
+                // through the patch: 32 rows x 64 bytes, written a row per lane, read four lanes to a row
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    st_shared_16(patch + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), pack8(v + 8 * q, f16));
+                __syncwarp();
+                const int cw = c0 + (lane & 3) * 8;
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const int row = it * 8 + (lane >> 2);
+                    const uint4 w = ld_shared_16(patch + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
+                    if (quad * 32 + row < t.rows && cw < p.tile_n && t.n0 + cw < p.n_cols)
+                        st_global_16(out + (t.out_row + quad * 32 + row) * p.n_cols + t.n0 + cw, w);
+                }
+            }
+            if (t.expert >= 0) ++n_done;
+        }
+    } else {
+        // ------------------------------ scales (both CTAs) ------------------------------
+        // All four warps bring the same words, each into its 32 lanes: word j of lane l is row j * 32 + l.  Rows of a
+        // weight block share one word, so a tile may start anywhere in it.
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        // A buffer is free again when the MMAs of two groups ago are complete, which the release of the last ring
+        // stage of that group tells: these warps follow the stage numbers and watch that barrier.  It cannot run a
+        // phase ahead of them, since the MMAs of this group wait for them.
+        constexpr int kStagesPerGroup = 4 / F8_STAGE_KB;
+        uint32_t buf = 0;
+        uint32_t n_stages = 0;              // ring stages up to the end of the previous group
+        uint32_t ends[F8_SCALE_BUFFERS] = {0, 0};  // the same up to the end of the group that used each buffer last
         bool alive = true;
         for (int tile = pair_id; tile < total_tiles && alive; tile += n_pairs) {
             F8PairTile t;
-            if (!f8_decode<PARTS>(p, tile, n_pairs_m, rank, t)) continue;
+            if (!f8_decode(p, tile, n_pairs_m, rank, t) || t.expert < 0) continue;
+            const int a_tile = t.a_row / 128;
+            for (int kb = 0; kb < p.k_blocks; kb += 4) {
+                const int q = kb >> 2;
+                const uint32_t one = 0x01010101u * FP8_SCALE_ONE;
+                uint4 wa = make_uint4(one, one, one, one);
+                if (a_tile < p.a_tiles)
+                    wa = __ldg(reinterpret_cast<const uint4*>(p.a_scales + (static_cast<int64_t>(q) * p.a_tiles + a_tile) * FP8_TILE_BYTES) + lane);
+                uint32_t wb[8];
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-                if (part >= t.parts) continue;
-                constexpr int kMaxLoads = 4;
-                const int loads = part == 0 ? 4 : 2;                 // 32-column loads per warp
-                const int c_first = part * 256 + half * loads * 32;  // accumulator column of this warp's first
-                uint32_t packed[kMaxLoads * 16];
-                if (t.expert >= 0) {
-                    if (!mbar_wait(smem_u32(&acc_full_bar[part]), acc_phase[part], abort_ptr, p.status)) {
+                for (int j = 0; j < 8; ++j) {
+                    const int block = (t.n0 + j * 32 + lane) / FP8_BLOCK;
+                    wb[j] = one;
+                    if (block < p.b_tiles_expert)
+                        wb[j] = __ldg(reinterpret_cast<const uint32_t*>(
+                            p.b_scales + (static_cast<int64_t>(q) * p.b_tiles + t.expert * p.b_tiles_expert + block) * FP8_TILE_BYTES));
+                }
+                if (ends[buf] > 0) {
+                    const uint32_t last = ends[buf] - 1;
+                    if (!mbar_wait(smem_u32(&empty_bar[last % F8_STAGES]), (last / F8_STAGES) & 1u, abort_ptr, p.status)) {
                         alive = false;
                         break;
                     }
-                    acc_phase[part] ^= 1u;
-                    tc_fence_after();
-#pragma unroll
-                    for (int j = 0; j < kMaxLoads; ++j) {
-                        if (j >= loads) continue;
-                        float v[32];
-                        tc_load_32(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + c_first + j * 32, v);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint4 w = pack8(v + 8 * i, f16);
-                            packed[j * 16 + 4 * i] = w.x;
-                            packed[j * 16 + 4 * i + 1] = w.y;
-                            packed[j * 16 + 4 * i + 2] = w.z;
-                            packed[j * 16 + 4 * i + 3] = w.w;
-                        }
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster_relaxed(map_to_rank(smem_u32(&acc_empty_bar[part]), 0));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kMaxLoads * 16; ++i) packed[i] = 0;
                 }
-#pragma unroll
-                for (int j = 0; j < kMaxLoads; j += 2) {  // 64 columns at a time through the patch
-                    if (j >= loads) continue;
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        st_shared_16(patch_addr(patch, lane, i), make_uint4(packed[j * 16 + 4 * i], packed[j * 16 + 4 * i + 1],
-                                                                            packed[j * 16 + 4 * i + 2], packed[j * 16 + 4 * i + 3]));
-                    __syncwarp();
-                    const int col = t.n0 + c_first + j * 32 + (lane & 7) * 8;
-#pragma unroll
-                    for (int it = 0; it < 8; ++it) {
-                        const int row = it * 4 + (lane >> 3);
-                        const uint4 w = ld_shared_16(patch_addr(patch, row, lane & 7));
-                        if (quad * 32 + row < t.rows && col < p.n_cols)
-                            st_global_16(out + (t.out_row + quad * 32 + row) * p.ldd + col, w);
-                    }
-                }
+                n_stages += min(kStagesPerGroup, (p.k_blocks - kb + F8_STAGE_KB - 1) / F8_STAGE_KB);
+                ends[buf] = n_stages;
+                tc_fence_after();
+                __syncwarp();
+                const uint32_t at = tmem_base + lanes + F8_SCALE_COL + buf * F8_SCALE_COLS;
+                tc_store_4(at, wa);
+                tc_store_4(at + 4, make_uint4(wb[0], wb[1], wb[2], wb[3]));
+                tc_store_4(at + 8, make_uint4(wb[4], wb[5], wb[6], wb[7]));
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster_relaxed(map_to_rank(smem_u32(&scale_full_bar[buf]), 0));
+                buf ^= 1u;
             }
         }
     }
@@ -379,38 +404,43 @@ static int encode_bytes(CUtensorMap* map, const void* base, uint64_t inner, uint
     FMAB_REQUIRE(r == CUDA_SUCCESS, FMA_B200_ERR_LAUNCH, "cuTensorMapEncodeTiled (8-bit operand) failed with CUresult %d", (int)r);
     return FMA_B200_OK;
 }
-// Scale tiles as rows of 128 words, boxes of `tiles` rows.
-static int encode_scales(CUtensorMap* map, const void* base, uint64_t n_tiles, uint32_t tiles) {
-    EncodeTiledFn fn = encode_fn();
-    FMAB_REQUIRE(fn != nullptr, FMA_B200_ERR_LAUNCH, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint64_t dims[2] = {FP8_TILE_BYTES / 4, n_tiles};
-    const cuuint64_t strides[1] = {FP8_TILE_BYTES};
-    const cuuint32_t box[2] = {FP8_TILE_BYTES / 4, tiles};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    FMAB_REQUIRE(r == CUDA_SUCCESS, FMA_B200_ERR_LAUNCH, "cuTensorMapEncodeTiled (scales) failed with CUresult %d", (int)r);
-    return FMA_B200_OK;
+// Columns per tile.  Few wide tiles read A least often; but the launch takes as long as its fullest pair of SMs, so
+// where the number of row tiles is known (no experts) the width that makes waves * (width + 24) smallest is taken, 24
+// columns standing for what a tile costs besides its columns: a prompt of up to 256 rows spreads over all SMs (256 x
+// 4096 x 4096: 13.7 us, with 256 columns 15.7; 2048 x 2048 x 1536: 10.7 and 11.6; no difference from two waves on).
+// With experts only the waste at the right edge is known: the tiles share it (520 columns: three tiles of 176, not
+// 256 + 256 + 8).
+static int tile_columns(int64_t layout_rows, int N, bool experts) {
+    const int64_t pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, m = (layout_rows + 255) / 256;
+    const int fewest = (N + F8_TILE_N - 1) / F8_TILE_N;
+    int best = 0;
+    int64_t best_cost = 0;
+    for (int n = fewest; n <= N / 64 + 1; ++n) {
+        const int width = ((N + n - 1) / n + 15) / 16 * 16;
+        const int64_t tiles = (N + width - 1) / width;
+        const int64_t cost = (m * tiles + pairs - 1) / pairs * (width + 24);
+        if (best == 0 || cost < best_cost) {
+            best = width;
+            best_cost = cost;
+        }
+        if (experts || m * n > 16 * pairs) break;  // many waves: the widest tile
+    }
+    return best;
 }
 
-template <int PARTS>
 static int launch_fp8(GemmFp8Params& p, cudaStream_t s) {
-    using Tile = F8Tile<PARTS>;
     static bool configured[64] = {false};  // per device: the attribute applies to the current device only
-    auto kernel = gemm_fp8_kernel<PARTS>;
     const int dev = current_device_slot();
     FMAB_REQUIRE(dev >= 0, FMA_B200_ERR_LAUNCH, "no current CUDA device with an ordinal below 64");
     if (!configured[dev]) {
-        FMAB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tile::SMEM));
+        FMAB_CUDA(cudaFuncSetAttribute(gemm_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F8_SMEM));
         configured[dev] = true;
     }
-    p.n_ntiles = (p.n_cols + Tile::N - 1) / Tile::N;
     const int64_t total = (p.layout_rows + 255) / 256 * p.n_ntiles;
     FMAB_REQUIRE(total < (1LL << 31), FMA_B200_ERR_BAD_ARG, "too many tiles");
     const int64_t max_pairs = sm_count() / 2;
     const int pairs = static_cast<int>(total < max_pairs ? total : max_pairs);
-    kernel<<<2 * pairs, F8_THREADS, Tile::SMEM, s>>>(p);
+    gemm_fp8_kernel<<<2 * pairs, F8_THREADS, F8_SMEM, s>>>(p);
     return check_launch("8-bit grouped GEMM");
 }
 
@@ -446,24 +476,20 @@ int fma_b200_fp8_gemm(const void* a, const void* a_scales, int64_t layout_rows, 
     p.tile_rows = tile_rows;
     p.rows_used = rows_used;
     p.out_rows = out_rows;
-    p.ldd = N;
     p.layout_rows = layout_rows;
     p.n_cols = N;
     p.k_blocks = (K + BK8 - 1) / BK8;
-    p.b_rows = N;
-    p.sa_tiles = static_cast<int32_t>(fp8_row_tiles(layout_rows));
-    p.sb_tiles_expert = static_cast<int32_t>(fp8_row_tiles(N));
-    p.sb_tiles = E * p.sb_tiles_expert;
+    p.tile_n = tile_columns(layout_rows, N, tile_expert != nullptr);
+    p.n_ntiles = (N + p.tile_n - 1) / p.tile_n;
+    p.a_scales = static_cast<const uint8_t*>(a_scales);
+    p.b_scales = static_cast<const uint8_t*>(w_scales);
+    p.a_tiles = static_cast<int32_t>(fp8_row_tiles(layout_rows));
+    p.b_tiles_expert = static_cast<int32_t>(fp8_row_tiles(N));
+    p.b_tiles = E * p.b_tiles_expert;
     p.f16 = dtype == FMA_B200_F16 ? 1 : 0;
-    const int64_t quads = fp8_quads(K);
     if (int rc = encode_bytes(&p.map_a, a, K, layout_rows, fp8_pitch(K), 128)) return rc;
-    if (int rc = encode_bytes(&p.map_b0, w, K, static_cast<uint64_t>(E) * N, fp8_pitch(K), 128)) return rc;
-    if (int rc = encode_bytes(&p.map_b1, w, K, static_cast<uint64_t>(E) * N, fp8_pitch(K), 64)) return rc;
-    if (int rc = encode_scales(&p.map_sa, a_scales, quads * p.sa_tiles, 1)) return rc;
-    const bool wide = N > 256;
-    if (int rc = encode_scales(&p.map_sb, w_scales, quads * p.sb_tiles, wide ? 3 : 2)) return rc;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return wide ? launch_fp8<2>(p, s) : launch_fp8<1>(p, s);
+    if (int rc = encode_bytes(&p.map_b, w, K, static_cast<uint64_t>(E) * N, fp8_pitch(K), p.tile_n / 2)) return rc;
+    return launch_fp8(p, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
