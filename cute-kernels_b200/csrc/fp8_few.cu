@@ -1,0 +1,387 @@
+// The 8-bit product for a few rows (serving single tokens): out[r, :] = x[r, :] . w[e(r)]^T in ONE launch, the rows of x
+// quantised on the way in.  The weights are read once, N * K bytes, and that is what bounds it; up to 16 rows ride along.
+//
+// The weights are the 128-row operand of tcgen05.mma and the tokens its 16 columns, so a tile is 128 weight rows and
+// TMA streams it without any thread touching it.  A cluster of up to eight CTAs shares a tile, each with its part of the
+// reduction (whole groups of 512 columns): 4096 weight rows are only 32 tiles, and every SM has to load for the memory
+// to run at its rate.  The parts are added through distributed shared memory in the order of the ranks.
+// (The same with mma.sync, weights from global memory into registers, ran at 2.5 TB/s where this one reaches more than
+// that: the 8-bit mma.sync costs several times the instructions of the loads.)
+#include "fp8.cuh"
+#include "gemm_pair.cuh"
+
+namespace fmab {
+
+constexpr int kFewThreads = 256;
+constexpr int kFewWarps = kFewThreads / 32;
+constexpr int kFewRows = 16;                          // rows of x per pass over the weights
+constexpr int kFewStages = 4;                         // k-blocks of 128 x 128 bytes in flight
+constexpr int kFewStageBytes = 128 * FP8_BLOCK;
+constexpr int kFewXBytes = kFewRows * FP8_BLOCK;      // rows of x per k-block
+constexpr int kFewScaleCol = 16;                      // tensor memory: accumulator 0-15, then 8 columns per quad
+constexpr int kFewScaleCols = 8;                      // (weights 4, rows of x 1)
+
+struct FewRows {
+    CUtensorMap map_w;
+    const void* x;
+    const uint8_t* w_scales;
+    void* out;
+    const void* counts;  // rows per expert; null: one expert
+    int32_t* status;
+    int64_t x_pitch;
+    int32_t index_bytes, E, rows, N, K, k_blocks, quads, tiles, b_tiles, split, quads_most;
+    uint32_t tmem_cols;
+};
+
+__device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit_elected(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// Expert, first row and number of rows of a chunk of at most 16 rows; experts in order, then the rows of no expert
+// (expert -2).  false: there are fewer chunks.  Counts that overshoot are cut off at p.rows.  Every warp for itself.
+__device__ __forceinline__ bool few_locate(const FewRows& p, int chunk, int& expert, int& row0, int& rows) {
+    const int lane = threadIdx.x & 31;
+    int done_rows = 0, done_chunks = 0;
+    if (p.counts == nullptr) {
+        expert = 0;
+        row0 = chunk * kFewRows;
+        rows = min(kFewRows, p.rows - row0);
+        return rows > 0;
+    }
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+        long long c = 0;
+        if (e0 + lane < p.E)
+            c = p.index_bytes == 8 ? static_cast<const long long*>(p.counts)[e0 + lane]
+                                   : static_cast<long long>(static_cast<const int32_t*>(p.counts)[e0 + lane]);
+        int end = static_cast<int>(c < 0 ? 0 : (c > p.rows ? p.rows : c));
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {  // running sum, cut off at p.rows
+            const int v = __shfl_up_sync(0xffffffffu, end, o);
+            if (lane >= o) end = min(end + v, p.rows);
+        }
+        end = min(done_rows + end, p.rows);
+        int begin = __shfl_up_sync(0xffffffffu, end, 1);
+        if (lane == 0) begin = done_rows;
+        const int mine = (end - begin + kFewRows - 1) / kFewRows;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const int first = done_chunks + upto - mine;  // this expert's first chunk
+        const uint32_t hit = __ballot_sync(0xffffffffu, chunk >= first && chunk < first + mine);
+        if (hit != 0) {
+            const int src = __ffs(hit) - 1;
+            expert = e0 + src;
+            row0 = __shfl_sync(0xffffffffu, begin + (chunk - first) * kFewRows, src);
+            rows = min(kFewRows, __shfl_sync(0xffffffffu, end, src) - row0);
+            return true;
+        }
+        done_rows = __shfl_sync(0xffffffffu, end, 31);
+        done_chunks += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    expert = -2;
+    row0 = done_rows + (chunk - done_chunks) * kFewRows;
+    rows = min(kFewRows, p.rows - row0);
+    return rows > 0;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kFewThreads, 3) few_rows_kernel(const __grid_constant__ FewRows p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full_bar[kFewStages], empty_bar[kFewStages], scale_bar, acc_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int item = blockIdx.x / p.split;
+    const int chunk = item / p.tiles, n0 = (item - chunk * p.tiles) * 128;
+    int expert, row0, rows;
+    if (!few_locate(p, chunk, expert, row0, rows)) return;  // the whole cluster
+    T* const out = static_cast<T*>(p.out) + static_cast<int64_t>(row0) * p.N + n0;
+    if (expert < 0) {
+        if (rank == 0)
+            for (int i = tid; i < rows * 128; i += kFewThreads)
+                if (n0 + (i & 127) < p.N) out[static_cast<int64_t>(i >> 7) * p.N + (i & 127)] = float_to_elem<T>(0.f);
+        return;
+    }
+    const int q0 = p.quads * rank / p.split, q1 = p.quads * (rank + 1) / p.split;  // this CTA's groups of 512 columns
+    const int k0 = 4 * q0, n_kb = min(4 * q1, p.k_blocks) - k0;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t xs = ring + kFewStages * kFewStageBytes;
+    uint8_t* const base = smem_raw + (ring - smem_u32(smem_raw));
+    uint8_t* const x8 = base + kFewStages * kFewStageBytes;
+    uint32_t* const sx = reinterpret_cast<uint32_t*>(x8 + 4 * p.quads_most * kFewXBytes);  // [quad][16]
+    volatile int* abort_ptr = &abort_flag;
+
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < kFewStages; ++s) {
+            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        mbar_init(smem_u32(&scale_bar), 4);
+        mbar_init(smem_u32(&acc_bar), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        for (int kb = 0; kb < min(kFewStages, n_kb); ++kb) {  // the weights start to flow before anything else is done
+            mbar_arrive_expect_tx(smem_u32(&full_bar[kb]), kFewStageBytes);
+            tma_load_2d(ring + kb * kFewStageBytes, &p.map_w, smem_u32(&full_bar[kb]), (k0 + kb) * FP8_BLOCK, expert * p.N + n0);
+        }
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                     "r"(p.tmem_cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+
+    // the rows of x in 8 bits, in the 128-byte swizzle of an MMA operand
+    {
+        constexpr int AHEAD = 4;  // rows whose loads are in flight together
+        const int n = rows * (q1 - q0), s = lane & 7, g = lane >> 3;
+        for (int i0 = warp; i0 < n; i0 += kFewWarps * AHEAD) {
+            uint4 raw[AHEAD][2];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = i0 + u * kFewWarps, q = i / rows, r = i - q * rows;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int c = (k0 + 4 * q + g) * FP8_BLOCK + LaneBlock<T>::column(s, j);
+                    raw[u][j] = i < n && c < p.K ? ld_global_16(static_cast<const T*>(p.x) + (row0 + r) * p.x_pitch + c) : make_uint4(0, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int i = i0 + u * kFewWarps, q = i / rows, r = i - q * rows, kb = 4 * q + g;
+                if (i >= n) break;
+                float v[16];
+                Elem<T>::unpack(raw[u][0], v);
+                Elem<T>::unpack(raw[u][1], v + 8);
+                uint32_t w[4];
+                const uint32_t word = quantize_lane_block(v, w);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int c = LaneBlock<T>::column(s, j);
+                    *reinterpret_cast<uint2*>(x8 + kb * kFewXBytes + r * FP8_BLOCK + (((c >> 4) ^ (r & 7)) << 4) + (c & 15)) =
+                        make_uint2(w[2 * j], w[2 * j + 1]);
+                }
+                if (lane == 0) sx[q * kFewRows + r] = word;
+            }
+        }
+    }
+    fence_smem_to_async();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int kb = kFewStages; kb < n_kb; ++kb) {
+                const int s = kb % kFewStages;
+                if (!mbar_wait(smem_u32(&empty_bar[s]), (kb / kFewStages - 1) & 1u, abort_ptr, p.status)) break;
+                mbar_arrive_expect_tx(smem_u32(&full_bar[s]), kFewStageBytes);
+                tma_load_2d(ring + s * kFewStageBytes, &p.map_w, smem_u32(&full_bar[s]), (k0 + kb) * FP8_BLOCK, expert * p.N + n0);
+            }
+        }
+    } else if (warp == 1) {
+        bool alive = mbar_wait(smem_u32(&scale_bar), 0, abort_ptr, p.status);
+        for (int kb = 0; kb < n_kb && alive; ++kb) {
+            const int s = kb % kFewStages;
+            alive = mbar_wait(smem_u32(&full_bar[s]), (kb / kFewStages) & 1u, abort_ptr, p.status);
+            if (!alive) break;
+            tc_fence_after();
+            const uint32_t byte = kb & 3, scales = tmem + kFewScaleCol + (kb >> 2) * kFewScaleCols;
+            const uint32_t idesc = (byte << 4) | (static_cast<uint32_t>(kFewRows >> 3) << 17) | (1u << 23) | (8u << 24) | (byte << 29);
+            const uint64_t a = make_smem_desc<false>(ring + s * kFewStageBytes);
+            const uint64_t b = make_smem_desc<false>(xs + kb * kFewXBytes);
+#pragma unroll
+            for (int ks = 0; ks < FP8_BLOCK / 32; ++ks)
+                tc_mma_f8(tmem, a + ks * 2, b + ks * 2, idesc, scales, scales + 4, (kb | ks) != 0);
+            tc_commit_elected(smem_u32(&empty_bar[s]));
+        }
+        if (alive) tc_commit_elected(smem_u32(&acc_bar));
+    }
+    float* const part = reinterpret_cast<float*>(base);  // [16 rows of x][128 weight rows], over the drained ring
+    if (warp >= 4) {
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        for (int q = 0; q < q1 - q0; ++q) {
+            const uint32_t ww = __ldg(reinterpret_cast<const uint32_t*>(
+                p.w_scales + (static_cast<int64_t>(q0 + q) * p.b_tiles + static_cast<int64_t>(expert) * p.tiles + n0 / 128) * FP8_TILE_BYTES));
+            const uint32_t wx = sx[q * kFewRows + (lane & 15)];
+            const uint32_t at = tmem + lanes + kFewScaleCol + q * kFewScaleCols;
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(ww) : "memory");
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(at + 4), "r"(wx) : "memory");
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&scale_bar));
+        if (mbar_wait(smem_u32(&acc_bar), 0, abort_ptr, p.status)) {
+            tc_fence_after();
+            uint32_t v[16];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                  "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                : "r"(tmem + lanes)
+                : "memory");
+            tc_load_wait();
+            const int n = (warp & 3) * 32 + lane;
+            if (p.split == 1) {
+#pragma unroll
+                for (int r = 0; r < kFewRows; ++r)
+                    if (r < rows && n0 + n < p.N) out[static_cast<int64_t>(r) * p.N + n] = float_to_elem<T>(__uint_as_float(v[r]));
+            } else {
+#pragma unroll
+                for (int r = 0; r < kFewRows; ++r)
+                    if (r < rows) part[r * 128 + n] = __uint_as_float(v[r]);
+            }
+        }
+    }
+    __syncwarp();
+    if (abort_flag && tid == 0) {
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);  // let copies in flight land
+    }
+    __syncwarp();
+    if (p.split > 1) {
+        cluster_sync_all();  // every part is in its CTA's shared memory
+        const int width = 128 / p.split;  // this CTA adds and writes its share of the weight rows
+        for (int i = tid; i < rows * width; i += kFewThreads) {
+            const int r = i / width, n = rank * width + i % width;
+            float sum = 0.f;
+            for (int c = 0; c < p.split; ++c) sum += ld_shared_cluster_f32(map_to_rank(ring + (r * 128 + n) * 4, c));
+            if (n0 + n < p.N) out[static_cast<int64_t>(r) * p.N + n] = float_to_elem<T>(sum);
+        }
+        tc_fence_before();
+        cluster_sync_all();  // nobody leaves while its part is being read
+    } else {
+        tc_fence_before();
+        __syncthreads();
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+    }
+}
+
+// CTAs per tile, in whole groups of 512 columns: until nearly every SM has one, and on while a CTA would read more than
+// 256 KB and there is room for all of them (three per SM).  Measured, one row: 14336 x 4096 (112 tiles) 16.1 / 14.1 / 17.0 us
+// with 1 / 2 / 4 CTAs per tile, 4096 x 4096 (32 tiles) 7.8 / 6.5 / 7.6 with 2 / 4 / 8, 4096 x 14336 16.9 / 14.6 with 4 / 8,
+// 8 rows of 8 experts of 1536 x 2048 (96 tiles) 9.5 / 10.9 with 2 / 4.
+constexpr int FEW_QUADS_MOST = 18;  // rows of x in 8 bits that fit into shared memory beside the ring
+static int few_split(int64_t items, int quads) {
+    const int64_t sms = sm_count();
+    int split = 1;
+    while (split < 8 && 2 * split <= quads &&
+           (100 * items * split < 85 * sms || (quads > 4 * split && 2 * items * split <= 3 * sms) || quads > FEW_QUADS_MOST * split))
+        split *= 2;
+    return split;
+}
+static int64_t few_smem(int quads_most) {
+    return kFewStages * static_cast<int64_t>(kFewStageBytes) + static_cast<int64_t>(quads_most) * (4 * kFewXBytes + kFewRows * 4) + 1024;
+}
+static int64_t few_chunks(int64_t rows, int32_t E, bool counts) {  // at most
+    if (!counts) return (rows + kFewRows - 1) / kFewRows;
+    const int64_t groups = E + 1 < rows ? E + 1 : rows, n = rows / kFewRows + groups;
+    return n < rows ? n : rows;
+}
+
+template <typename T>
+static int launch_few(const FewRows& p, int64_t items, cudaStream_t s) {
+    static bool configured[64] = {false};  // per device: the attribute applies to the current device only
+    const int dev = current_device_slot();
+    FMAB_REQUIRE(dev >= 0, FMA_B200_ERR_LAUNCH, "no current CUDA device with an ordinal below 64");
+    if (!configured[dev]) {
+        FMAB_CUDA(cudaFuncSetAttribute(few_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
+        configured[dev] = true;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(items * p.split));
+    config.blockDim = dim3(kFewThreads);
+    config.dynamicSmemBytes = static_cast<size_t>(few_smem(p.quads_most));
+    config.stream = s;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = static_cast<unsigned>(p.split);
+    cluster.val.clusterDim.y = 1;
+    cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    FMAB_CUDA(cudaLaunchKernelEx(&config, few_rows_kernel<T>, p));
+    return check_launch("fp8_few_rows");
+}
+
+}  // namespace fmab
+
+extern "C" {
+
+int fma_b200_fp8_few_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, const void* w, const void* w_scales,
+                          int32_t E, int32_t N, int32_t K, const void* counts, int32_t index_bytes, void* out, void* stream) {
+    using namespace fmab;
+    FMAB_REQUIRE(dtype == FMA_B200_BF16 || dtype == FMA_B200_F16, FMA_B200_ERR_UNSUPPORTED,
+                 "dtype %d: the 8-bit product takes and returns bfloat16 or half", dtype);
+    FMAB_REQUIRE(rows >= 0 && rows < (1LL << 30), FMA_B200_ERR_BAD_ARG, "rows=%lld", (long long)rows);
+    FMAB_REQUIRE(E >= 1 && E <= 1024, FMA_B200_ERR_BAD_ARG, "E=%d not in [1,1024]", E);
+    FMAB_REQUIRE(N >= 8 && K >= 8 && N % 8 == 0 && K % 8 == 0 && N < (1 << 30) && K < (1 << 30), FMA_B200_ERR_BAD_ARG,
+                 "N=%d and K=%d must be positive multiples of 8", N, K);
+    FMAB_REQUIRE(static_cast<int64_t>(E) * N < (1LL << 31) - 1024, FMA_B200_ERR_BAD_ARG, "E*N overflows");
+    FMAB_REQUIRE(x_pitch >= K && x_pitch % 8 == 0, FMA_B200_ERR_BAD_ARG, "x: row pitch %lld", (long long)x_pitch);
+    FMAB_REQUIRE(E == 1 || counts != nullptr, FMA_B200_ERR_BAD_ARG, "several experts need their counts");
+    FMAB_REQUIRE(counts == nullptr || index_bytes == 4 || index_bytes == 8, FMA_B200_ERR_UNSUPPORTED, "index_bytes=%d", index_bytes);
+    if (rows == 0) return FMA_B200_OK;
+    FMAB_REQUIRE(x && w && w_scales && out, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    FMAB_REQUIRE(aligned16(x) && aligned16(w) && aligned16(w_scales) && aligned16(out), FMA_B200_ERR_BAD_ARG,
+                 "pointers not 16-byte aligned");
+    FewRows p;
+    memset(&p, 0, sizeof(p));
+    p.status = device_status_ptr();
+    FMAB_REQUIRE(p.status != nullptr, FMA_B200_ERR_LAUNCH, "no device status word");
+    p.x = x;
+    p.x_pitch = x_pitch;
+    p.w_scales = static_cast<const uint8_t*>(w_scales);
+    p.out = out;
+    p.counts = counts;
+    p.index_bytes = index_bytes;
+    p.E = E;
+    p.rows = static_cast<int32_t>(rows);
+    p.N = N;
+    p.K = K;
+    p.k_blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
+    p.quads = static_cast<int32_t>(fp8_quads(K));
+    p.tiles = static_cast<int32_t>(fp8_row_tiles(N));
+    p.b_tiles = E * p.tiles;
+    const int64_t items = few_chunks(rows, E, counts != nullptr) * p.tiles;
+    p.split = few_split(items, p.quads);
+    p.quads_most = (p.quads + p.split - 1) / p.split;
+    p.tmem_cols = 32;
+    while (p.tmem_cols < static_cast<uint32_t>(kFewScaleCol + kFewScaleCols * p.quads_most)) p.tmem_cols *= 2;
+    FMAB_REQUIRE(p.quads_most <= FEW_QUADS_MOST, FMA_B200_ERR_UNSUPPORTED, "K=%d is too large for the product of a few rows", K);
+    FMAB_REQUIRE(items * p.split < (1LL << 31), FMA_B200_ERR_BAD_ARG, "too many tiles");
+    if (int rc = encode_bytes(&p.map_w, w, K, static_cast<uint64_t>(E) * N, fp8_pitch(K), 128)) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == FMA_B200_BF16 ? launch_few<__nv_bfloat16>(p, items, s) : launch_few<__half>(p, items, s);
+}
+
+}  // extern "C"

@@ -2,93 +2,12 @@
 // layout of the MoE layer), quantising weights with their transposed copy, dequantising, and SwiGLU that keeps its
 // inputs in 8 bits for the backward pass.  All are bound by HBM traffic: one pass over the data, 128-bit reads, every
 // value read once and written once; the block maximum lives in registers between the two.
-//
-// Row kernels: a warp takes 512 columns of a row (one scale word); 8 lanes share a block of 128 columns, so the block
-// maximum is three shuffles and every load instruction of the 8 lanes covers 128 contiguous bytes.
 #include "fp8.cuh"
 
 namespace fmab {
 
 constexpr int kQThreads = 256;
 constexpr int kQWarps = kQThreads / 32;
-
-template <typename T>
-struct LaneBlock {                                    // a lane's 16 of the block's 128 columns
-    static constexpr int V = Elem<T>::kPerVec;        // columns per 128-bit access
-    static constexpr int N = 16 / V;                  // accesses
-    // column (inside the block) of access j for the lane's place s = lane % 8
-    __device__ static __forceinline__ int column(int s, int j) { return j * 8 * V + s * V; }
-};
-
-__device__ __forceinline__ uint32_t max_over_8_lanes(uint32_t v) {
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-
-// Reads the lane's 16 values of columns [col0, cols); columns beyond are zero.
-template <typename T>
-__device__ __forceinline__ void load_lane_block(const T* row, int col0, int cols, int s, float* x) {
-    using B = LaneBlock<T>;
-#pragma unroll
-    for (int j = 0; j < B::N; ++j) {
-        const int c = col0 + B::column(s, j);
-        const uint4 v = c < cols ? ld_stream_16(row + c) : make_uint4(0, 0, 0, 0);
-        Elem<T>::unpack(v, x + j * B::V);
-    }
-}
-template <typename T>
-__device__ __forceinline__ void store_lane_block(T* row, int col0, int cols, int s, const float* x) {
-    using B = LaneBlock<T>;
-#pragma unroll
-    for (int j = 0; j < B::N; ++j) {
-        const int c = col0 + B::column(s, j);
-        if (c < cols) st_global_16(row + c, Elem<T>::pack(x + j * B::V));
-    }
-}
-// The lane's 16 bytes to / from the value row (pitch columns, of which those from `cols` on are zero).
-template <typename T>
-__device__ __forceinline__ void store_lane_bytes(uint8_t* row, int col0, int pitch, int s, const uint32_t* w) {
-    using B = LaneBlock<T>;
-#pragma unroll
-    for (int j = 0; j < B::N; ++j) {
-        const int c = col0 + B::column(s, j);
-        if (c >= pitch) continue;
-        if (B::V == 8)
-            *reinterpret_cast<uint2*>(row + c) = make_uint2(w[2 * j], w[2 * j + 1]);
-        else
-            *reinterpret_cast<uint32_t*>(row + c) = w[j];
-    }
-}
-template <typename T>
-__device__ __forceinline__ void load_lane_bytes(const uint8_t* row, int col0, int pitch, int s, uint32_t* w) {
-    using B = LaneBlock<T>;
-#pragma unroll
-    for (int j = 0; j < B::N; ++j) {
-        const int c = col0 + B::column(s, j);
-        if (B::V == 8) {
-            const uint2 v = c < pitch ? *reinterpret_cast<const uint2*>(row + c) : make_uint2(0, 0);
-            w[2 * j] = v.x;
-            w[2 * j + 1] = v.y;
-        } else {
-            w[j] = c < pitch ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
-        }
-    }
-}
-// Scale byte of the 8 lanes' block and its 16 packed values per lane; returns the warp's scale word (all lanes).
-__device__ __forceinline__ uint32_t quantize_lane_block(const float* x, uint32_t* w) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m = max(m, fp8_magnitude(x[i]));
-    const uint32_t byte = fp8_scale_byte(max_over_8_lanes(m));
-    const float inverse = fp8_inverse(byte);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = fp8_pack4(x + 4 * i, inverse);
-    uint32_t word = byte << (8 * ((threadIdx.x & 31) >> 3));
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    word |= __shfl_xor_sync(0xffffffffu, word, 16);
-    return word;
-}
 
 // Where a source row goes.  rows: to itself.  groups: rows of expert e are consecutive in the source
 // ([offsets[e], offsets[e+1])) and start at pad_offsets[e] in the layout.  slots: source row t goes to the k rows

@@ -390,20 +390,6 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
 }
 
 // ---- host side -------------------------------------------------------------------------------------
-// Bytes [outer, inner] with row pitch `pitch`, boxes of box_outer rows x 128 bytes, 128-byte swizzle.
-static int encode_bytes(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_outer) {
-    EncodeTiledFn fn = encode_fn();
-    FMAB_REQUIRE(fn != nullptr, FMA_B200_ERR_LAUNCH, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint64_t dims[2] = {inner, outer};
-    const cuuint64_t strides[1] = {pitch};
-    const cuuint32_t box[2] = {BK8, box_outer};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    FMAB_REQUIRE(r == CUDA_SUCCESS, FMA_B200_ERR_LAUNCH, "cuTensorMapEncodeTiled (8-bit operand) failed with CUresult %d", (int)r);
-    return FMA_B200_OK;
-}
 // Columns per tile.  Few wide tiles read A least often; but the launch takes as long as its fullest pair of SMs, so
 // where the number of row tiles is known (no experts) the width that makes waves * (width + 24) smallest is taken, 24
 // columns standing for what a tile costs besides its columns: a prompt of up to 256 rows spreads over all SMs (256 x

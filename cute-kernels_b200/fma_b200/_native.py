@@ -91,6 +91,7 @@ SIGNATURES: dict[str, tuple] = {
         ctypes.c_int,
         [_P, _P, _I64, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _P, _P],
     ),
+    "fma_b200_fp8_few_rows": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P, _I32, _I32, _I32, _P, _I32, _P, _P]),
     "fma_b200_swiglu_fp8_forward": (
         ctypes.c_int,
         [_P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P],

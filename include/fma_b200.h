@@ -465,6 +465,14 @@ int fma_b200_fp8_gemm(const void* a, const void* a_scales, int64_t layout_rows, 
                       const int32_t* tile_expert, const int32_t* tile_row, const int32_t* tile_rows,
                       const int32_t* rows_used, void* stream);
 /*
+ * The same product for a few rows, in one launch: x [rows, K] in bfloat16 or half is quantised on the way in; counts
+ * [E] (4- or 8-byte integers on the device, NULL: one expert) consecutive rows per expert, rows behind the last
+ * expert's give zeros.  For any number of rows, but meant for up to about 16 per expert: an expert's weights are read
+ * once per 16 of its rows.
+ */
+int fma_b200_fp8_few_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, const void* w, const void* w_scales,
+                          int32_t E, int32_t N, int32_t K, const void* counts, int32_t index_bytes, void* out, void* stream);
+/*
  * SwiGLU that keeps its inputs in 8 bits.  forward: out as fma_b200_swiglu_forward (may be NULL), and with gate8 / up8
  * / out8 (each may be NULL) the 8-bit form of gate, up and the rounded out in 1 x 128 blocks.  backward:
  * fma_b200_swiglu_backward on the values that gate8 and up8 stand for.
