@@ -22,6 +22,7 @@ struct QuantRows {
     const int32_t* pad_offsets;
     const int32_t* row_of_slot;
     const int32_t* slot_of_row;
+    const int32_t* rows_used; // rows: source rows from here on are left alone; null: all rows
     int64_t x_pitch;
     int64_t rows;             // source rows
     int64_t row_blocks;       // blocks that quantise; the others zero the padding rows
@@ -74,7 +75,8 @@ __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRow
                                  (static_cast<int64_t>(gridDim.x) - p.row_blocks) * kQWarps);
         return;
     }
-    const int64_t n_items = p.rows * p.quads;
+    const int64_t rows = TO == TO_ROWS && p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
+    const int64_t n_items = rows * p.quads;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQWarps + warp; i < n_items; i += p.row_blocks * kQWarps) {
         const int64_t row = i / p.quads;
         const int q = static_cast<int>(i - row * p.quads);
@@ -472,12 +474,13 @@ int64_t fma_b200_fp8_scale_bytes(int64_t rows, int64_t cols) {
     return fmab::fp8_quads(cols) * fmab::fp8_row_tiles(rows) * fmab::FP8_TILE_BYTES;
 }
 
-int fma_b200_fp8_quantize_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols, void* values,
-                               void* scales, void* stream) {
+int fma_b200_fp8_quantize_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols,
+                               const int32_t* rows_used, void* values, void* scales, void* stream) {
     using namespace fmab;
     QuantRows p;
     if (int rc = fill_quantize(p, x, x_pitch, dtype, rows, cols, rows, values, scales)) return rc;
     if (rows == 0) return FMA_B200_OK;
+    p.rows_used = rows_used;
     return launch_quantize<TO_ROWS>(p, dtype, 0, static_cast<cudaStream_t>(stream));
 }
 

@@ -23,8 +23,10 @@ import torch.nn as nn
 
 from .. import _native
 from ..kernel_backend import KernelBackend
+from ..ops.fp8 import quantize_fp8_weight
 from ..ops.grouped_gemm import grouped_gemm
 from ..ops.swiglu import swiglu_packed
+from . import _fp8_experts
 from . import _kernels as K
 
 
@@ -250,6 +252,11 @@ class Experts(nn.Module):
 
 
 class MoE(nn.Module):
+    # Set to True to run the SwiGLU experts on 8-bit operands (bfloat16 / float16 layers): the products take e4m3 operands
+    # with a scale per block of 128, and the backward pass works from 8-bit activations (modules/_fp8_experts.py).
+    fp8_experts = False
+    _held_experts = None  # what quantize_experts() made
+
     def __init__(
         self,
         num_experts: int,
@@ -307,6 +314,8 @@ class MoE(nn.Module):
         original_shape = hidden_states.shape
         hidden_states = hidden_states.reshape(-1, self.hidden_size)
         if torch.compiler.is_compiling():
+            if self.fp8_experts:
+                raise RuntimeError("fp8_experts is not available under torch.compile")
             return self._forward_traced(hidden_states, original_shape)
 
         with torch.cuda.device(hidden_states.device):
@@ -347,7 +356,7 @@ class MoE(nn.Module):
         self._routed = (selected_experts, workspace, router_logits)
         return router_logits, router_weights, selected_experts
 
-    def _sort_selected(self, selected_experts: torch.Tensor) -> K.RowMaps:
+    def _sort_selected(self, selected_experts: torch.Tensor, row_align: int = K.ROW_ALIGN) -> K.RowMaps:
         """Row maps for `selected_experts`; reuses what the routing kernel prepared when these are the ids
         it produced in this forward."""
         routed = getattr(self, "_routed", None)
@@ -355,9 +364,10 @@ class MoE(nn.Module):
         self.last_router_stats = None
         with torch.no_grad():
             if routed is None or routed[0] is not selected_experts:
-                return K.moe_sort(selected_experts, self.num_experts)
+                return K.moe_sort(selected_experts, self.num_experts, row_align=row_align)
             want = bool(getattr(self, "collect_router_stats", False))
-            maps = K.moe_sort(selected_experts, self.num_experts, routed_workspace=routed[1], want_mean_prob=want)
+            maps = K.moe_sort(selected_experts, self.num_experts, row_align=row_align, routed_workspace=routed[1],
+                              want_mean_prob=want)  # fmt: skip
         if maps.router_mean_prob is not None:
             logits = routed[2]
             mean_prob = maps.router_mean_prob
@@ -383,6 +393,8 @@ class MoE(nn.Module):
         self, hidden_states: torch.Tensor, router_weights: torch.Tensor, selected_experts: torch.Tensor
     ) -> torch.Tensor:
         T = hidden_states.size(0)
+        if self.fp8_experts:
+            return self._compute_experts_fp8(hidden_states, router_weights, selected_experts)
         maps = self._sort_selected(selected_experts)
         self.last_row_maps = maps  # expert_count etc. for callers that log load balance
 
@@ -397,3 +409,43 @@ class MoE(nn.Module):
         grouped = self.act(grouped)
         grouped = self.c_proj.grouped_forward(grouped, maps)
         return _Combine.apply(grouped, router_weights, maps, T)
+
+    # ---- experts on 8-bit operands ------------------------------------------------------------------
+    def _experts_in_8_bits(self, transpose: bool):
+        return tuple(quantize_fp8_weight(w, transpose) for w in (self.c_fc.weight, self.c_proj.weight))
+
+    def _expert_weights_seen(self):
+        return tuple((w._version, w.data_ptr(), w.dtype, w.device) for w in (self.c_fc.weight, self.c_proj.weight))
+
+    @torch.no_grad()
+    def quantize_experts(self) -> None:
+        """For serving with fp8_experts: quantises the expert weights once, for all later forward passes without gradients
+        (otherwise, and whenever gradients are recorded, every forward quantises the weights it finds).  After the
+        weights have changed, call it again; until then such a forward raises an error."""
+        with torch.cuda.device(self.c_fc.weight.device):
+            self._held_experts = (*self._experts_in_8_bits(False), self._expert_weights_seen())
+
+    def _compute_experts_fp8(self, hidden_states, router_weights, selected_experts):
+        if not (self.is_glu and _is_swiglu_packed(self.act) and self.c_fc.bias is None and self.c_proj.bias is None):
+            raise RuntimeError("fp8_experts needs SwiGLU experts (is_glu, swiglu_packed) without bias")
+        if hidden_states.dtype not in (torch.bfloat16, torch.float16) or self.c_fc.weight.dtype != hidden_states.dtype:
+            raise RuntimeError(f"fp8_experts runs bfloat16 and float16 layers, got {hidden_states.dtype} tokens and "
+                               f"{self.c_fc.weight.dtype} weights")  # fmt: skip
+        T = hidden_states.size(0)
+        graph = torch.is_grad_enabled() and any(
+            t.requires_grad for t in (hidden_states, router_weights, self.c_fc.weight, self.c_proj.weight))  # fmt: skip
+        held = None
+        if not graph and self._held_experts is not None:
+            if self._held_experts[2] != self._expert_weights_seen():
+                raise RuntimeError("the expert weights have changed since quantize_experts(): call it again")
+            held = self._held_experts[:2]
+        if held is None:
+            held = self._experts_in_8_bits(graph)
+        if not graph and _fp8_experts.few(T * self.top_k, held[1]):
+            maps = self._sort_selected(selected_experts, row_align=1)
+            self.last_row_maps = maps
+            return _fp8_experts.few_tokens(hidden_states, router_weights, *held, maps)
+        maps = self._sort_selected(selected_experts)
+        self.last_row_maps = maps
+        return _fp8_experts.Fp8SwigluExperts.apply(hidden_states, router_weights, self.c_fc.weight, self.c_proj.weight,
+                                                   *held, maps)  # fmt: skip

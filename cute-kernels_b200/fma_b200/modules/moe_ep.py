@@ -425,6 +425,8 @@ class ExpertParallelMoE(MoE):
     def _compute_experts(self, hidden_states, router_weights, selected_experts):
         if self.ep_size == 1:
             return super()._compute_experts(hidden_states, router_weights, selected_experts)
+        if self.fp8_experts:
+            raise RuntimeError("fp8_experts is not available with the experts sharded over several ranks")
         maps = self._sort_selected(selected_experts)
         self.last_row_maps = maps
         fused = self.is_glu and _is_swiglu_packed(self.act) and self.c_fc.bias is None and self.c_proj.bias is None

@@ -114,13 +114,13 @@ def _dequantize(values, scales, batch: int, rows: int, shape, dtype, rows_used: 
     return out
 
 
-def _quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+def _quantize_rows(x: torch.Tensor, rows_used: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """x [rows, cols] as _rows_2d gives it -> (values, scales)."""
     rows, cols = x.shape
     values = torch.empty(rows, _pitch(cols), dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=x.device)
-    call("fma_b200_fp8_quantize_rows", ptr(x), x.stride(0), dtype_code(x.dtype), rows, cols, ptr(values), ptr(scales),
-         stream_ptr(x.device))  # fmt: skip
+    call("fma_b200_fp8_quantize_rows", ptr(x), x.stride(0), dtype_code(x.dtype), rows, cols, ptr(rows_used), ptr(values),
+         ptr(scales), stream_ptr(x.device))  # fmt: skip
     return values, scales
 
 

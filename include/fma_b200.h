@@ -417,7 +417,8 @@ int fma_b200_grouped_gemm(const void* A, const void* B, void* D, const uint32_t*
  * (row % 32) * 16 + (row / 32 % 4) * 4 + b % 4; fma_b200_fp8_scale_bytes(rows, cols) is the size of the array.
  * cols is a multiple of 8, pitches are in elements and whole multiples of 16 bytes, pointers 16-byte aligned.
  *
- * quantize_rows      x [rows, cols] (row pitch x_pitch) -> values, scales, blocks of 1 x 128
+ * quantize_rows      x [rows, cols] (row pitch x_pitch) -> values, scales, blocks of 1 x 128.  Here and below rows_used
+ *                    (device, may be NULL) limits the rows: those from *rows_used on are not touched.
  * quantize_groups    the same for rows that are grouped by expert without alignment: source rows
  *                    [offsets[e], offsets[e+1]) go to layout rows pad_offsets[e].. ; the padding rows below
  *                    pad_offsets[E] become zeros; source rows from offsets[E] on are left out.  copy (may be NULL)
@@ -428,12 +429,11 @@ int fma_b200_grouped_gemm(const void* A, const void* B, void* D, const uint32_t*
  *                    transposed copy [E, K, pitch(N)].  Scale tiles count ceil(N/128) (transposed: ceil(K/128))
  *                    row tiles per expert, so their size is scale_bytes(E * ceil(N/128) * 128, K)
  * dequantize         batch matrices [rows, cols] with 1 x 128 or 128 x 128 blocks -> out, contiguous; what a rounding
- *                    to e4m3 lifted above the type's range becomes its largest finite value.  rows_used (device,
- *                    may be NULL): rows from *rows_used on are not touched.
+ *                    to e4m3 lifted above the type's range becomes its largest finite value
  */
 int64_t fma_b200_fp8_scale_bytes(int64_t rows, int64_t cols);
-int fma_b200_fp8_quantize_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols, void* values,
-                               void* scales, void* stream);
+int fma_b200_fp8_quantize_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols,
+                               const int32_t* rows_used, void* values, void* scales, void* stream);
 int fma_b200_fp8_quantize_groups(const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols,
                                  const int32_t* offsets, const int32_t* pad_offsets, int32_t E, int64_t layout_rows,
                                  void* values, void* scales, void* copy, void* stream);

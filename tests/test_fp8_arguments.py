@@ -1,0 +1,115 @@
+"""The 8-bit operators without a GPU: refusals of the C entry points (checked before any CUDA call), sizes, and the
+definition that the GPU tests compare with against torch's own e4m3 conversion."""
+
+import ctypes
+
+import pytest
+import torch
+
+import _fp8_ref as R
+
+
+def test_entry_points_refuse_bad_arguments():
+    from fma_b200 import _native
+
+    lib = _native.lib()
+    null, at = ctypes.c_void_p(None), ctypes.c_void_p(16)
+    odd = ctypes.c_void_p(24)
+    OK, BAD, UNSUPPORTED = 0, 1, 2
+    assert lib.fma_b200_fp8_scale_bytes(1, 8) == 512
+    assert lib.fma_b200_fp8_scale_bytes(129, 513) == 4 * 512
+    assert lib.fma_b200_fp8_scale_bytes(0, 4096) == 0
+    assert lib.fma_b200_fp8_scale_bytes(-1, 8) == 0
+    q = lib.fma_b200_fp8_quantize_rows
+    assert q(at, 16, 7, 4, 16, null, at, at, null) == UNSUPPORTED
+    assert q(at, 16, 1, 4, 12, null, at, at, null) == BAD  # width
+    assert q(at, 8, 1, 4, 16, null, at, at, null) == BAD  # pitch below the width
+    assert q(at, 20, 1, 4, 16, null, at, at, null) == BAD  # pitch not whole 16 bytes
+    assert q(null, 16, 1, 4, 16, null, at, at, null) == BAD
+    assert q(odd, 16, 1, 4, 16, null, at, at, null) == BAD
+    assert q(at, 16, 1, -1, 16, null, at, at, null) == BAD
+    assert q(null, 16, 1, 0, 16, null, null, null, null) == OK
+    g = lib.fma_b200_fp8_quantize_groups
+    assert g(at, 16, 1, 4, 16, at, at, 0, 256, at, at, null, null) == BAD
+    assert g(at, 16, 1, 4, 16, null, at, 2, 256, at, at, null, null) == BAD
+    assert g(at, 16, 1, 4, 16, at, at, 2, 256, at, at, odd, null) == BAD
+    s = lib.fma_b200_fp8_quantize_scatter
+    assert s(at, 1, 4, 16, 0, at, at, at, 2, 256, at, at, null) == BAD  # k
+    assert s(at, 1, 4, 16, 2, at, null, at, 2, 256, at, at, null) == BAD
+    w = lib.fma_b200_fp8_quantize_weight
+    assert w(at, 1, 1, 12, 16, at, at, null, null, null) == BAD  # N
+    assert w(at, 1, 2000, 16, 16, at, at, null, null, null) == BAD  # E
+    assert w(at, 1, 1, 16, 16, at, at, at, null, null) == BAD  # transposed values without scales
+    assert w(at, 1, 1024, 1 << 22, 16, at, at, null, null, null) == BAD  # E * N
+    d = lib.fma_b200_fp8_dequantize
+    assert d(at, at, 0, 4, 16, null, at, 1, null) == BAD
+    assert d(at, at, 1, 4, 16, null, at, 5, null) == UNSUPPORTED
+    assert d(at, null, 1, 4, 16, null, at, 1, null) == BAD
+    m = lib.fma_b200_fp8_group_maps
+    assert m(at, 2, 4, 100, 2048, at, at, at, at, at, null) == UNSUPPORTED
+    assert m(at, 4, 4, 100, 1024, at, at, at, at, at, null) == BAD  # layout too small: 256 + 4 * 256
+    assert m(at, 4, 1025, 100, 1 << 20, at, at, at, at, at, null) == BAD
+    assert m(null, 4, 4, 100, 2048, at, at, at, at, at, null) == BAD
+    p = lib.fma_b200_fp8_gemm
+    assert p(at, at, 256, at, at, 1, 16, 16, at, 0, 256, null, null, null, null, null) == UNSUPPORTED  # fp32 result
+    assert p(at, at, 256, at, at, 2, 16, 16, at, 1, 256, null, null, null, null, null) == BAD  # experts without a table
+    assert p(at, at, 256, at, at, 1, 12, 16, at, 1, 256, null, null, null, null, null) == BAD
+    assert p(at, at, 256, at, at, 1, 16, 20, at, 1, 256, null, null, null, null, null) == BAD
+    assert p(at, null, 256, at, at, 1, 16, 16, at, 1, 256, null, null, null, null, null) == BAD
+    assert p(null, null, 0, null, null, 1, 16, 16, null, 1, 0, null, null, null, null, null) == OK
+    f = lib.fma_b200_fp8_few_rows
+    assert f(at, 16, 0, 4, at, at, 1, 16, 16, null, 4, at, null) == UNSUPPORTED
+    assert f(at, 8, 1, 4, at, at, 1, 16, 16, null, 4, at, null) == BAD
+    assert f(at, 16, 1, 4, at, at, 3, 16, 16, null, 4, at, null) == BAD  # experts without counts
+    assert f(at, 16, 1, 4, at, at, 3, 16, 16, at, 2, at, null) == UNSUPPORTED
+    assert f(at, 16, 1, 4, null, at, 1, 16, 16, null, 4, at, null) == BAD
+    assert f(null, 16, 1, 0, null, null, 1, 16, 16, null, 4, null, null) == OK
+    v = lib.fma_b200_linear_wgrad
+    assert v(at, at, at, 0, 4, 1, 16, 16, at, null) == UNSUPPORTED
+    assert v(at, at, at, 1, 0, 1, 16, 16, at, null) == BAD
+    assert v(at, at, at, 1, 4, 1, 16, 16, null, null) == BAD
+    fw, bw = lib.fma_b200_swiglu_fp8_forward, lib.fma_b200_swiglu_fp8_backward
+    assert fw(at, 16, at, 16, at, 16, 1, 4, 12, null, at, at, at, at, null, null, null) == BAD
+    assert fw(at, 16, at, 16, at, 16, 1, 4, 16, null, at, null, at, at, null, null, null) == BAD  # values without scales
+    assert fw(at, 16, null, 16, at, 16, 1, 4, 16, null, at, at, at, at, null, null, null) == BAD
+    assert bw(at, at, at, null, at, 16, at, 16, at, 16, 1, 4, 16, null, null) == BAD
+    assert bw(at, at, at, at, at, 12, at, 16, at, 16, 1, 4, 16, null, null) == BAD
+
+
+def test_operators_need_cuda_tensors():
+    import fma_b200 as fma
+
+    x, w = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
+    for call in (lambda: fma.quantize_fp8(x), lambda: fma.quantize_fp8_weight(w), lambda: fma.linear_fp8(x, w),
+                 lambda: fma.grouped_linear_fp8(x, w[None], torch.tensor([4])),
+                 lambda: fma.swiglu_fp8_checkpoint(x, x)):  # fmt: skip
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_layer_switch_is_off_and_leaves_the_state_dict_alone():
+    import fma_b200 as fma
+
+    moe = fma.MoE(4, 2, 32, 16, fma.swiglu_packed, True, False, 0.02)
+    assert moe.fp8_experts is False
+    keys = list(moe.state_dict())
+    moe.fp8_experts = True
+    assert list(moe.state_dict()) == keys
+
+
+@pytest.mark.parametrize("tall", [1, 128])
+def test_definition_against_torchs_conversion(tall):
+    x = torch.randn(200, 300, generator=torch.Generator().manual_seed(3)) * torch.exp2(torch.arange(200.0) / 8 - 12)[:, None]
+    x[7] = 0
+    held = R.hold(x, tall)
+    for r in range(0, 200, tall):
+        for c in range(0, 300, 128):
+            part = x[r : r + tall, c : c + 128]
+            amax = float(part.abs().max())
+            e = 0
+            if amax > 0:
+                e = -60
+                while amax > 448 * 2.0**e:
+                    e += 1
+            want = (part * 2.0**-e).to(torch.float8_e4m3fn).double() * 2.0**e
+            assert torch.equal(held[r : r + tall, c : c + 128], want)
