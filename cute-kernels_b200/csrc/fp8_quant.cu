@@ -9,6 +9,22 @@ namespace fmab {
 constexpr int kQThreads = 256;
 constexpr int kQWarps = kQThreads / 32;
 
+// Work of the row kernels: an item is a row, or a part of one (`per_item` groups of 512 columns) where there are few
+// rows; a warp has the loads of AHEAD groups in flight before it touches the first.  (One group per item, the row found
+// by a 64-bit division each time, ran at 70 % of the copy rate.)
+struct RowItems {
+    uint32_t items, parts;  // items; parts of a row
+    int32_t quads, per_item;
+    __device__ __forceinline__ void decode(uint32_t i, int64_t& row, int& q0, int& q1) const {
+        const uint32_t r = parts == 1 ? i : i / parts;
+        row = r;
+        q0 = static_cast<int>(i - r * parts) * per_item;
+        q1 = min(quads, q0 + per_item);
+    }
+};
+template <typename T>
+constexpr int kAhead = Elem<T>::kPerVec == 8 ? 4 : 2;
+
 // Where a source row goes.  rows: to itself.  groups: rows of expert e are consecutive in the source
 // ([offsets[e], offsets[e+1])) and start at pad_offsets[e] in the layout.  slots: source row t goes to the k rows
 // row_of_slot[t*k ..] of the MoE layer's layout.
@@ -25,10 +41,11 @@ struct QuantRows {
     const int32_t* rows_used; // rows: source rows from here on are left alone; null: all rows
     int64_t x_pitch;
     int64_t rows;             // source rows
-    int64_t row_blocks;       // blocks that quantise; the others zero the padding rows
+    RowItems work;
+    uint32_t row_blocks;      // blocks that quantise; the others zero the padding rows
     int64_t layout_rows;
     int64_t row_tiles;        // scale tiles per quad
-    int32_t cols, pitch, quads, n_groups, k;
+    int32_t cols, pitch, n_groups, k;
 };
 
 // Largest e with offsets[e] <= row (empty experts are skipped: of equal offsets the last one counts).
@@ -41,65 +58,91 @@ __device__ __forceinline__ int group_of_row(const int32_t* offsets, int n, int32
     return lo;
 }
 
+template <typename T>
+__device__ __forceinline__ void zero_row(const QuantRows& p, int64_t row) {
+    const int lane = threadIdx.x & 31;
+    for (int c = lane * 16; c < p.pitch; c += 512) st_global_16(p.values + row * p.pitch + c, make_uint4(0, 0, 0, 0));
+    for (int q = lane; q < p.work.quads; q += 32)
+        *reinterpret_cast<uint32_t*>(p.scales + fp8_scale_word(row, q, p.row_tiles)) = 0x01010101u * FP8_SCALE_ONE;
+    if (p.copy != nullptr) {
+        constexpr int V = Elem<T>::kPerVec;
+        for (int c = lane * V; c < p.cols; c += 32 * V) st_global_16(static_cast<T*>(p.copy) + row * p.cols + c, make_uint4(0, 0, 0, 0));
+    }
+}
+
 // Padding rows of the layout below its used end: zero values, zero copies.
 template <typename T, int TO>
-__device__ void zero_padding_rows(const QuantRows& p, int64_t first_row, int64_t step) {
-    const int lane = threadIdx.x & 31;
-    const int64_t used = min(static_cast<int64_t>(p.pad_offsets[p.n_groups]), p.layout_rows);
-    for (int64_t row = first_row; row < used; row += step) {
-        bool token;
-        if (TO == TO_SLOTS) {
-            token = p.slot_of_row[row] >= 0;
-        } else {
-            const int e = group_of_row(p.pad_offsets, p.n_groups, static_cast<int32_t>(row));
-            token = row - p.pad_offsets[e] < p.offsets[e + 1] - p.offsets[e];
-        }
-        if (token) continue;
-        for (int c = lane * 16; c < p.pitch; c += 512)
-            st_global_16(p.values + row * p.pitch + c, make_uint4(0, 0, 0, 0));
-        for (int q = lane; q < p.quads; q += 32)
-            *reinterpret_cast<uint32_t*>(p.scales + fp8_scale_word(row, q, p.row_tiles)) = 0x01010101u * FP8_SCALE_ONE;
-        if (TO == TO_GROUPS && p.copy != nullptr) {
-            constexpr int V = Elem<T>::kPerVec;
-            for (int c = lane * V; c < p.cols; c += 32 * V)
-                st_global_16(static_cast<T*>(p.copy) + row * p.cols + c, make_uint4(0, 0, 0, 0));
+__device__ void zero_padding_rows(const QuantRows& p, uint32_t warp_id, uint32_t n_warps) {
+    if (TO == TO_SLOTS) {
+        const int64_t used = min(static_cast<int64_t>(p.pad_offsets[p.n_groups]), p.layout_rows);
+        for (int64_t row = warp_id; row < used; row += n_warps)
+            if (p.slot_of_row[row] < 0) zero_row<T>(p, row);
+    } else {
+        for (uint32_t i = warp_id; i < static_cast<uint32_t>(p.n_groups) * 8; i += n_warps) {  // eight warps per group
+            const int e = static_cast<int>(i >> 3);
+            const int64_t end = min(static_cast<int64_t>(p.pad_offsets[e + 1]), p.layout_rows);
+            for (int64_t row = p.pad_offsets[e] + (p.offsets[e + 1] - p.offsets[e]) + (i & 7); row < end; row += 8) zero_row<T>(p, row);
         }
     }
 }
 
 template <typename T, int TO>
 __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRows p) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
+    constexpr int V = Elem<T>::kPerVec, N = LaneBlock<T>::N, AHEAD = kAhead<T>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     if (TO != TO_ROWS && blockIdx.x >= p.row_blocks) {
-        zero_padding_rows<T, TO>(p, (blockIdx.x - p.row_blocks) * kQWarps + warp,
-                                 (static_cast<int64_t>(gridDim.x) - p.row_blocks) * kQWarps);
+        zero_padding_rows<T, TO>(p, (blockIdx.x - p.row_blocks) * kQWarps + warp, (gridDim.x - p.row_blocks) * kQWarps);
         return;
     }
     const int64_t rows = TO == TO_ROWS && p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
-    const int64_t n_items = rows * p.quads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQWarps + warp; i < n_items; i += p.row_blocks * kQWarps) {
-        const int64_t row = i / p.quads;
-        const int q = static_cast<int>(i - row * p.quads);
-        const int col0 = q * FP8_QUAD + (lane >> 3) * FP8_BLOCK;
-        float x[16];
-        load_lane_block<T>(static_cast<const T*>(p.x) + row * p.x_pitch, col0, p.cols, s, x);
-        uint32_t w[4];
-        const uint32_t word = quantize_lane_block(x, w);
-        const int copies = TO == TO_SLOTS ? p.k : 1;
-        for (int j = 0; j < copies; ++j) {
-            int64_t to = row;
-            if (TO == TO_SLOTS) {
-                to = __ldg(p.row_of_slot + row * p.k + j);
-            } else if (TO == TO_GROUPS) {
-                if (row >= __ldg(p.offsets + p.n_groups)) break;  // a row of no expert
-                const int e = group_of_row(p.offsets, p.n_groups, static_cast<int32_t>(row));
-                to = __ldg(p.pad_offsets + e) + (row - __ldg(p.offsets + e));
+    for (uint32_t i = blockIdx.x * kQWarps + warp; i < p.work.items; i += p.row_blocks * kQWarps) {
+        int64_t row;
+        int q0, q1;
+        p.work.decode(i, row, q0, q1);
+        if (row >= rows) break;
+        int64_t to = row;
+        if (TO == TO_GROUPS) {
+            if (row >= __ldg(p.offsets + p.n_groups)) break;  // from here on: rows of no expert
+            const int e = group_of_row(p.offsets, p.n_groups, static_cast<int32_t>(row));
+            to = __ldg(p.pad_offsets + e) + (row - __ldg(p.offsets + e));
+            if (to >= p.layout_rows) continue;
+        }
+        const T* const src = static_cast<const T*>(p.x) + row * p.x_pitch;
+        for (int qa = q0; qa < q1; qa += AHEAD) {
+            uint4 raw[AHEAD][N];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const int c = (qa + u) * FP8_QUAD + g * FP8_BLOCK + LaneBlock<T>::column(s, j);
+                    raw[u][j] = qa + u < q1 && c < p.cols ? ld_stream_16(src + c) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int q = qa + u, col0 = q * FP8_QUAD + g * FP8_BLOCK;
+                if (q >= q1) break;
+                float x[16];
+#pragma unroll
+                for (int j = 0; j < N; ++j) Elem<T>::unpack(raw[u][j], x + j * V);
+                uint32_t w[4];
+                const uint32_t word = quantize_lane_block(x, w);
+                const int copies = TO == TO_SLOTS ? p.k : 1;
+                for (int j = 0; j < copies; ++j) {
+                    if (TO == TO_SLOTS) {
+                        to = __ldg(p.row_of_slot + row * p.k + j);
+                        if (to < 0 || to >= p.layout_rows) continue;
+                    }
+                    store_lane_bytes<T>(p.values + to * p.pitch, col0, p.pitch, s, w);
+                    if (lane == 0) *reinterpret_cast<uint32_t*>(p.scales + fp8_scale_word(to, q, p.row_tiles)) = word;
+                }
+                if (TO == TO_GROUPS && p.copy != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const int c = col0 + LaneBlock<T>::column(s, j);
+                        if (c < p.cols) st_global_16(static_cast<T*>(p.copy) + to * p.cols + c, raw[u][j]);
+                    }
+                }
             }
-            if (TO != TO_ROWS && (to < 0 || to >= p.layout_rows)) continue;
-            store_lane_bytes<T>(p.values + to * p.pitch, col0, p.pitch, s, w);
-            if (lane == 0) *reinterpret_cast<uint32_t*>(p.scales + fp8_scale_word(to, q, p.row_tiles)) = word;
-            if (TO == TO_GROUPS && p.copy != nullptr)
-                store_lane_block<T>(static_cast<T*>(p.copy) + to * p.cols, col0, p.cols, s, x);
         }
     }
 }
@@ -212,30 +255,45 @@ struct Dequant {
     void* out;
     const int32_t* rows_used;  // rows from here on are left alone; null: all rows
     int64_t rows, row_tiles;   // rows over the whole batch
-    int32_t rows_per, tiles_per, cols, pitch, quads;  // of one matrix of the batch
+    RowItems work;
+    int32_t batch, rows_per, tiles_per, cols, pitch;  // of one matrix of the batch
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) dequantize_rows_kernel(const Dequant p) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
+    constexpr int AHEAD = 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
-    const int64_t n_items = rows * p.quads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQWarps + warp; i < n_items; i += static_cast<int64_t>(gridDim.x) * kQWarps) {
-        const int64_t row = i / p.quads;
-        const int q = static_cast<int>(i - row * p.quads);
-        const int64_t b = row / p.rows_per;
-        const int64_t scale_row = b * p.tiles_per * FP8_TILE_ROWS + (row - b * p.rows_per);
-        const int col0 = q * FP8_QUAD + (lane >> 3) * FP8_BLOCK;
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(p.scales + fp8_scale_word(scale_row, q, p.row_tiles));
-        const float factor = fp8_factor((word >> (8 * (lane >> 3))) & 0xffu);
-        uint32_t w[4];
-        float x[16];
-        load_lane_bytes<T>(p.values + row * p.pitch, col0, p.pitch, s, w);
+    for (uint32_t i = blockIdx.x * kQWarps + warp; i < p.work.items; i += gridDim.x * kQWarps) {
+        int64_t row;
+        int q0, q1;
+        p.work.decode(i, row, q0, q1);
+        if (row >= rows) break;
+        int64_t scale_row = row;
+        if (p.batch > 1) {
+            const uint32_t b = static_cast<uint32_t>(row) / static_cast<uint32_t>(p.rows_per);
+            scale_row = static_cast<int64_t>(b) * p.tiles_per * FP8_TILE_ROWS + (row - static_cast<int64_t>(b) * p.rows_per);
+        }
+        for (int qa = q0; qa < q1; qa += AHEAD) {
+            uint32_t w[AHEAD][4], word[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) fp8_unpack4(w[j], factor, x + 4 * j);
+            for (int u = 0; u < AHEAD; ++u) {
+                if (qa + u >= q1) break;
+                load_lane_bytes<T>(p.values + row * p.pitch, (qa + u) * FP8_QUAD + g * FP8_BLOCK, p.pitch, s, w[u]);
+                word[u] = *reinterpret_cast<const uint32_t*>(p.scales + fp8_scale_word(scale_row, qa + u, p.row_tiles));
+            }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = finite_in<T>(x[j]);
-        store_lane_block<T>(static_cast<T*>(p.out) + row * p.cols, col0, p.cols, s, x);
+            for (int u = 0; u < AHEAD; ++u) {
+                if (qa + u >= q1) break;
+                const float factor = fp8_factor((word[u] >> (8 * g)) & 0xffu);
+                float x[16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fp8_unpack4(w[u][j], factor, x + 4 * j);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = finite_in<T>(x[j]);
+                store_lane_block<T>(static_cast<T*>(p.out) + row * p.cols, (qa + u) * FP8_QUAD + g * FP8_BLOCK, p.cols, s, x);
+            }
+        }
     }
 }
 
@@ -258,17 +316,19 @@ struct SwigluFp8 {
     uint8_t *gate8, *gate_scales, *up8, *up_scales, *out8, *out_scales;
     const int32_t* rows_used;
     int64_t rows, row_tiles;
-    int32_t cols, pitch, quads;
+    RowItems work;
+    int32_t cols, pitch;
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) swiglu_fp8_forward_kernel(const SwigluFp8 p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
-    const int64_t n_items = rows * p.quads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQWarps + warp; i < n_items; i += static_cast<int64_t>(gridDim.x) * kQWarps) {
-        const int64_t row = i / p.quads;
-        const int q = static_cast<int>(i - row * p.quads);
+    for (uint32_t i = blockIdx.x * kQWarps + warp; i < p.work.items; i += gridDim.x * kQWarps) {
+        int64_t row;
+        int q, q1;
+        p.work.decode(i, row, q, q1);
+        if (row >= rows) break;
         const int col0 = q * FP8_QUAD + (lane >> 3) * FP8_BLOCK;
         const int64_t scale_at = fp8_scale_word(row, q, p.row_tiles);
         float g[16], u[16];
@@ -302,10 +362,11 @@ template <typename T>
 __global__ void __launch_bounds__(kQThreads) swiglu_fp8_backward_kernel(const SwigluFp8 p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
-    const int64_t n_items = rows * p.quads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kQWarps + warp; i < n_items; i += static_cast<int64_t>(gridDim.x) * kQWarps) {
-        const int64_t row = i / p.quads;
-        const int q = static_cast<int>(i - row * p.quads);
+    for (uint32_t i = blockIdx.x * kQWarps + warp; i < p.work.items; i += gridDim.x * kQWarps) {
+        int64_t row;
+        int q, q1;
+        p.work.decode(i, row, q, q1);
+        if (row >= rows) break;
         const int col0 = q * FP8_QUAD + (lane >> 3) * FP8_BLOCK;
         const int64_t scale_at = fp8_scale_word(row, q, p.row_tiles);
         uint32_t wg[4], wu[4];
@@ -413,10 +474,23 @@ __global__ void __launch_bounds__(kMapThreads) group_maps_kernel(const GroupMaps
 }
 
 // ---- host side -------------------------------------------------------------------------------------
-static int64_t row_grid(int64_t items) {
+static uint32_t row_grid(int64_t items) {
     const int64_t want = (items + kQWarps - 1) / kQWarps;
     const int64_t cap = static_cast<int64_t>(sm_count()) * 64;
-    return want < 1 ? 1 : (want > cap ? cap : want);
+    return static_cast<uint32_t>(want < 1 ? 1 : (want > cap ? cap : want));
+}
+// `most` groups of 512 columns per item at most; fewer where the rows alone would not give every SM 16 warps.
+static int make_items(RowItems& w, int64_t rows, int64_t cols, int most) {
+    w.quads = static_cast<int32_t>(fp8_quads(cols));
+    const int64_t warps = 16LL * sm_count();
+    w.per_item = w.quads < most ? w.quads : most;
+    while (w.per_item > 1 && rows * ((w.quads + w.per_item - 1) / w.per_item) < warps) w.per_item = (w.per_item + 1) / 2;
+    w.parts = static_cast<uint32_t>((w.quads + w.per_item - 1) / w.per_item);
+    const int64_t items = rows * w.parts;
+    FMAB_REQUIRE(items < (1LL << 32) - (1LL << 24), FMA_B200_ERR_BAD_ARG, "rows=%lld of %lld columns are too many", (long long)rows,
+                 (long long)cols);
+    w.items = static_cast<uint32_t>(items);
+    return FMA_B200_OK;
 }
 
 static int check_rows_cols(int32_t dtype, int64_t rows, int64_t cols) {
@@ -434,11 +508,10 @@ static int check_pitch(const char* what, int32_t dtype, int64_t pitch, int64_t c
 
 template <int TO>
 static int launch_quantize(QuantRows& p, int32_t dtype, int64_t extra_rows, cudaStream_t s) {
-    p.row_blocks = row_grid(p.rows * p.quads);
-    int64_t grid = p.row_blocks;
-    if (TO != TO_ROWS) grid += row_grid(extra_rows);
+    p.row_blocks = row_grid(p.work.items);
+    const uint32_t grid = p.row_blocks + (TO != TO_ROWS ? row_grid(extra_rows) : 0);
     dispatch_dtype(dtype, [&](auto tag) {
-        quantize_rows_kernel<decltype(tag), TO><<<static_cast<unsigned>(grid), kQThreads, 0, s>>>(p);
+        quantize_rows_kernel<decltype(tag), TO><<<grid, kQThreads, 0, s>>>(p);
     });
     return check_launch("fp8_quantize");
 }
@@ -456,7 +529,7 @@ static int fill_quantize(QuantRows& p, const void* x, int64_t x_pitch, int32_t d
     p.row_tiles = fp8_row_tiles(layout_rows);
     p.cols = static_cast<int32_t>(cols);
     p.pitch = static_cast<int32_t>(fp8_pitch(cols));
-    p.quads = static_cast<int32_t>(fp8_quads(cols));
+    if (int rc = make_items(p.work, rows, cols, 8)) return rc;
     p.values = static_cast<uint8_t*>(values);
     p.scales = static_cast<uint8_t*>(scales);
     if (rows == 0) return FMA_B200_OK;
@@ -498,7 +571,7 @@ int fma_b200_fp8_quantize_groups(const void* x, int64_t x_pitch, int32_t dtype, 
     p.offsets = offsets;
     p.pad_offsets = pad_offsets;
     p.n_groups = E;
-    return launch_quantize<TO_GROUPS>(p, dtype, E * 64LL, static_cast<cudaStream_t>(stream));
+    return launch_quantize<TO_GROUPS>(p, dtype, E * 8LL, static_cast<cudaStream_t>(stream));
 }
 
 int fma_b200_fp8_quantize_scatter(const void* x, int32_t dtype, int64_t T, int64_t cols, int32_t k,
@@ -567,12 +640,12 @@ int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batc
     p.rows_per = static_cast<int32_t>(rows);
     p.tiles_per = static_cast<int32_t>(fp8_row_tiles(rows));
     p.row_tiles = static_cast<int64_t>(batch) * p.tiles_per;
+    p.batch = batch;
     p.cols = static_cast<int32_t>(cols);
     p.pitch = static_cast<int32_t>(fp8_pitch(cols));
-    p.quads = static_cast<int32_t>(fp8_quads(cols));
+    if (int rc = make_items(p.work, p.rows, cols, 8)) return rc;
     dispatch_dtype(dtype, [&](auto tag) {
-        dequantize_rows_kernel<decltype(tag)><<<static_cast<unsigned>(row_grid(p.rows * p.quads)), kQThreads, 0,
-                                                static_cast<cudaStream_t>(stream)>>>(p);
+        dequantize_rows_kernel<decltype(tag)><<<row_grid(p.work.items), kQThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
     });
     return check_launch("fp8_dequantize");
 }
@@ -639,9 +712,9 @@ int fma_b200_swiglu_fp8_forward(const void* gate, int64_t gate_pitch, const void
     p.row_tiles = fp8_row_tiles(rows);
     p.cols = static_cast<int32_t>(cols);
     p.pitch = static_cast<int32_t>(fp8_pitch(cols));
-    p.quads = static_cast<int32_t>(fp8_quads(cols));
+    if (int rc = make_items(p.work, rows, cols, 1)) return rc;
     dispatch_dtype(dtype, [&](auto tag) {
-        swiglu_fp8_forward_kernel<decltype(tag)><<<static_cast<unsigned>(row_grid(rows * p.quads)), kQThreads, 0,
+        swiglu_fp8_forward_kernel<decltype(tag)><<<row_grid(p.work.items), kQThreads, 0,
                                                    static_cast<cudaStream_t>(stream)>>>(p);
     });
     return check_launch("swiglu_fp8_forward");
@@ -677,9 +750,9 @@ int fma_b200_swiglu_fp8_backward(const void* gate8, const void* gate_scales, con
     p.row_tiles = fp8_row_tiles(rows);
     p.cols = static_cast<int32_t>(cols);
     p.pitch = static_cast<int32_t>(fp8_pitch(cols));
-    p.quads = static_cast<int32_t>(fp8_quads(cols));
+    if (int rc = make_items(p.work, rows, cols, 1)) return rc;
     dispatch_dtype(dtype, [&](auto tag) {
-        swiglu_fp8_backward_kernel<decltype(tag)><<<static_cast<unsigned>(row_grid(rows * p.quads)), kQThreads, 0,
+        swiglu_fp8_backward_kernel<decltype(tag)><<<row_grid(p.work.items), kQThreads, 0,
                                                     static_cast<cudaStream_t>(stream)>>>(p);
     });
     return check_launch("swiglu_fp8_backward");
