@@ -141,6 +141,44 @@ __device__ __forceinline__ void load_lane_bytes(const uint8_t* row, int col0, in
         }
     }
 }
+// The 16-bit types' magnitudes are compared two at a time as integers, and only a block with an infinity or NaN takes
+// the general way (150 instructions per 16 values, against about 75).
+template <typename T>
+struct Magnitude16 {
+    static constexpr bool kPacked = false;
+};
+template <>
+struct Magnitude16<__nv_bfloat16> {
+    static constexpr bool kPacked = true;
+    static constexpr uint32_t kInf = 0x7f80;
+    __device__ static __forceinline__ uint32_t float_bits(uint32_t m) { return m << 16; }
+};
+template <>
+struct Magnitude16<__half> {
+    static constexpr bool kPacked = true;
+    static constexpr uint32_t kInf = 0x7c00;
+    __device__ static __forceinline__ uint32_t float_bits(uint32_t m) {
+        return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+    }
+};
+__device__ __forceinline__ uint32_t max_magnitudes16(uint32_t m, const uint4& v) {
+    m = __vmaxu2(m, v.x & 0x7fff7fffu);
+    m = __vmaxu2(m, v.y & 0x7fff7fffu);
+    m = __vmaxu2(m, v.z & 0x7fff7fffu);
+    return __vmaxu2(m, v.w & 0x7fff7fffu);
+}
+// Four finite values, scaled, as e4m3 bytes.
+__device__ __forceinline__ uint32_t fp8_pack4_finite(const float* x, float inverse) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inverse, x[1] * inverse), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inverse, x[3] * inverse), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
+// The warp's scale word (all lanes) from each lane's scale byte.
+__device__ __forceinline__ uint32_t scale_word_of(uint32_t byte) {
+    uint32_t word = byte << (8 * ((threadIdx.x & 31) >> 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    return word | __shfl_xor_sync(0xffffffffu, word, 16);
+}
 // Scale byte of the 8 lanes' block and its 16 packed values per lane; returns the warp's scale word (all lanes).
 __device__ __forceinline__ uint32_t quantize_lane_block(const float* x, uint32_t* w) {
     uint32_t m = 0;
@@ -150,10 +188,26 @@ __device__ __forceinline__ uint32_t quantize_lane_block(const float* x, uint32_t
     const float inverse = fp8_inverse(byte);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = fp8_pack4(x + 4 * i, inverse);
-    uint32_t word = byte << (8 * ((threadIdx.x & 31) >> 3));
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    word |= __shfl_xor_sync(0xffffffffu, word, 16);
-    return word;
+    return scale_word_of(byte);
+}
+// The same from the lane's values as they were loaded.
+template <typename T>
+__device__ __forceinline__ uint32_t quantize_lane_raw(const uint4* raw, uint32_t* w) {
+    float x[16];
+#pragma unroll
+    for (int j = 0; j < LaneBlock<T>::N; ++j) Elem<T>::unpack(raw[j], x + j * LaneBlock<T>::V);
+    if constexpr (Magnitude16<T>::kPacked) {
+        const uint32_t pair = max_magnitudes16(max_magnitudes16(0, raw[0]), raw[1]);
+        const uint32_t m = max_over_8_lanes(max(pair & 0xffffu, pair >> 16));
+        if (!__any_sync(0xffffffffu, m >= Magnitude16<T>::kInf)) {
+            const uint32_t byte = fp8_scale_byte(Magnitude16<T>::float_bits(m));
+            const float inverse = fp8_inverse(byte);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = fp8_pack4_finite(x + 4 * i, inverse);
+            return scale_word_of(byte);
+        }
+    }
+    return quantize_lane_block(x, w);
 }
 
 }  // namespace fmab

@@ -175,11 +175,8 @@ __global__ void __launch_bounds__(kFewThreads, 3) few_rows_kernel(const __grid_c
             for (int u = 0; u < AHEAD; ++u) {
                 const int i = i0 + u * kFewWarps, q = i / rows, r = i - q * rows, kb = 4 * q + g;
                 if (i >= n) break;
-                float v[16];
-                Elem<T>::unpack(raw[u][0], v);
-                Elem<T>::unpack(raw[u][1], v + 8);
                 uint32_t w[4];
-                const uint32_t word = quantize_lane_block(v, w);
+                const uint32_t word = quantize_lane_raw<T>(raw[u], w);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int c = LaneBlock<T>::column(s, j);

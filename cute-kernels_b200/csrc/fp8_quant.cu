@@ -70,7 +70,8 @@ __device__ __forceinline__ void zero_row(const QuantRows& p, int64_t row) {
     }
 }
 
-// Padding rows of the layout below its used end: zero values, zero copies.
+// Padding rows: zero values, zero copies.  slots: all below the layout's used end, since whole tiles are written from
+// them; groups: up to a multiple of 64, the rows that the weight gradient reads.
 template <typename T, int TO>
 __device__ void zero_padding_rows(const QuantRows& p, uint32_t warp_id, uint32_t n_warps) {
     if (TO == TO_SLOTS) {
@@ -80,15 +81,16 @@ __device__ void zero_padding_rows(const QuantRows& p, uint32_t warp_id, uint32_t
     } else {
         for (uint32_t i = warp_id; i < static_cast<uint32_t>(p.n_groups) * 8; i += n_warps) {  // eight warps per group
             const int e = static_cast<int>(i >> 3);
-            const int64_t end = min(static_cast<int64_t>(p.pad_offsets[e + 1]), p.layout_rows);
-            for (int64_t row = p.pad_offsets[e] + (p.offsets[e + 1] - p.offsets[e]) + (i & 7); row < end; row += 8) zero_row<T>(p, row);
+            const int64_t count = p.offsets[e + 1] - p.offsets[e], first = p.pad_offsets[e];
+            const int64_t end = min(first + (count + 63) / 64 * 64, p.layout_rows);
+            for (int64_t row = first + count + (i & 7); row < end; row += 8) zero_row<T>(p, row);
         }
     }
 }
 
 template <typename T, int TO>
 __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRows p) {
-    constexpr int V = Elem<T>::kPerVec, N = LaneBlock<T>::N, AHEAD = kAhead<T>;
+    constexpr int N = LaneBlock<T>::N, AHEAD = kAhead<T>;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     if (TO != TO_ROWS && blockIdx.x >= p.row_blocks) {
         zero_padding_rows<T, TO>(p, (blockIdx.x - p.row_blocks) * kQWarps + warp, (gridDim.x - p.row_blocks) * kQWarps);
@@ -121,11 +123,8 @@ __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRow
             for (int u = 0; u < AHEAD; ++u) {
                 const int q = qa + u, col0 = q * FP8_QUAD + g * FP8_BLOCK;
                 if (q >= q1) break;
-                float x[16];
-#pragma unroll
-                for (int j = 0; j < N; ++j) Elem<T>::unpack(raw[u][j], x + j * V);
                 uint32_t w[4];
-                const uint32_t word = quantize_lane_block(x, w);
+                const uint32_t word = quantize_lane_raw<T>(raw[u], w);
                 const int copies = TO == TO_SLOTS ? p.k : 1;
                 for (int j = 0; j < copies; ++j) {
                     if (TO == TO_SLOTS) {
@@ -183,21 +182,38 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const QuantWeight 
 #pragma unroll
         for (int j = 0; j < 8 / V; ++j)
             raw[i][j] = (r0 + i < p.N && c0 < p.K) ? ld_stream_16(src + static_cast<int64_t>(i) * p.K + j * V) : make_uint4(0, 0, 0, 0);
+    auto block_max = [&](uint32_t m) {
+        m = __reduce_max_sync(0xffffffffu, m);
+        if ((tid & 31) == 0) warp_max[tid >> 5] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, warp_max[i]);
+        return m;
+    };
     uint32_t m = 0;
+    bool finite = false;
+    if constexpr (Magnitude16<T>::kPacked) {
+        uint32_t pair = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i) pair = max_magnitudes16(pair, raw[i][0]);
+        m = block_max(max(pair & 0xffffu, pair >> 16));
+        finite = m < Magnitude16<T>::kInf;
+        m = Magnitude16<T>::float_bits(m);
+        if (!finite) __syncthreads();  // warp_max is written again
+    }
+    if (!finite) {
+        m = 0;
 #pragma unroll
-        for (int j = 0; j < 8 / V; ++j) {
-            float x[V];
-            Elem<T>::unpack(raw[i][j], x);
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int v = 0; v < V; ++v) m = max(m, fp8_magnitude(x[v]));
-        }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if ((tid & 31) == 0) warp_max[tid >> 5] = m;
-    __syncthreads();
+            for (int j = 0; j < 8 / V; ++j) {
+                float x[V];
+                Elem<T>::unpack(raw[i][j], x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, warp_max[i]);
+                for (int v = 0; v < V; ++v) m = max(m, fp8_magnitude(x[v]));
+            }
+        m = block_max(m);
+    }
     const uint32_t byte = fp8_scale_byte(m);
     const float inverse = fp8_inverse(byte);
     uint32_t lo[8], hi[8];
@@ -206,8 +222,8 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const QuantWeight 
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8 / V; ++j) Elem<T>::unpack(raw[i][j], x + j * V);
-        lo[i] = fp8_pack4(x, inverse);
-        hi[i] = fp8_pack4(x + 4, inverse);
+        lo[i] = finite ? fp8_pack4_finite(x, inverse) : fp8_pack4(x, inverse);
+        hi[i] = finite ? fp8_pack4_finite(x + 4, inverse) : fp8_pack4(x + 4, inverse);
         if (r0 + i < p.N && c0 < p.pitch)
             *reinterpret_cast<uint2*>(p.values + (static_cast<int64_t>(e) * p.N + r0 + i) * p.pitch + c0) = make_uint2(lo[i], hi[i]);
     }
@@ -331,19 +347,29 @@ __global__ void __launch_bounds__(kQThreads) swiglu_fp8_forward_kernel(const Swi
         if (row >= rows) break;
         const int col0 = q * FP8_QUAD + (lane >> 3) * FP8_BLOCK;
         const int64_t scale_at = fp8_scale_word(row, q, p.row_tiles);
-        float g[16], u[16];
-        load_lane_block<T>(static_cast<const T*>(p.gate) + row * p.gate_pitch, col0, p.cols, s, g);
-        load_lane_block<T>(static_cast<const T*>(p.up) + row * p.up_pitch, col0, p.cols, s, u);
+        uint4 rg[LaneBlock<T>::N], ru[LaneBlock<T>::N];
+#pragma unroll
+        for (int j = 0; j < LaneBlock<T>::N; ++j) {
+            const int c = col0 + LaneBlock<T>::column(s, j);
+            rg[j] = c < p.cols ? ld_stream_16(static_cast<const T*>(p.gate) + row * p.gate_pitch + c) : make_uint4(0, 0, 0, 0);
+            ru[j] = c < p.cols ? ld_stream_16(static_cast<const T*>(p.up) + row * p.up_pitch + c) : make_uint4(0, 0, 0, 0);
+        }
         uint32_t w[4];
         if (p.gate8 != nullptr) {
-            const uint32_t word = quantize_lane_block(g, w);
+            const uint32_t word = quantize_lane_raw<T>(rg, w);
             store_lane_bytes<T>(p.gate8 + row * p.pitch, col0, p.pitch, s, w);
             if (lane == 0) *reinterpret_cast<uint32_t*>(p.gate_scales + scale_at) = word;
         }
         if (p.up8 != nullptr) {
-            const uint32_t word = quantize_lane_block(u, w);
+            const uint32_t word = quantize_lane_raw<T>(ru, w);
             store_lane_bytes<T>(p.up8 + row * p.pitch, col0, p.pitch, s, w);
             if (lane == 0) *reinterpret_cast<uint32_t*>(p.up_scales + scale_at) = word;
+        }
+        float g[16], u[16];
+#pragma unroll
+        for (int j = 0; j < LaneBlock<T>::N; ++j) {
+            Elem<T>::unpack(rg[j], g + j * LaneBlock<T>::V);
+            Elem<T>::unpack(ru[j], u + j * LaneBlock<T>::V);
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) u[j] = u[j] * g[j] * sigmoid_for<T>(g[j]);
@@ -403,7 +429,7 @@ __global__ void __launch_bounds__(kQThreads) swiglu_fp8_backward_kernel(const Sw
 constexpr int kMapThreads = 1024;
 struct GroupMaps {
     const void* counts;
-    int32_t *offsets, *pad_offsets, *tile_expert, *tile_row, *tile_rows;
+    int32_t *offsets, *pad_offsets, *group_rows, *tile_expert, *tile_row, *tile_rows;
     int64_t rows;
     int32_t index_bytes, E, n_tiles;
 };
@@ -447,6 +473,7 @@ __global__ void __launch_bounds__(kMapThreads) group_maps_kernel(const GroupMaps
     const int32_t rest = static_cast<int32_t>(p.rows) - off[n];
     if (t == 0) pad[n + 1] = pad[n] + (rest + 255) / 256 * 256;
     __syncthreads();
+    if (t < n) p.group_rows[t] = off[t + 1] - off[t];
     if (t <= n) {
         p.offsets[t] = off[t];
         p.pad_offsets[t] = pad[t];
@@ -651,8 +678,8 @@ int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batc
 }
 
 int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, int64_t rows, int64_t layout_rows,
-                            int32_t* offsets, int32_t* pad_offsets, int32_t* tile_expert, int32_t* tile_row,
-                            int32_t* tile_rows, void* stream) {
+                            int32_t* offsets, int32_t* pad_offsets, int32_t* group_rows, int32_t* tile_expert,
+                            int32_t* tile_row, int32_t* tile_rows, void* stream) {
     using namespace fmab;
     FMAB_REQUIRE(index_bytes == 4 || index_bytes == 8, FMA_B200_ERR_UNSUPPORTED, "index_bytes=%d", index_bytes);
     FMAB_REQUIRE(E >= 1 && E <= kMapThreads, FMA_B200_ERR_BAD_ARG, "E=%d not in [1,1024]", E);
@@ -660,7 +687,7 @@ int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, 
                      layout_rows >= (rows + 255) / 256 * 256 + 256LL * (E < rows ? E : rows),
                  FMA_B200_ERR_BAD_ARG, "layout_rows=%lld is too small for %lld rows of %d experts", (long long)layout_rows,
                  (long long)rows, E);
-    FMAB_REQUIRE(counts && offsets && pad_offsets && tile_expert && tile_row && tile_rows, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    FMAB_REQUIRE(counts && offsets && pad_offsets && group_rows && tile_expert && tile_row && tile_rows, FMA_B200_ERR_BAD_ARG, "NULL pointer");
     GroupMaps p;
     p.counts = counts;
     p.index_bytes = index_bytes;
@@ -669,6 +696,7 @@ int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, 
     p.n_tiles = static_cast<int32_t>(layout_rows / 128);
     p.offsets = offsets;
     p.pad_offsets = pad_offsets;
+    p.group_rows = group_rows;
     p.tile_expert = tile_expert;
     p.tile_row = tile_row;
     p.tile_rows = tile_rows;

@@ -77,7 +77,7 @@ SIGNATURES: dict[str, tuple] = {
     "fma_b200_moe_gemm_wgrad": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _I32, _P]),
     "fma_b200_moe_gemm_forward_swiglu": (ctypes.c_int, [_P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _I32, _P]),
     "fma_b200_moe_gemm_dgrad_swiglu": (ctypes.c_int, [_P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _I32, _P]),
-    "fma_b200_linear_wgrad": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P]),
+    "fma_b200_linear_wgrad": (ctypes.c_int, [_P, _P, _P, _I32, _I64, _I32, _I32, _I32, _P, _P, _P]),
     "fma_b200_grouped_gemm_workspace_bytes": (_I64, [_I32, _I64]),
     "fma_b200_grouped_gemm": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P, _I64, _P]),
     "fma_b200_fp8_scale_bytes": (_I64, [_I64, _I64]),
@@ -86,7 +86,7 @@ SIGNATURES: dict[str, tuple] = {
     "fma_b200_fp8_quantize_scatter": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _P, _P, _P, _I32, _I64, _P, _P, _P]),
     "fma_b200_fp8_quantize_weight": (ctypes.c_int, [_P, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P]),
     "fma_b200_fp8_dequantize": (ctypes.c_int, [_P, _P, _I32, _I64, _I64, _P, _P, _I32, _P]),
-    "fma_b200_fp8_group_maps": (ctypes.c_int, [_P, _I32, _I32, _I64, _I64, _P, _P, _P, _P, _P, _P]),
+    "fma_b200_fp8_group_maps": (ctypes.c_int, [_P, _I32, _I32, _I64, _I64, _P, _P, _P, _P, _P, _P, _P]),
     "fma_b200_fp8_gemm": (
         ctypes.c_int,
         [_P, _P, _I64, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _P, _P],

@@ -13,43 +13,42 @@ from __future__ import annotations
 import torch
 
 from .._native import call, dtype_code
-from ..ops.fp8 import (
-    _FEW_ROWS,
-    _FEW_ROWS_MAX_WIDTH,
-    Fp8Weight,
-    _dequantize,
-    _few_rows,
-    _pitch,
-    _quantize_rows,
-    _scale_bytes,
-    ptr,
-    stream_ptr,
-)
+from ..ops.fp8 import _FEW_ROWS, _FEW_ROWS_MAX_WIDTH, Fp8Weight, _dequantize, _few_rows, _Held, _quantize_rows, ptr, stream_ptr
 from ..ops.swiglu import swiglu_packed
 from . import _kernels as K
 
 
-def _quantize_scatter(x: torch.Tensor, maps: K.RowMaps):
+def _quantize_scatter(x: torch.Tensor, maps: K.RowMaps) -> _Held:
     T, H = x.shape
-    values = torch.empty(maps.rows_cap, _pitch(H), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty(_scale_bytes(maps.rows_cap, H), dtype=torch.uint8, device=x.device)
+    held = _Held(maps.rows_cap, H, x.device)
     call("fma_b200_fp8_quantize_scatter", ptr(x), dtype_code(x.dtype), T, H, maps.top_k, ptr(maps.row_of_slot),
-         ptr(maps.slot_of_row), ptr(maps.pad_offsets), maps.num_experts, maps.rows_cap, ptr(values), ptr(scales),
+         ptr(maps.slot_of_row), ptr(maps.pad_offsets), maps.num_experts, maps.rows_cap, held.values, held.scales,
          stream_ptr(x.device))  # fmt: skip
-    return values, scales
+    return held
 
 
-def _product(values, scales, w_values, w_scales, N: int, K_: int, dtype, maps: K.RowMaps) -> torch.Tensor:
-    out = torch.empty(maps.rows_cap, N, dtype=dtype, device=values.device)
-    call("fma_b200_fp8_gemm", ptr(values), ptr(scales), maps.rows_cap, ptr(w_values), ptr(w_scales), maps.num_experts, N,
-         K_, ptr(out), dtype_code(dtype), maps.rows_cap, ptr(maps.mtile_expert), None, None,
-         ptr(maps.pad_offsets[maps.num_experts :]), stream_ptr(values.device))  # fmt: skip
+def _used(maps: K.RowMaps) -> int:
+    """Address of the number of layout rows in use."""
+    return maps.pad_offsets.data_ptr() + 4 * maps.num_experts
+
+
+def _product(a: _Held, w_values, w_scales, N: int, dtype, maps: K.RowMaps) -> torch.Tensor:
+    dev = a.buffer.device
+    out = torch.empty(maps.rows_cap, N, dtype=dtype, device=dev)
+    call("fma_b200_fp8_gemm", a.values, a.scales, maps.rows_cap, ptr(w_values), ptr(w_scales), maps.num_experts, N, a.cols,
+         ptr(out), dtype_code(dtype), maps.rows_cap, ptr(maps.mtile_expert), None, None, _used(maps),
+         stream_ptr(dev))  # fmt: skip
     return out
 
 
-def _empty8(rows: int, cols: int, device):
-    return (torch.empty(rows, _pitch(cols), dtype=torch.float8_e4m3fn, device=device),
-            torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=device))  # fmt: skip
+def _weight_gradient(d_rows: torch.Tensor, a: _Held, maps: K.RowMaps) -> torch.Tensor:
+    """d_rows^T times the values that `a` stands for, per expert over its token rows."""
+    E, N, dtype, dev = maps.num_experts, d_rows.size(1), d_rows.dtype, d_rows.device
+    x = _dequantize(a.values, a.scales, 1, a.rows, (a.rows, a.cols), dtype, dev, _used(maps))
+    d_w = torch.empty(E, N, a.cols, dtype=dtype, device=dev)
+    call("fma_b200_linear_wgrad", ptr(d_rows), ptr(x), ptr(d_w), dtype_code(dtype), a.rows, E, N, a.cols,
+         ptr(maps.pad_offsets), ptr(maps.expert_count), stream_ptr(dev))  # fmt: skip
+    return d_w
 
 
 class Fp8SwigluExperts(torch.autograd.Function):
@@ -58,54 +57,46 @@ class Fp8SwigluExperts(torch.autograd.Function):
         x, weights = x.contiguous(), weights.contiguous()
         T, H = x.shape
         I, dev, cap = held_proj.shape[-1], x.device, maps.rows_cap
-        used = ptr(maps.pad_offsets[maps.num_experts :])
-        x8, x_scales = _quantize_scatter(x, maps)
-        pre = _product(x8, x_scales, held_fc.values, held_fc.scales, 2 * I, H, x.dtype, maps)
+        x8 = _quantize_scatter(x, maps)
+        pre = _product(x8, held_fc.values, held_fc.scales, 2 * I, x.dtype, maps)
         keep = any(ctx.needs_input_grad)
-        up8, up_scales = _empty8(cap, I, dev) if keep else (None, None)
-        gate8, gate_scales = _empty8(cap, I, dev) if keep else (None, None)
-        act8, act_scales = _empty8(cap, I, dev)
+        act8, up8, gate8 = _Held(cap, I, dev), *((_Held(cap, I, dev) if keep else None) for _ in range(2))
+        at = (gate8.values, gate8.scales, up8.values, up8.scales) if keep else (None,) * 4
         call("fma_b200_swiglu_fp8_forward", pre.data_ptr() + I * pre.element_size(), 2 * I, ptr(pre), 2 * I, None, I,
-             dtype_code(x.dtype), cap, I, used, ptr(gate8), ptr(gate_scales), ptr(up8), ptr(up_scales), ptr(act8),
-             ptr(act_scales), stream_ptr(dev))  # fmt: skip
+             dtype_code(x.dtype), cap, I, _used(maps), *at, act8.values, act8.scales, stream_ptr(dev))  # fmt: skip
         del pre
-        out = _product(act8, act_scales, held_proj.values, held_proj.scales, H, I, x.dtype, maps)
+        out = _product(act8, held_proj.values, held_proj.scales, H, x.dtype, maps)
         y = K.combine(out, weights, maps, T)
-        ctx.save_for_backward(x8, x_scales, up8, up_scales, gate8, gate_scales, act8, act_scales, out, weights,
-                              held_fc.transposed, held_fc.transposed_scales, held_proj.transposed,
-                              held_proj.transposed_scales)  # fmt: skip
+        if keep:
+            ctx.save_for_backward(x8.buffer, up8.buffer, gate8.buffer, act8.buffer, out, weights, held_fc.transposed,
+                                  held_fc.transposed_scales, held_proj.transposed, held_proj.transposed_scales)  # fmt: skip
         ctx.maps, ctx.sizes, ctx.dtype = maps, (T, H, I), x.dtype
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        (x8, x_scales, up8, up_scales, gate8, gate_scales, act8, act_scales, out, weights, fc_t, fc_t_scales, proj_t,
-         proj_t_scales) = ctx.saved_tensors  # fmt: skip
+        x8, up8, gate8, act8, out, weights, fc_t, fc_t_scales, proj_t, proj_t_scales = ctx.saved_tensors
         maps, (T, H, I), dtype, dev = ctx.maps, ctx.sizes, ctx.dtype, dy.device
-        E, cap = maps.num_experts, maps.rows_cap
-        used = maps.pad_offsets[E:]
+        cap, used = maps.rows_cap, _used(maps)
+        x8 = _Held(cap, H, dev, x8)
+        up8, gate8, act8 = (_Held(cap, I, dev, b) for b in (up8, gate8, act8))
         need_x, need_w, need_fc, need_proj = ctx.needs_input_grad[:4]
-        d_out, d_w = K.combine_backward(dy.contiguous(), out, weights, maps, need_w)
-        d_x = d_w_fc = d_w_proj = None
-        if need_proj:
-            act = _dequantize(act8, act_scales, 1, cap, (cap, I), dtype, used)
-            d_w_proj = K.gemm_wgrad(d_out, act, E, maps.pad_offsets)
-            del act
-        if need_x or need_fc:
-            d8, d_scales = _quantize_rows(d_out, used)
-            d_act = _product(d8, d_scales, proj_t, proj_t_scales, I, H, dtype, maps)
-            d_pre = torch.empty(cap, 2 * I, dtype=dtype, device=dev)
-            call("fma_b200_swiglu_fp8_backward", ptr(gate8), ptr(gate_scales), ptr(up8), ptr(up_scales), ptr(d_act), I,
-                 d_pre.data_ptr() + I * d_pre.element_size(), 2 * I, ptr(d_pre), 2 * I, dtype_code(dtype), cap, I, ptr(used),
-                 stream_ptr(dev))  # fmt: skip
-            if need_fc:
-                xg = _dequantize(x8, x_scales, 1, cap, (cap, H), dtype, used)
-                d_w_fc = K.gemm_wgrad(d_pre, xg, E, maps.pad_offsets)
-                del xg
-            if need_x:
-                d8, d_scales = _quantize_rows(d_pre, used)
-                d_xg = _product(d8, d_scales, fc_t, fc_t_scales, H, 2 * I, dtype, maps)
-                d_x = K.scatter_backward(d_xg, maps, T)
+        with torch.cuda.device(dev):
+            d_out, d_w = K.combine_backward(dy.contiguous(), out, weights, maps, need_w)
+            d_x = d_w_fc = d_w_proj = None
+            if need_proj:
+                d_w_proj = _weight_gradient(d_out, act8, maps)
+            if need_x or need_fc:
+                d_act = _product(_quantize_rows(d_out, used), proj_t, proj_t_scales, I, dtype, maps)
+                d_pre = torch.empty(cap, 2 * I, dtype=dtype, device=dev)
+                call("fma_b200_swiglu_fp8_backward", gate8.values, gate8.scales, up8.values, up8.scales, ptr(d_act), I,
+                     d_pre.data_ptr() + I * d_pre.element_size(), 2 * I, ptr(d_pre), 2 * I, dtype_code(dtype), cap, I, used,
+                     stream_ptr(dev))  # fmt: skip
+                if need_fc:
+                    d_w_fc = _weight_gradient(d_pre, x8, maps)
+                if need_x:
+                    d_xg = _product(_quantize_rows(d_pre, used), fc_t, fc_t_scales, H, dtype, maps)
+                    d_x = K.scatter_backward(d_xg, maps, T)
         return d_x, d_w, d_w_fc, d_w_proj, None, None, None
 
 

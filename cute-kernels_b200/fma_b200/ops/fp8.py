@@ -66,27 +66,54 @@ def _check_cols(name: str, cols: int) -> None:
         raise RuntimeError(f"{name}: the width must be a positive multiple of 8, got {cols}")
 
 
+class _Held:
+    """8-bit rows [rows, cols] on the device: one buffer with the values (row pitch: cols rounded up to 16) and, behind
+    them, the scales in the order in which the tensor cores read them."""
+
+    __slots__ = ("buffer", "rows", "cols", "values", "scales")
+
+    def __init__(self, rows: int, cols: int, device: torch.device, buffer: torch.Tensor | None = None):
+        size = rows * _pitch(cols)
+        if buffer is None:
+            buffer = torch.empty(size + _scale_bytes(rows, cols), dtype=torch.uint8, device=device)
+        self.buffer, self.rows, self.cols = buffer, rows, cols
+        self.values = buffer.data_ptr()
+        self.scales = self.values + size
+
+
 class Fp8Blocks:
-    """A tensor held in 8 bits: e4m3 `values` (rows padded to a multiple of 16 columns), `scales` in the order the
-    tensor cores read them, and the shape, dtype and device it came from."""
+    """A tensor held in 8 bits, with the shape and dtype it came from: e4m3 values and a scale per 128 columns of a row."""
 
-    __slots__ = ("values", "scales", "shape", "dtype")
+    __slots__ = ("_held", "shape", "dtype")
 
-    def __init__(self, values: torch.Tensor, scales: torch.Tensor, shape: torch.Size, dtype: torch.dtype):
-        self.values, self.scales, self.shape, self.dtype = values, scales, shape, dtype
+    def __init__(self, held: _Held, shape: torch.Size, dtype: torch.dtype):
+        self._held, self.shape, self.dtype = held, shape, dtype
+
+    @property
+    def device(self) -> torch.device:
+        return self._held.buffer.device
 
     @property
     def nbytes(self) -> int:
-        return self.values.numel() + self.scales.numel()
+        return self._held.buffer.numel()
+
+    @property
+    def values(self) -> torch.Tensor:
+        """The e4m3 values without their scales, [rows, cols]."""
+        h = self._held
+        pitch = _pitch(h.cols)
+        return h.buffer[: h.rows * pitch].view(torch.float8_e4m3fn).view(h.rows, pitch)[:, : h.cols]
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The values it stands for, rounded to `dtype` (default: the type it was made from)."""
-        return _dequantize(self.values, self.scales, 1, self.values.size(0), self.shape, dtype or self.dtype)
+        h = self._held
+        return _dequantize(h.values, h.scales, 1, h.rows, self.shape, dtype or self.dtype, h.buffer.device)
 
 
 class Fp8Weight:
-    """A weight [N, K] or [E, N, K] held in 8 bits with a scale per 128 x 128 block.  `transposed` is the second copy
-    that input gradients read, or None."""
+    """A weight [N, K] or [E, N, K] held in 8 bits with a scale per 128 x 128 block: e4m3 `values` (row pitch: K rounded
+    up to 16) and `scales` in the order in which the tensor cores read them.  `transposed` is the second copy that input
+    gradients read, or None."""
 
     __slots__ = ("values", "scales", "transposed", "transposed_scales", "shape", "dtype")
 
@@ -100,28 +127,29 @@ class Fp8Weight:
         return self.values.device
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The values it stands for, rounded to `dtype` (default: the type it was made from)."""
         experts = self.shape[0] if len(self.shape) == 3 else 1
-        return _dequantize(self.values, self.scales, experts, self.shape[-2], self.shape, dtype or self.dtype)
+        return _dequantize(self.values.data_ptr(), self.scales.data_ptr(), experts, self.shape[-2], self.shape,
+                           dtype or self.dtype, self.values.device)  # fmt: skip
 
 
-def _dequantize(values, scales, batch: int, rows: int, shape, dtype, rows_used: torch.Tensor | None = None) -> torch.Tensor:
-    out = torch.empty(shape, dtype=dtype, device=values.device)
+def _dequantize(values: int, scales: int, batch: int, rows: int, shape, dtype, device, rows_used: int | None = None) -> torch.Tensor:
     code = dtype_code(dtype)
-    if out.numel():
-        with _on(values.device):
-            call("fma_b200_fp8_dequantize", ptr(values), ptr(scales), batch, rows, shape[-1], ptr(rows_used), ptr(out),
-                 code, stream_ptr(values.device))  # fmt: skip
+    out = torch.empty(shape, dtype=dtype, device=device)
+    if rows:
+        with _on(device):
+            call("fma_b200_fp8_dequantize", values, scales, batch, rows, shape[-1], rows_used, out.data_ptr(), code,
+                 stream_ptr(device))  # fmt: skip
     return out
 
 
-def _quantize_rows(x: torch.Tensor, rows_used: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """x [rows, cols] as _rows_2d gives it -> (values, scales)."""
+def _quantize_rows(x: torch.Tensor, rows_used: int | None = None) -> _Held:
+    """x [rows, cols] as _rows_2d gives it."""
     rows, cols = x.shape
-    values = torch.empty(rows, _pitch(cols), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty(_scale_bytes(rows, cols), dtype=torch.uint8, device=x.device)
-    call("fma_b200_fp8_quantize_rows", ptr(x), x.stride(0), dtype_code(x.dtype), rows, cols, ptr(rows_used), ptr(values),
-         ptr(scales), stream_ptr(x.device))  # fmt: skip
-    return values, scales
+    held = _Held(rows, cols, x.device)
+    call("fma_b200_fp8_quantize_rows", x.data_ptr(), x.stride(0), dtype_code(x.dtype), rows, cols, rows_used, held.values,
+         held.scales, stream_ptr(x.device))  # fmt: skip
+    return held
 
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Blocks:
@@ -133,8 +161,8 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Blocks:
         raise RuntimeError("quantize_fp8: x needs at least one dimension")
     _check_cols("quantize_fp8", x.size(-1))
     with _on(x.device):
-        values, scales = _quantize_rows(_rows_2d(x.detach()))
-    return Fp8Blocks(values, scales, x.shape, x.dtype)
+        held = _quantize_rows(_rows_2d(x.detach()))
+    return Fp8Blocks(held, x.shape, x.dtype)
 
 
 def quantize_fp8_weight(weight: torch.Tensor, transpose: bool = False) -> Fp8Weight:
@@ -164,43 +192,51 @@ def quantize_fp8_weight(weight: torch.Tensor, transpose: bool = False) -> Fp8Wei
 
 
 class GroupMaps:
-    """Where rows that are grouped by expert without alignment lie in the 256-aligned layout (all on the device)."""
+    """Where rows that are grouped by expert without alignment lie in the 256-aligned layout.  One int32 buffer on the
+    device; the attributes are addresses in it."""
 
-    __slots__ = ("offsets", "pad_offsets", "tile_expert", "tile_row", "tile_rows", "layout_rows", "num_experts")
+    __slots__ = ("buffer", "offsets", "pad_offsets", "used", "used_all", "group_rows", "tile_expert", "tile_row", "tile_rows",
+                 "layout_rows", "num_experts")  # fmt: skip
 
     def __init__(self, expert_frequency: torch.Tensor, rows: int):
-        E = expert_frequency.numel()
-        dev = expert_frequency.device
+        E, dev = expert_frequency.numel(), expert_frequency.device
         self.num_experts = E
         self.layout_rows = (rows + 255) // 256 * 256 + 256 * min(E, rows)
         tiles = self.layout_rows // 128
-        buffer = torch.empty(2 * E + 3 + 3 * tiles, dtype=torch.int32, device=dev)
-        self.pad_offsets, self.offsets, self.tile_expert, self.tile_row, self.tile_rows = buffer.split(
-            (E + 2, E + 1, tiles, tiles, tiles))  # fmt: skip
-        call("fma_b200_fp8_group_maps", ptr(expert_frequency), expert_frequency.element_size(), E, rows,
-             self.layout_rows, ptr(self.offsets), ptr(self.pad_offsets), ptr(self.tile_expert), ptr(self.tile_row),
-             ptr(self.tile_rows), stream_ptr(dev))  # fmt: skip
+        self.buffer = torch.empty(3 * E + 3 + 3 * tiles, dtype=torch.int32, device=dev)
+        at = self.buffer.data_ptr()
+        self.pad_offsets = at
+        self.used = at + 4 * E  # rows of the layout that experts use, and with the rows of no expert
+        self.used_all = at + 4 * (E + 1)
+        self.offsets = at + 4 * (E + 2)
+        self.group_rows = at + 4 * (2 * E + 3)
+        self.tile_expert = at + 4 * (3 * E + 3)
+        self.tile_row = self.tile_expert + 4 * tiles
+        self.tile_rows = self.tile_row + 4 * tiles
+        call("fma_b200_fp8_group_maps", expert_frequency.data_ptr(), expert_frequency.element_size(), E, rows,
+             self.layout_rows, self.offsets, self.pad_offsets, self.group_rows, self.tile_expert, self.tile_row,
+             self.tile_rows, stream_ptr(dev))  # fmt: skip
 
 
-def _quantize_groups(x: torch.Tensor, maps: GroupMaps, copy: torch.Tensor | None = None):
+def _quantize_groups(x: torch.Tensor, maps: GroupMaps, copy: torch.Tensor | None = None) -> _Held:
     rows, cols = x.shape
-    values = torch.empty(maps.layout_rows, _pitch(cols), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty(_scale_bytes(maps.layout_rows, cols), dtype=torch.uint8, device=x.device)
-    call("fma_b200_fp8_quantize_groups", ptr(x), x.stride(0), dtype_code(x.dtype), rows, cols, ptr(maps.offsets),
-         ptr(maps.pad_offsets), maps.num_experts, maps.layout_rows, ptr(values), ptr(scales), ptr(copy),
+    held = _Held(maps.layout_rows, cols, x.device)
+    call("fma_b200_fp8_quantize_groups", x.data_ptr(), x.stride(0), dtype_code(x.dtype), rows, cols, maps.offsets,
+         maps.pad_offsets, maps.num_experts, maps.layout_rows, held.values, held.scales, ptr(copy),
          stream_ptr(x.device))  # fmt: skip
-    return values, scales
+    return held
 
 
-def _product(values, scales, w_values, w_scales, E: int, N: int, K: int, dtype: torch.dtype, out_rows: int,
+def _product(a: _Held, w_values: torch.Tensor, w_scales: torch.Tensor, E: int, N: int, dtype: torch.dtype, out_rows: int,
              maps: GroupMaps | None) -> torch.Tensor:
-    """[out_rows, N] = rows of `values` times the rows of the weight copy, both reduced over K."""
-    out = torch.empty(out_rows, N, dtype=dtype, device=values.device)
+    """[out_rows, N] = rows of `a` times the rows of the weight copy, both reduced over a's columns."""
+    dev = a.buffer.device
+    out = torch.empty(out_rows, N, dtype=dtype, device=dev)
     tables = (None, None, None, None)
     if maps is not None:
-        tables = (maps.tile_expert, maps.tile_row, maps.tile_rows, maps.pad_offsets[E + 1 :])
-    call("fma_b200_fp8_gemm", ptr(values), ptr(scales), values.size(0), ptr(w_values), ptr(w_scales), E, N, K, ptr(out),
-         dtype_code(dtype), out_rows, *(ptr(t) for t in tables), stream_ptr(values.device))  # fmt: skip
+        tables = (maps.tile_expert, maps.tile_row, maps.tile_rows, maps.used_all)
+    call("fma_b200_fp8_gemm", a.values, a.scales, a.rows, w_values.data_ptr(), w_scales.data_ptr(), E, N, a.cols,
+         out.data_ptr(), dtype_code(dtype), out_rows, *tables, stream_ptr(dev))  # fmt: skip
     return out
 
 
@@ -221,15 +257,14 @@ def _few_rows(x: torch.Tensor, held: Fp8Weight, E: int, N: int, K: int, expert_f
 
 def _forward(x: torch.Tensor, held: Fp8Weight, expert_frequency):
     """The product, the row maps and the 8-bit rows it ran on."""
-    N, K = held.shape[-2:]
-    E = held.shape[0] if len(held.shape) == 3 else 1
-    maps = None
-    if expert_frequency is not None:
-        maps = GroupMaps(expert_frequency, x.size(0))
-        values, scales = _quantize_groups(x, maps)
+    N = held.shape[-2]
+    if expert_frequency is None:
+        maps, rows = None, _quantize_rows(x)
     else:
-        values, scales = _quantize_rows(x)
-    return _product(values, scales, held.values, held.scales, E, N, K, x.dtype, x.size(0), maps), maps, values, scales
+        maps = GroupMaps(expert_frequency, x.size(0))
+        rows = _quantize_groups(x, maps)
+    E = 1 if maps is None else maps.num_experts
+    return _product(rows, held.values, held.scales, E, N, x.dtype, x.size(0), maps), maps, rows
 
 
 class _LinearFp8(torch.autograd.Function):
@@ -238,44 +273,43 @@ class _LinearFp8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, held: Fp8Weight, expert_frequency):
         N, K = held.shape[-2:]
-        E = held.shape[0] if len(held.shape) == 3 else 1
-        out, maps, values, scales = _forward(x, held, expert_frequency)
-        ctx.maps, ctx.sizes, ctx.dtype = maps, (x.size(0), E, N, K), x.dtype
-        kept = [values, scales] if ctx.needs_input_grad[1] else [None, None]
+        out, maps, rows = _forward(x, held, expert_frequency)
+        ctx.maps, ctx.sizes, ctx.dtype = maps, (x.size(0), N, K), x.dtype
+        kept = [rows.buffer if ctx.needs_input_grad[1] else None]
         kept += [held.transposed, held.transposed_scales] if ctx.needs_input_grad[0] else [None, None]
         ctx.save_for_backward(*kept)
         return out
 
     @staticmethod
     def backward(ctx, d_out):
-        values, scales, turned, turned_scales = ctx.saved_tensors
-        rows, E, N, K = ctx.sizes
-        maps, dtype = ctx.maps, ctx.dtype
-        with _on(d_out.device):
+        buffer, turned, turned_scales = ctx.saved_tensors
+        rows, N, K = ctx.sizes
+        maps, dtype, dev = ctx.maps, ctx.dtype, d_out.device
+        want_x, want_w = ctx.needs_input_grad[:2]
+        d_x = d_w = None
+        with _on(dev):
             d_out = _rows_2d(d_out)
-            d_x = d_w = None
-            want_w = ctx.needs_input_grad[1]
             if maps is None:
-                d_rows = d_out
-                if ctx.needs_input_grad[0]:
-                    d_values, d_scales = _quantize_rows(d_out)
+                E, layout, used = 1, rows, None
+                d_rows = d_out.contiguous()
+                d8 = _quantize_rows(d_out) if want_x else None
             else:
+                E, layout, used = maps.num_experts, maps.layout_rows, maps.used
                 # the same pass lays the rows out for the weight gradient
-                d_rows = torch.empty(maps.layout_rows, N, dtype=dtype, device=d_out.device) if want_w else None
-                d_values, d_scales = _quantize_groups(d_out, maps, d_rows)
-            if ctx.needs_input_grad[0]:
-                d_x = _product(d_values, d_scales, turned, turned_scales, E, K, N, dtype, rows, maps)
+                d_rows = torch.empty(layout, N, dtype=dtype, device=dev) if want_w else None
+                d8 = _quantize_groups(d_out, maps, d_rows)
+            if want_x:
+                d_x = _product(d8, turned, turned_scales, E, K, dtype, rows, maps)
             if want_w:
-                layout = values.size(0)
+                x8 = _Held(layout, K, dev, buffer)
+                x_rows = _dequantize(x8.values, x8.scales, 1, layout, (layout, K), dtype, dev, used)
                 if maps is None:
-                    x_rows = _dequantize(values, scales, 1, layout, (layout, K), dtype)
-                    ends = torch.arange(0, 2 * rows, rows, dtype=torch.int32, device=d_out.device)
+                    ends = torch.arange(0, 2 * rows, rows, dtype=torch.int32, device=dev)
+                    segments, d_w = (ends.data_ptr(), None), torch.empty(N, K, dtype=dtype, device=dev)
                 else:
-                    x_rows = _dequantize(values, scales, 1, layout, (layout, K), dtype, maps.pad_offsets[E:])
-                    ends = maps.pad_offsets
-                d_w = torch.empty((E, N, K) if maps is not None else (N, K), dtype=dtype, device=d_out.device)
-                call("fma_b200_linear_wgrad", ptr(d_rows.contiguous()), ptr(x_rows), ptr(d_w), dtype_code(dtype), layout,
-                     E, N, K, ptr(ends), stream_ptr(d_out.device))  # fmt: skip
+                    segments, d_w = (maps.pad_offsets, maps.group_rows), torch.empty(E, N, K, dtype=dtype, device=dev)
+                call("fma_b200_linear_wgrad", d_rows.data_ptr(), x_rows.data_ptr(), d_w.data_ptr(), dtype_code(dtype), layout,
+                     E, N, K, *segments, stream_ptr(dev))  # fmt: skip
         return d_x, d_w, None, None
 
 
@@ -360,44 +394,43 @@ def grouped_linear_fp8(
 
 
 def _swiglu_fp8(gate: torch.Tensor, up: torch.Tensor, keep: bool):
-    """out, and with `keep` the 8-bit gate and up back to back with their scales."""
+    """out, and with `keep` gate and up in 8 bits: one buffer of twice their rows."""
     shape, cols = gate.shape, gate.size(-1)
     gate, up = _rows_2d(gate), _rows_2d(up)
-    rows, dev, code = gate.size(0), gate.device, dtype_code(gate.dtype)
+    rows, dev = gate.size(0), gate.device
     out = torch.empty(shape, dtype=gate.dtype, device=dev)
-    if not keep:
-        call("fma_b200_swiglu_fp8_forward", gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0), out.data_ptr(), cols,
-             code, rows, cols, None, None, None, None, None, None, None, stream_ptr(dev))  # fmt: skip
-        return out, None, None
-    size, scale_bytes = rows * _pitch(cols), _scale_bytes(rows, cols)
-    held = torch.empty(2 * size, dtype=torch.float8_e4m3fn, device=dev)
-    scales = torch.empty(2 * scale_bytes, dtype=torch.uint8, device=dev)
-    h, s = held.data_ptr(), scales.data_ptr()
+    kept, at = None, (None, None, None, None)
+    if keep:
+        size, scale_bytes = rows * _pitch(cols), _scale_bytes(rows, cols)
+        kept = torch.empty(2 * (size + scale_bytes), dtype=torch.uint8, device=dev)
+        first = kept.data_ptr()
+        at = (first, first + 2 * size, first + size, first + 2 * size + scale_bytes)
     call("fma_b200_swiglu_fp8_forward", gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0), out.data_ptr(), cols,
-         code, rows, cols, None, h, s, h + size, s + scale_bytes, None, None, stream_ptr(dev))  # fmt: skip
-    return out, held, scales
+         dtype_code(gate.dtype), rows, cols, None, *at, None, None, stream_ptr(dev))  # fmt: skip
+    return out, kept
 
 
 class _SwigluFp8Checkpoint(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up):
-        out, held, scales = _swiglu_fp8(gate, up, True)
-        ctx.save_for_backward(held, scales)
+        out, kept = _swiglu_fp8(gate, up, True)
+        ctx.save_for_backward(kept)
         ctx.shape = gate.shape
         return out
 
     @staticmethod
     def backward(ctx, d_out):
-        held, scales = ctx.saved_tensors
+        (kept,) = ctx.saved_tensors
         cols, dev = ctx.shape[-1], d_out.device
         gate_grad = torch.empty(ctx.shape, dtype=d_out.dtype, device=dev)
         up_grad = torch.empty(ctx.shape, dtype=d_out.dtype, device=dev)
         with _on(dev):
             d_out = _rows_2d(d_out)
-            h, s, size, scale_bytes = held.data_ptr(), scales.data_ptr(), held.numel() // 2, scales.numel() // 2
-            call("fma_b200_swiglu_fp8_backward", h, s, h + size, s + scale_bytes, d_out.data_ptr(), d_out.stride(0),
-                 gate_grad.data_ptr(), cols, up_grad.data_ptr(), cols, dtype_code(d_out.dtype), d_out.size(0), cols, None,
-                 stream_ptr(dev))  # fmt: skip
+            rows = d_out.size(0)
+            size, scale_bytes, first = rows * _pitch(cols), _scale_bytes(rows, cols), kept.data_ptr()
+            call("fma_b200_swiglu_fp8_backward", first, first + 2 * size, first + size, first + 2 * size + scale_bytes,
+                 d_out.data_ptr(), d_out.stride(0), gate_grad.data_ptr(), cols, up_grad.data_ptr(), cols,
+                 dtype_code(d_out.dtype), rows, cols, None, stream_ptr(dev))  # fmt: skip
         return gate_grad, up_grad
 
 

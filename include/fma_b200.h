@@ -360,10 +360,11 @@ int fma_b200_moe_gemm_wgrad(const void* dY, const void* X, void* dW, int32_t dty
 /*
  * fma_b200_moe_gemm_wgrad (16-bit types, one segment per expert) for any number of rows: dY and X end at `rows`, and
  * seg_offsets [E+1] at the rows that count; a plain linear map is E = 1 with {0, rows}.  With several experts each
- * segment starts on a multiple of 64 rows and its padding rows are zero.
+ * segment starts on a multiple of 64 rows; seg_rows [E] (may be NULL: all of a segment's rows) is the number of rows to
+ * reduce over in it, of which the last 64-row block is read whole: its rows behind them are zero.
  */
 int fma_b200_linear_wgrad(const void* dY, const void* X, void* dW, int32_t dtype, int64_t rows, int32_t E, int32_t OUT,
-                          int32_t IN, const int32_t* seg_offsets, void* stream);
+                          int32_t IN, const int32_t* seg_offsets, const int32_t* seg_rows, void* stream);
 /*
  * Up projection with SwiGLU in the epilogue: W is [E, 2*I, IN] with rows 0..I-1 = up and
  * I..2I-1 = gate (the chunk order of swiglu_packed, fma/ops/swiglu/__init__.py:153).
@@ -420,8 +421,8 @@ int fma_b200_grouped_gemm(const void* A, const void* B, void* D, const uint32_t*
  * quantize_rows      x [rows, cols] (row pitch x_pitch) -> values, scales, blocks of 1 x 128.  Here and below rows_used
  *                    (device, may be NULL) limits the rows: those from *rows_used on are not touched.
  * quantize_groups    the same for rows that are grouped by expert without alignment: source rows
- *                    [offsets[e], offsets[e+1]) go to layout rows pad_offsets[e].. ; the padding rows below
- *                    pad_offsets[E] become zeros; source rows from offsets[E] on are left out.  copy (may be NULL)
+ *                    [offsets[e], offsets[e+1]) go to layout rows pad_offsets[e].. ; the rows behind an expert's, up to
+ *                    a multiple of 64, become zeros; source rows from offsets[E] on are left out.  copy (may be NULL)
  *                    receives the rows themselves, unquantised, in the same layout [layout_rows, cols].
  * quantize_scatter   token t goes to the k rows row_of_slot[t*k..] of the layout of fma_b200_moe_sort (negative:
  *                    nowhere), padding rows below pad_offsets[E] become zeros: fma_b200_moe_scatter in 8 bits
@@ -447,13 +448,13 @@ int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batc
 /*
  * Maps for rows grouped by expert without alignment: counts [E] (4- or 8-byte integers on the device) rows per
  * expert, rows = rows there are.  Writes offsets[E+1] (running sums, cut off at `rows`), pad_offsets[E+2] (first row of
- * each expert in a layout aligned to 256 rows; entry E+1 is the end with the rows of no expert), and for every
- * 128-row tile of the layout its expert (-1 unused, -2 rows behind the last expert's), first source row and number
+ * each expert in a layout aligned to 256 rows; entry E+1 is the end with the rows of no expert), group_rows[E] (the
+ * counts after the cut), and for every 128-row tile of the layout its expert (-1 unused, -2 rows behind the last expert's), first source row and number
  * of source rows.  layout_rows is a multiple of 256, at least round_up(rows, 256) + 256 * min(E, rows).
  */
 int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, int64_t rows, int64_t layout_rows,
-                            int32_t* offsets, int32_t* pad_offsets, int32_t* tile_expert, int32_t* tile_row,
-                            int32_t* tile_rows, void* stream);
+                            int32_t* offsets, int32_t* pad_offsets, int32_t* group_rows, int32_t* tile_expert,
+                            int32_t* tile_row, int32_t* tile_rows, void* stream);
 /*
  * out[r, :] = a[r, :] . w[e(r)]^T for 8-bit a [layout_rows, K] (1 x 128 blocks) and w [E, N, K] (128 x 128 blocks),
  * fp32 sums, out bfloat16 or half with row pitch N.  tile_expert / tile_row / tile_rows as from group_maps (or the

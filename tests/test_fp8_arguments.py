@@ -46,10 +46,10 @@ def test_entry_points_refuse_bad_arguments():
     assert d(at, at, 1, 4, 16, null, at, 5, null) == UNSUPPORTED
     assert d(at, null, 1, 4, 16, null, at, 1, null) == BAD
     m = lib.fma_b200_fp8_group_maps
-    assert m(at, 2, 4, 100, 2048, at, at, at, at, at, null) == UNSUPPORTED
-    assert m(at, 4, 4, 100, 1024, at, at, at, at, at, null) == BAD  # layout too small: 256 + 4 * 256
-    assert m(at, 4, 1025, 100, 1 << 20, at, at, at, at, at, null) == BAD
-    assert m(null, 4, 4, 100, 2048, at, at, at, at, at, null) == BAD
+    assert m(at, 2, 4, 100, 2048, at, at, at, at, at, at, null) == UNSUPPORTED
+    assert m(at, 4, 4, 100, 1024, at, at, at, at, at, at, null) == BAD  # layout too small: 256 + 4 * 256
+    assert m(at, 4, 1025, 100, 1 << 20, at, at, at, at, at, at, null) == BAD
+    assert m(null, 4, 4, 100, 2048, at, at, at, at, at, at, null) == BAD
     p = lib.fma_b200_fp8_gemm
     assert p(at, at, 256, at, at, 1, 16, 16, at, 0, 256, null, null, null, null, null) == UNSUPPORTED  # fp32 result
     assert p(at, at, 256, at, at, 2, 16, 16, at, 1, 256, null, null, null, null, null) == BAD  # experts without a table
@@ -65,9 +65,9 @@ def test_entry_points_refuse_bad_arguments():
     assert f(at, 16, 1, 4, null, at, 1, 16, 16, null, 4, at, null) == BAD
     assert f(null, 16, 1, 0, null, null, 1, 16, 16, null, 4, null, null) == OK
     v = lib.fma_b200_linear_wgrad
-    assert v(at, at, at, 0, 4, 1, 16, 16, at, null) == UNSUPPORTED
-    assert v(at, at, at, 1, 0, 1, 16, 16, at, null) == BAD
-    assert v(at, at, at, 1, 4, 1, 16, 16, null, null) == BAD
+    assert v(at, at, at, 0, 4, 1, 16, 16, at, null, null) == UNSUPPORTED
+    assert v(at, at, at, 1, 0, 1, 16, 16, at, null, null) == BAD
+    assert v(at, at, at, 1, 4, 1, 16, 16, null, null, null) == BAD
     fw, bw = lib.fma_b200_swiglu_fp8_forward, lib.fma_b200_swiglu_fp8_backward
     assert fw(at, 16, at, 16, at, 16, 1, 4, 12, null, at, at, at, at, null, null, null) == BAD
     assert fw(at, 16, at, 16, at, 16, 1, 4, 16, null, at, null, at, at, null, null, null) == BAD  # values without scales
