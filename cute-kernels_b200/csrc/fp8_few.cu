@@ -117,6 +117,8 @@ __global__ void __launch_bounds__(kFewThreads, 3) few_rows_kernel(const __grid_c
     const int item = blockIdx.x / p.split;
     const int chunk = item / p.tiles, n0 = (item - chunk * p.tiles) * 128;
     int expert, row0, rows;
+    allow_next();
+    wait_for_previous();
     if (!few_locate(p, chunk, expert, row0, rows)) return;  // the whole cluster
     T* const out = static_cast<T*>(p.out) + static_cast<int64_t>(row0) * p.N + n0;
     if (expert < 0) {
@@ -314,20 +316,8 @@ static int launch_few(const FewRows& p, int64_t items, cudaStream_t s) {
         FMAB_CUDA(cudaFuncSetAttribute(few_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024));
         configured[dev] = true;
     }
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(items * p.split));
-    config.blockDim = dim3(kFewThreads);
-    config.dynamicSmemBytes = static_cast<size_t>(few_smem(p.quads_most));
-    config.stream = s;
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = static_cast<unsigned>(p.split);
-    cluster.val.clusterDim.y = 1;
-    cluster.val.clusterDim.z = 1;
-    config.attrs = &cluster;
-    config.numAttrs = 1;
-    FMAB_CUDA(cudaLaunchKernelEx(&config, few_rows_kernel<T>, p));
-    return check_launch("fp8_few_rows");
+    return launch_chained("fp8_few_rows", few_rows_kernel<T>, dim3(static_cast<unsigned>(items * p.split)), kFewThreads,
+                          static_cast<size_t>(few_smem(p.quads_most)), static_cast<unsigned>(p.split), s, p);
 }
 
 }  // namespace fmab

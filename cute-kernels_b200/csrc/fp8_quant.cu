@@ -91,6 +91,8 @@ __device__ void zero_padding_rows(const QuantRows& p, uint32_t warp_id, uint32_t
 template <typename T, int TO>
 __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRows p) {
     constexpr int N = LaneBlock<T>::N, AHEAD = kAhead<T>;
+    allow_next();
+    wait_for_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     if (TO != TO_ROWS && blockIdx.x >= p.row_blocks) {
         zero_padding_rows<T, TO>(p, (blockIdx.x - p.row_blocks) * kQWarps + warp, (gridDim.x - p.row_blocks) * kQWarps);
@@ -169,6 +171,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) quantize_weight_kernel(const QuantWeight p) {
     __shared__ uint32_t warp_max[8];
     __shared__ __align__(16) uint8_t turned[FP8_BLOCK][FP8_BLOCK + 16];
+    allow_next();
+    wait_for_previous();
     constexpr int V = Elem<T>::kPerVec;
     const int tid = threadIdx.x;
     const int kb = blockIdx.x % p.k_blocks;
@@ -277,6 +281,8 @@ struct Dequant {
 
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) dequantize_rows_kernel(const Dequant p) {
+    allow_next();
+    wait_for_previous();
     constexpr int AHEAD = 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
@@ -338,6 +344,8 @@ struct SwigluFp8 {
 
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) swiglu_fp8_forward_kernel(const SwigluFp8 p) {
+    allow_next();
+    wait_for_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
     for (uint32_t i = blockIdx.x * kQWarps + warp; i < p.work.items; i += gridDim.x * kQWarps) {
@@ -386,6 +394,8 @@ __global__ void __launch_bounds__(kQThreads) swiglu_fp8_forward_kernel(const Swi
 
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) swiglu_fp8_backward_kernel(const SwigluFp8 p) {
+    allow_next();
+    wait_for_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
     for (uint32_t i = blockIdx.x * kQWarps + warp; i < p.work.items; i += gridDim.x * kQWarps) {
@@ -437,6 +447,8 @@ struct GroupMaps {
 __global__ void __launch_bounds__(kMapThreads) group_maps_kernel(const GroupMaps p) {
     __shared__ int32_t off[1024 + 2], pad[1024 + 3];
     __shared__ long long scan[kMapThreads];
+    allow_next();
+    wait_for_previous();
     const int t = threadIdx.x;
     long long c = 0;
     if (t < p.E) {
@@ -537,10 +549,11 @@ template <int TO>
 static int launch_quantize(QuantRows& p, int32_t dtype, int64_t extra_rows, cudaStream_t s) {
     p.row_blocks = row_grid(p.work.items);
     const uint32_t grid = p.row_blocks + (TO != TO_ROWS ? row_grid(extra_rows) : 0);
+    int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        quantize_rows_kernel<decltype(tag), TO><<<grid, kQThreads, 0, s>>>(p);
+        rc = launch_chained("fp8_quantize", quantize_rows_kernel<decltype(tag), TO>, dim3(grid), kQThreads, 0, 0, s, p);
     });
-    return check_launch("fp8_quantize");
+    return rc;
 }
 
 static int fill_quantize(QuantRows& p, const void* x, int64_t x_pitch, int32_t dtype, int64_t rows, int64_t cols,
@@ -644,10 +657,12 @@ int fma_b200_fp8_quantize_weight(const void* w, int32_t dtype, int32_t E, int32_
     p.k_blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
     FMAB_REQUIRE(static_cast<int64_t>(p.n_blocks) * p.k_blocks < (1LL << 31), FMA_B200_ERR_BAD_ARG, "N*K overflows");
     const dim3 grid(static_cast<unsigned>(p.n_blocks * p.k_blocks), static_cast<unsigned>(E));
+    int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        quantize_weight_kernel<decltype(tag)><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        rc = launch_chained("fp8_quantize_weight", quantize_weight_kernel<decltype(tag)>, grid, 256, 0, 0,
+                            static_cast<cudaStream_t>(stream), p);
     });
-    return check_launch("fp8_quantize_weight");
+    return rc;
 }
 
 int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batch, int64_t rows, int64_t cols,
@@ -671,10 +686,12 @@ int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batc
     p.cols = static_cast<int32_t>(cols);
     p.pitch = static_cast<int32_t>(fp8_pitch(cols));
     if (int rc = make_items(p.work, p.rows, cols, 8)) return rc;
+    int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        dequantize_rows_kernel<decltype(tag)><<<row_grid(p.work.items), kQThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        rc = launch_chained("fp8_dequantize", dequantize_rows_kernel<decltype(tag)>, dim3(row_grid(p.work.items)), kQThreads, 0, 0,
+                            static_cast<cudaStream_t>(stream), p);
     });
-    return check_launch("fp8_dequantize");
+    return rc;
 }
 
 int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, int64_t rows, int64_t layout_rows,
@@ -700,8 +717,7 @@ int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, 
     p.tile_expert = tile_expert;
     p.tile_row = tile_row;
     p.tile_rows = tile_rows;
-    group_maps_kernel<<<1, kMapThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-    return check_launch("fp8_group_maps");
+    return launch_chained("fp8_group_maps", group_maps_kernel, dim3(1), kMapThreads, 0, 0, static_cast<cudaStream_t>(stream), p);
 }
 
 int fma_b200_swiglu_fp8_forward(const void* gate, int64_t gate_pitch, const void* up, int64_t up_pitch, void* out,
@@ -741,11 +757,12 @@ int fma_b200_swiglu_fp8_forward(const void* gate, int64_t gate_pitch, const void
     p.cols = static_cast<int32_t>(cols);
     p.pitch = static_cast<int32_t>(fp8_pitch(cols));
     if (int rc = make_items(p.work, rows, cols, 1)) return rc;
+    int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        swiglu_fp8_forward_kernel<decltype(tag)><<<row_grid(p.work.items), kQThreads, 0,
-                                                   static_cast<cudaStream_t>(stream)>>>(p);
+        rc = launch_chained("swiglu_fp8_forward", swiglu_fp8_forward_kernel<decltype(tag)>, dim3(row_grid(p.work.items)), kQThreads, 0, 0,
+                            static_cast<cudaStream_t>(stream), p);
     });
-    return check_launch("swiglu_fp8_forward");
+    return rc;
 }
 
 int fma_b200_swiglu_fp8_backward(const void* gate8, const void* gate_scales, const void* up8, const void* up_scales,
@@ -779,11 +796,12 @@ int fma_b200_swiglu_fp8_backward(const void* gate8, const void* gate_scales, con
     p.cols = static_cast<int32_t>(cols);
     p.pitch = static_cast<int32_t>(fp8_pitch(cols));
     if (int rc = make_items(p.work, rows, cols, 1)) return rc;
+    int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        swiglu_fp8_backward_kernel<decltype(tag)><<<row_grid(p.work.items), kQThreads, 0,
-                                                    static_cast<cudaStream_t>(stream)>>>(p);
+        rc = launch_chained("swiglu_fp8_backward", swiglu_fp8_backward_kernel<decltype(tag)>, dim3(row_grid(p.work.items)), kQThreads, 0, 0,
+                            static_cast<cudaStream_t>(stream), p);
     });
-    return check_launch("swiglu_fp8_backward");
+    return rc;
 }
 
 }  // extern "C"

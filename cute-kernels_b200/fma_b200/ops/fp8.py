@@ -47,15 +47,16 @@ def _scale_bytes(rows: int, cols: int) -> int:
 
 def _rows_2d(x: torch.Tensor) -> torch.Tensor:
     """x as [rows, cols] with unit column stride, rows of a single pitch and 16-byte aligned rows; a copy if it has to be."""
-    cols = x.size(-1)
-    if x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0:
-        return x
+    cols, size = x.size(-1), x.element_size()
+    if x.dim() == 2 and x.stride(1) == 1 and x.data_ptr() % 16 == 0:
+        pitch = x.stride(0)
+        if pitch >= cols and pitch * size % 16 == 0:
+            return x
     if x.dim() == 1:
         x = x.unsqueeze(0)
     x = _as_rows(x)
-    size = x.element_size()
     pitch = x.stride(-2) if x.size(-2) > 1 or x.dim() > 2 else cols
-    rows = x.numel() // cols if cols else 0
+    rows = x.numel() // cols
     if pitch < cols or pitch * size % 16 != 0 or x.data_ptr() % 16 != 0:
         x, pitch = x.clone(memory_format=torch.contiguous_format), cols
     return x.as_strided((rows, cols), (pitch, 1))
@@ -115,16 +116,12 @@ class Fp8Weight:
     up to 16) and `scales` in the order in which the tensor cores read them.  `transposed` is the second copy that input
     gradients read, or None."""
 
-    __slots__ = ("values", "scales", "transposed", "transposed_scales", "shape", "dtype")
+    __slots__ = ("values", "scales", "transposed", "transposed_scales", "shape", "dtype", "device")
 
     def __init__(self, values, scales, transposed, transposed_scales, shape: torch.Size, dtype: torch.dtype):
         self.values, self.scales = values, scales
         self.transposed, self.transposed_scales = transposed, transposed_scales
-        self.shape, self.dtype = shape, dtype
-
-    @property
-    def device(self) -> torch.device:
-        return self.values.device
+        self.shape, self.dtype, self.device = shape, dtype, values.device
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The values it stands for, rounded to `dtype` (default: the type it was made from)."""
@@ -248,10 +245,11 @@ _FEW_ROWS_MAX_WIDTH = 1 << 16
 
 
 def _few_rows(x: torch.Tensor, held: Fp8Weight, E: int, N: int, K: int, expert_frequency) -> torch.Tensor:
-    out = torch.empty(x.size(0), N, dtype=x.dtype, device=x.device)
-    index_bytes = 4 if expert_frequency is None else expert_frequency.element_size()
-    call("fma_b200_fp8_few_rows", x.data_ptr(), x.stride(0), dtype_code(x.dtype), x.size(0), held.values.data_ptr(),
-         held.scales.data_ptr(), E, N, K, ptr(expert_frequency), index_bytes, out.data_ptr(), stream_ptr(x.device))  # fmt: skip
+    dev, dtype, rows = x.device, x.dtype, x.size(0)
+    out = torch.empty(rows, N, dtype=dtype, device=dev)
+    counts, index_bytes = (None, 4) if expert_frequency is None else (expert_frequency.data_ptr(), expert_frequency.element_size())
+    call("fma_b200_fp8_few_rows", x.data_ptr(), x.stride(0), dtype_code(dtype), rows, held.values.data_ptr(),
+         held.scales.data_ptr(), E, N, K, counts, index_bytes, out.data_ptr(), stream_ptr(dev))  # fmt: skip
     return out
 
 
@@ -313,14 +311,14 @@ class _LinearFp8(torch.autograd.Function):
         return d_x, d_w, None, None
 
 
-def _linear(name: str, x, weight, expert_frequency, quantized):
+def _check_linear(name: str, x, weight, expert_frequency, quantized) -> None:
     held = weight if isinstance(weight, Fp8Weight) else quantized
     parameter = None if isinstance(weight, Fp8Weight) else weight
     if held is not None and not isinstance(held, Fp8Weight):
         raise RuntimeError(f"{name}: quantized must be what quantize_fp8_weight returns")
     if held is not None and parameter is not None and held.shape != parameter.shape:
         raise RuntimeError(f"{name}: quantized has shape {tuple(held.shape)}, weight {tuple(parameter.shape)}")
-    shape = parameter.shape if parameter is not None else held.shape
+    shape = weight.shape
     _native.require_cuda(x, parameter, expert_frequency)
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise RuntimeError(f"{name}: x must be bfloat16 or float16, got {x.dtype}")
@@ -336,40 +334,51 @@ def _linear(name: str, x, weight, expert_frequency, quantized):
             raise RuntimeError(f"{name}: x must be [rows, {shape[-1]}], got {tuple(x.shape)}")
         if expert_frequency.numel() != shape[0] or expert_frequency.dim() != 1:
             raise RuntimeError(f"{name}: expert_frequency must hold one count for each of the {shape[0]} experts")
+        if not 1 <= shape[0] <= 1024:
+            raise RuntimeError(f"{name}: 1 to 1024 experts, got {shape[0]}")
         if expert_frequency.dtype not in (torch.int32, torch.uint32, torch.int64):
             raise RuntimeError(f"{name}: expert_frequency must be int32, uint32 or int64, got {expert_frequency.dtype}")
-        expert_frequency = expert_frequency.contiguous()
-    for t in (parameter if parameter is not None else held.values, expert_frequency):
+    for t in (weight, held, expert_frequency):
         if t is not None and t.device != x.device:
             raise RuntimeError(f"{name}: x is on {x.device}, another argument on {t.device}")
+    _check_cols(name, shape[-2])
+    _check_cols(name, shape[-1])
+
+
+def _linear(name: str, x, weight, expert_frequency, quantized):
+    _check_linear(name, x, weight, expert_frequency, quantized)
+    if isinstance(weight, Fp8Weight):
+        held, parameter = weight, None
+    else:
+        held, parameter = quantized, weight
+    shape, dims, grouped = weight.shape, x.dim(), expert_frequency is not None
     N, K = shape[-2:]
-    _check_cols(name, N)
-    _check_cols(name, K)
-    lead = x.shape[:-1]
-    rows = x.numel() // K
+    rows = x.size(0) if dims == 2 else x.numel() // K
     grad = torch.is_grad_enabled()
     grad_x = grad and x.requires_grad
     grad_w = grad and parameter is not None and parameter.requires_grad
     if grad_x and held is not None and held.transposed is None:
         raise RuntimeError(f"{name}: the gradient of x needs quantize_fp8_weight(weight, transpose=True)")
     if rows == 0:
-        out = x.new_empty(*lead, N)
+        out = x.new_empty(*x.shape[:-1], N)
         if grad_x or grad_w:  # keep the graph: every gradient is zero
             out = out + (x.sum() if grad_x else 0) * 0 + (parameter.sum() if grad_w else 0) * 0
         return out
     with _on(x.device):
         if held is None:
             held = quantize_fp8_weight(parameter, transpose=grad_x)
-        x2 = x if x.dim() == 2 else x.reshape(rows, K)
+        x2 = _rows_2d(x if dims == 2 else x.reshape(rows, K))
+        if grouped and not expert_frequency.is_contiguous():
+            expert_frequency = expert_frequency.contiguous()
         if grad_x or grad_w:
-            out = _LinearFp8.apply(_rows_2d(x2), parameter, held, expert_frequency)
+            out = _LinearFp8.apply(x2, parameter, held, expert_frequency)
         else:
-            x2, E = _rows_2d(x2), shape[0] if grouped else 1
+            E = shape[0] if grouped else 1
             if rows <= _FEW_ROWS * E and K <= _FEW_ROWS_MAX_WIDTH:
                 out = _few_rows(x2, held, E, N, K, expert_frequency)
             else:
                 out = _forward(x2, held, expert_frequency)[0]
-    return out if x.dim() == 2 else out.view(*lead, N)
+    return out if dims == 2 else out.view(*x.shape[:-1], N)
 
 
 def linear_fp8(x: torch.Tensor, weight: torch.Tensor | Fp8Weight, quantized: Fp8Weight | None = None) -> torch.Tensor:
