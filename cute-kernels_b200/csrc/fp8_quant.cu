@@ -170,7 +170,7 @@ struct QuantWeight {
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_weight_kernel(const QuantWeight p) {
     __shared__ uint32_t warp_max[8];
-    __shared__ __align__(16) uint8_t turned[FP8_BLOCK][FP8_BLOCK + 16];
+    __shared__ __align__(16) uint8_t turned[FP8_BLOCK][FP8_BLOCK];  // 8-byte pieces of column c at piece ^ (c / 8 % 16): no bank conflicts
     allow_next();
     wait_for_previous();
     constexpr int V = Elem<T>::kPerVec;
@@ -243,19 +243,20 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const QuantWeight 
     transpose_4x4(hi[0], hi[1], hi[2], hi[3]);
     transpose_4x4(hi[4], hi[5], hi[6], hi[7]);
     const int tc = (tid & 15) * 8, tr = (tid >> 4) * 8;
+    const int to = tr ^ ((tid & 15) * 8);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        *reinterpret_cast<uint2*>(&turned[tc + j][tr]) = make_uint2(lo[j], lo[4 + j]);
-        *reinterpret_cast<uint2*>(&turned[tc + 4 + j][tr]) = make_uint2(hi[j], hi[4 + j]);
+        *reinterpret_cast<uint2*>(&turned[tc + j][to]) = make_uint2(lo[j], lo[4 + j]);
+        *reinterpret_cast<uint2*>(&turned[tc + 4 + j][to]) = make_uint2(hi[j], hi[4 + j]);
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int piece = i * 256 + tid, col = piece >> 3, at = (piece & 7) * 16;
+        const int piece = i * 256 + tid, col = piece >> 3, at = (piece & 7) * 16, key = (col >> 3) & 15;
         const int k = kb * FP8_BLOCK + col, n = nb * FP8_BLOCK + at;
-        if (k < p.K && n < p.pitch_t)
-            st_global_16(p.values_t + (static_cast<int64_t>(e) * p.K + k) * p.pitch_t + n,
-                         *reinterpret_cast<const uint4*>(&turned[col][at]));
+        uint4 v = *reinterpret_cast<const uint4*>(&turned[col][at ^ ((key & 14) * 8)]);
+        if (key & 1) v = make_uint4(v.z, v.w, v.x, v.y);
+        if (k < p.K && n < p.pitch_t) st_global_16(p.values_t + (static_cast<int64_t>(e) * p.K + k) * p.pitch_t + n, v);
     }
 }
 
