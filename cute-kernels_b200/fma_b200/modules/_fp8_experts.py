@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from .._native import call, dtype_code
-from ..ops.fp8 import _FEW_ROWS, _FEW_ROWS_MAX_WIDTH, Fp8Weight, _dequantize, _few_rows, _Held, _quantize_rows, ptr, stream_ptr
+from ..ops.fp8 import Fp8Weight, _dequantize, _few, _few_rows, _Held, _quantize_rows, ptr, stream_ptr
 from ..ops.swiglu import swiglu_packed
 from . import _kernels as K
 
@@ -103,7 +103,7 @@ class Fp8SwigluExperts(torch.autograd.Function):
 def few(rows: int, held_proj: Fp8Weight) -> bool:
     """Whether `few_tokens` is the faster way for this many routed rows."""
     E, H, I = held_proj.shape
-    return 0 < rows <= _FEW_ROWS * E and max(H, I) <= _FEW_ROWS_MAX_WIDTH
+    return rows > 0 and _few(rows, E, max(H, I))
 
 
 def few_tokens(x, weights, held_fc: Fp8Weight, held_proj: Fp8Weight, maps: K.RowMaps) -> torch.Tensor:

@@ -237,11 +237,14 @@ def _product(a: _Held, w_values: torch.Tensor, w_scales: torch.Tensor, E: int, N
     return out
 
 
-# Up to this many rows per expert the product reads x itself and runs in one launch; above, x is quantised first and the
-# rows share tiles of 256.  Measured with weights of 4096 x 4096: 8.3 us against 17.6 for 16 rows, 12.1 against 16.0 for 32; of
-# 14336 x 4096: 19.6 / 22.7 and 35.6 / 20.6; 128 experts of 1536 x 2048: 81 / 115 for 1024 rows, 102 / 118 for 2048, 158 / 120 for 4096.
-_FEW_ROWS = 16
 _FEW_ROWS_MAX_WIDTH = 1 << 16
+
+
+def _few(rows: int, E: int, K: int) -> bool:
+    """Whether the product that reads x itself, in one launch, is the faster way.  Above, x is quantised by a launch of its
+    own.  Measured with weights of 4096 x 4096: 5.8 us against 7.4 for one row, 7.6 / 7.9 for 16, 12.0 / 8.7 for 32; of
+    14336 x 4096: 13.8 / 16.6, 17.9 / 17.4, 34.2 / 18.4; 128 experts of 1536 x 2048: 81 / 94 for 8 rows each, 101 / 95 for 16."""
+    return rows <= (16 if E == 1 else 12 * E) and K <= _FEW_ROWS_MAX_WIDTH
 
 
 def _few_rows(x: torch.Tensor, held: Fp8Weight, E: int, N: int, K: int, expert_frequency) -> torch.Tensor:
@@ -374,7 +377,7 @@ def _linear(name: str, x, weight, expert_frequency, quantized):
             out = _LinearFp8.apply(x2, parameter, held, expert_frequency)
         else:
             E = shape[0] if grouped else 1
-            if rows <= _FEW_ROWS * E and K <= _FEW_ROWS_MAX_WIDTH:
+            if _few(rows, E, K):
                 out = _few_rows(x2, held, E, N, K, expert_frequency)
             else:
                 out = _forward(x2, held, expert_frequency)[0]

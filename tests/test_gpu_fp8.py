@@ -92,7 +92,7 @@ def test_weight(dtype, shape):
 
 # ---- the linear map --------------------------------------------------------------------------------
 LINEAR = [(1, 8, 8), (1, 128, 16), (5, 1000, 1544), (16, 520, 136), (17, 392, 264), (127, 128, 128), (129, 264, 520), (300, 2056, 1032),
-          (1025, 136, 392)]  # fmt: skip
+          (1025, 136, 392), (9, 4104, 264), (40, 2056, 392), (64, 1024, 2048), (90, 4104, 136), (120, 8200, 72), (33, 520, 8)]  # fmt: skip
 
 
 @pytest.mark.parametrize("dtype", HALF)
@@ -189,6 +189,9 @@ GROUPED = [
     (136, 392, [0, 0, 0, 40]),
     (128, 8, [37]),
     (392, 264, [17] * 40),
+    (2056, 136, [1, 70, 0, 16]),  # reductions that several CTAs share
+    (2056, 136, [20, 0, 0, 0]),
+    (1032, 264, [128, 0, 127, 129, 1, 64, 65, 33]),
 ]
 
 
