@@ -301,7 +301,6 @@ __global__ void __launch_bounds__(kFewThreads, 3) few_rows_kernel(const __grid_c
 // the way in would be repeated by every tile of weights (1 us per row of 4096 columns, measured), so it is a launch of
 // its own here.
 constexpr int kSomeThreads = 192;
-constexpr int kSomeRows = 128;
 constexpr int kSomeStagesMost = 5;
 constexpr int kSomeBoxes = 4;  // loads of 16, 32, 64, 128 rows of x
 constexpr int kSomeQuadsFit = 16;  // scales of 512-column groups beside a 128-column accumulator in 256 columns
