@@ -117,7 +117,7 @@ int fma_b200_linear_wgrad(const void* dY, const void* X, void* dW, int32_t dtype
     FMAB_REQUIRE(dtype == FMA_B200_BF16 || dtype == FMA_B200_F16, FMA_B200_ERR_UNSUPPORTED, "dtype %d", dtype);
     FMAB_REQUIRE(rows >= 1, FMA_B200_ERR_BAD_ARG, "rows=%lld", (long long)rows);
     if (int rc = check_layer_gemm(dtype, (rows + 127) / 128 * 128, E, OUT, IN)) return rc;
-    FMAB_REQUIRE(dW && seg_offsets && dY && X, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    FMAB_REQUIRE(dW && dY && X && (seg_offsets || (E == 1 && !seg_rows)), FMA_B200_ERR_BAD_ARG, "NULL pointer");
     FMAB_REQUIRE(aligned16(dY) && aligned16(X) && aligned16(dW), FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
     return tc2_wgrad(dY, X, dW, rows, E, OUT, IN, seg_offsets, 1, seg_rows, dtype == FMA_B200_F16,
                      static_cast<cudaStream_t>(stream));

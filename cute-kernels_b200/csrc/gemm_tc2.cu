@@ -133,6 +133,10 @@ __device__ __forceinline__ void decode_pair_segment(const GemmParams& p, const P
         a_k0 = 0;
         b_k0 = t.b_k_base;
         len = p.k_len;
+    } else if (p.seg_offsets == nullptr) {  // one expert, all rows
+        a_k0 = 0;
+        b_k0 = 0;
+        len = p.k_len;
     } else {
         const int32_t* o = p.seg_offsets + s * p.n_groups + t.group;
         a_k0 = o[0];
@@ -944,6 +948,7 @@ int tc2_wgrad(const void* dY, const void* X, void* dW, int64_t rows_cap, int E, 
     p.mode = MODE_WGRAD;
     p.seg_offsets = seg_offsets;
     p.seg_rows = seg_rows;
+    p.k_len = static_cast<int32_t>(rows_cap);
     p.n_seg = n_seg;
     p.d = static_cast<__nv_bfloat16*>(dW);
     p.ldd = IN;

@@ -9,8 +9,6 @@ from . import _native
 from .kernel_backend import KernelBackend
 from .modules import Experts, ExpertParallelMoE, MoE, shard_expert_state_dict, unshard_expert_state_dicts
 from .ops import (
-    Fp8Blocks,
-    Fp8Weight,
     continuous_count,
     grouped_gemm,
     grouped_linear_fp8,
@@ -38,8 +36,6 @@ __all__ = [
     "swiglu_packed",
     "pack_sequence",
     "unpack_sequence",
-    "Fp8Blocks",
-    "Fp8Weight",
     "quantize_fp8",
     "quantize_fp8_weight",
     "linear_fp8",
@@ -49,3 +45,9 @@ __all__ = [
     "set_seed",
     "ceil_divide",
 ]
+
+
+def __getattr__(name: str):
+    if name in ("Fp8Blocks", "Fp8Weight"):  # what quantize_fp8 and quantize_fp8_weight return
+        return getattr(_native.binding(), name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

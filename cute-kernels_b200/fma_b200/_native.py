@@ -8,6 +8,7 @@ entry point; the argument types below mirror it.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from ctypes import c_int32, c_int64, c_void_p
 from pathlib import Path
@@ -125,6 +126,24 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = argtypes
         _lib = handle
     return _lib
+
+
+_binding = None
+
+
+def binding():
+    """The torch binding of the 8-bit operators (csrc/torch_fp8.cpp), loaded once; raises if it has not been built."""
+    global _binding
+    if _binding is None:
+        lib()  # the binding is linked against it
+        path = _LIB_PATH.with_name("fma_b200_torch.so")
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build the CUDA kernels with `python cute-kernels_b200/build.py`")
+        spec = importlib.util.spec_from_file_location(path.stem, path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _binding = module
+    return _binding
 
 
 # Kernels launched per entry-point call (the sort is three kernels; status queries launch none).

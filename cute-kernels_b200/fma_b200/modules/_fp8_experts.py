@@ -12,10 +12,42 @@ from __future__ import annotations
 
 import torch
 
-from .._native import call, dtype_code
-from ..ops.fp8 import Fp8Weight, _dequantize, _few, _few_rows, _Held, _quantize_rows, ptr, stream_ptr
+from .. import _native
+from .._native import call, dtype_code, ptr, stream_ptr
 from ..ops.swiglu import swiglu_packed
 from . import _kernels as K
+
+
+class _Held:
+    """8-bit rows [rows, cols] on the device: one buffer with the values (row pitch: cols rounded up to 16) and, behind
+    them, the scales; `values` and `scales` are addresses in it."""
+
+    __slots__ = ("buffer", "rows", "cols", "values", "scales")
+
+    def __init__(self, rows: int, cols: int, device: torch.device, buffer: torch.Tensor | None = None):
+        size = rows * ((cols + 15) // 16 * 16)
+        if buffer is None:
+            scale_bytes = int(_native.lib().fma_b200_fp8_scale_bytes(rows, cols))
+            buffer = torch.empty(size + scale_bytes, dtype=torch.uint8, device=device)
+        self.buffer, self.rows, self.cols = buffer, rows, cols
+        self.values = buffer.data_ptr()
+        self.scales = self.values + size
+
+
+def _quantize_rows(x: torch.Tensor, rows_used: int) -> _Held:
+    held = _Held(*x.shape, x.device)
+    call("fma_b200_fp8_quantize_rows", ptr(x), x.stride(0), dtype_code(x.dtype), held.rows, held.cols, rows_used, held.values,
+         held.scales, stream_ptr(x.device))  # fmt: skip
+    return held
+
+
+def _few_rows(x: torch.Tensor, held, counts: torch.Tensor) -> torch.Tensor:
+    E, N, K_ = held.shape
+    values, scales, _, _ = held.addresses
+    out = torch.empty(x.size(0), N, dtype=x.dtype, device=x.device)
+    call("fma_b200_fp8_few_rows", ptr(x), x.stride(0), dtype_code(x.dtype), x.size(0), values, scales, E, N, K_, ptr(counts),
+         counts.element_size(), ptr(out), stream_ptr(x.device))  # fmt: skip
+    return out
 
 
 def _quantize_scatter(x: torch.Tensor, maps: K.RowMaps) -> _Held:
@@ -32,10 +64,10 @@ def _used(maps: K.RowMaps) -> int:
     return maps.pad_offsets.data_ptr() + 4 * maps.num_experts
 
 
-def _product(a: _Held, w_values, w_scales, N: int, dtype, maps: K.RowMaps) -> torch.Tensor:
+def _product(a: _Held, w_values: int, w_scales: int, N: int, dtype, maps: K.RowMaps) -> torch.Tensor:
     dev = a.buffer.device
     out = torch.empty(maps.rows_cap, N, dtype=dtype, device=dev)
-    call("fma_b200_fp8_gemm", a.values, a.scales, maps.rows_cap, ptr(w_values), ptr(w_scales), maps.num_experts, N, a.cols,
+    call("fma_b200_fp8_gemm", a.values, a.scales, maps.rows_cap, w_values, w_scales, maps.num_experts, N, a.cols,
          ptr(out), dtype_code(dtype), maps.rows_cap, ptr(maps.mtile_expert), None, None, _used(maps),
          stream_ptr(dev))  # fmt: skip
     return out
@@ -44,7 +76,9 @@ def _product(a: _Held, w_values, w_scales, N: int, dtype, maps: K.RowMaps) -> to
 def _weight_gradient(d_rows: torch.Tensor, a: _Held, maps: K.RowMaps) -> torch.Tensor:
     """d_rows^T times the values that `a` stands for, per expert over its token rows."""
     E, N, dtype, dev = maps.num_experts, d_rows.size(1), d_rows.dtype, d_rows.device
-    x = _dequantize(a.values, a.scales, 1, a.rows, (a.rows, a.cols), dtype, dev, _used(maps))
+    x = torch.empty(a.rows, a.cols, dtype=dtype, device=dev)
+    call("fma_b200_fp8_dequantize", a.values, a.scales, 1, a.rows, a.cols, _used(maps), ptr(x), dtype_code(dtype),
+         stream_ptr(dev))  # fmt: skip
     d_w = torch.empty(E, N, a.cols, dtype=dtype, device=dev)
     call("fma_b200_linear_wgrad", ptr(d_rows), ptr(x), ptr(d_w), dtype_code(dtype), a.rows, E, N, a.cols,
          ptr(maps.pad_offsets), ptr(maps.expert_count), stream_ptr(dev))  # fmt: skip
@@ -53,29 +87,31 @@ def _weight_gradient(d_rows: torch.Tensor, a: _Held, maps: K.RowMaps) -> torch.T
 
 class Fp8SwigluExperts(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weights, w_fc, w_proj, held_fc: Fp8Weight, held_proj: Fp8Weight, maps: K.RowMaps):
+    def forward(ctx, x, weights, w_fc, w_proj, held_fc, held_proj, maps: K.RowMaps):
         x, weights = x.contiguous(), weights.contiguous()
         T, H = x.shape
         I, dev, cap = held_proj.shape[-1], x.device, maps.rows_cap
         x8 = _quantize_scatter(x, maps)
-        pre = _product(x8, held_fc.values, held_fc.scales, 2 * I, x.dtype, maps)
+        fc, proj = held_fc.addresses, held_proj.addresses
+        pre = _product(x8, *fc[:2], 2 * I, x.dtype, maps)
         keep = any(ctx.needs_input_grad)
         act8, up8, gate8 = _Held(cap, I, dev), *((_Held(cap, I, dev) if keep else None) for _ in range(2))
         at = (gate8.values, gate8.scales, up8.values, up8.scales) if keep else (None,) * 4
         call("fma_b200_swiglu_fp8_forward", pre.data_ptr() + I * pre.element_size(), 2 * I, ptr(pre), 2 * I, None, I,
              dtype_code(x.dtype), cap, I, _used(maps), *at, act8.values, act8.scales, stream_ptr(dev))  # fmt: skip
         del pre
-        out = _product(act8, held_proj.values, held_proj.scales, H, x.dtype, maps)
+        out = _product(act8, *proj[:2], H, x.dtype, maps)
         y = K.combine(out, weights, maps, T)
         if keep:
-            ctx.save_for_backward(x8.buffer, up8.buffer, gate8.buffer, act8.buffer, out, weights, held_fc.transposed,
-                                  held_fc.transposed_scales, held_proj.transposed, held_proj.transposed_scales)  # fmt: skip
+            ctx.save_for_backward(x8.buffer, up8.buffer, gate8.buffer, act8.buffer, out, weights)
+            ctx.held = held_fc, held_proj  # their transposed copies
         ctx.maps, ctx.sizes, ctx.dtype = maps, (T, H, I), x.dtype
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x8, up8, gate8, act8, out, weights, fc_t, fc_t_scales, proj_t, proj_t_scales = ctx.saved_tensors
+        x8, up8, gate8, act8, out, weights = ctx.saved_tensors
+        fc, proj = (h.addresses for h in ctx.held)
         maps, (T, H, I), dtype, dev = ctx.maps, ctx.sizes, ctx.dtype, dy.device
         cap, used = maps.rows_cap, _used(maps)
         x8 = _Held(cap, H, dev, x8)
@@ -87,7 +123,7 @@ class Fp8SwigluExperts(torch.autograd.Function):
             if need_proj:
                 d_w_proj = _weight_gradient(d_out, act8, maps)
             if need_x or need_fc:
-                d_act = _product(_quantize_rows(d_out, used), proj_t, proj_t_scales, I, dtype, maps)
+                d_act = _product(_quantize_rows(d_out, used), *proj[2:], I, dtype, maps)
                 d_pre = torch.empty(cap, 2 * I, dtype=dtype, device=dev)
                 call("fma_b200_swiglu_fp8_backward", gate8.values, gate8.scales, up8.values, up8.scales, ptr(d_act), I,
                      d_pre.data_ptr() + I * d_pre.element_size(), 2 * I, ptr(d_pre), 2 * I, dtype_code(dtype), cap, I, used,
@@ -95,22 +131,21 @@ class Fp8SwigluExperts(torch.autograd.Function):
                 if need_fc:
                     d_w_fc = _weight_gradient(d_pre, x8, maps)
                 if need_x:
-                    d_xg = _product(_quantize_rows(d_pre, used), fc_t, fc_t_scales, H, dtype, maps)
+                    d_xg = _product(_quantize_rows(d_pre, used), *fc[2:], H, dtype, maps)
                     d_x = K.scatter_backward(d_xg, maps, T)
         return d_x, d_w, d_w_fc, d_w_proj, None, None, None
 
 
-def few(rows: int, held_proj: Fp8Weight) -> bool:
+def few(rows: int, held_proj) -> bool:
     """Whether `few_tokens` is the faster way for this many routed rows."""
     E, H, I = held_proj.shape
-    return rows > 0 and _few(rows, E, max(H, I))
+    return rows > 0 and _native.binding().few(rows, E, max(H, I))
 
 
-def few_tokens(x, weights, held_fc: Fp8Weight, held_proj: Fp8Weight, maps: K.RowMaps) -> torch.Tensor:
+def few_tokens(x, weights, held_fc, held_proj, maps: K.RowMaps) -> torch.Tensor:
     """The layer without gradients for a few rows per expert; `maps` sorted with row_align = 1."""
-    T, H = x.shape
-    I, E, R = held_proj.shape[-1], maps.num_experts, T * maps.top_k
-    xg = K.scatter(x.contiguous(), maps)[:R]
-    act = swiglu_packed(_few_rows(xg, held_fc, E, 2 * I, H, maps.expert_count))
-    out = _few_rows(act, held_proj, E, H, I, maps.expert_count)
+    T = x.size(0)
+    xg = K.scatter(x.contiguous(), maps)[: T * maps.top_k]
+    act = swiglu_packed(_few_rows(xg, held_fc, maps.expert_count))
+    out = _few_rows(act, held_proj, maps.expert_count)
     return K.combine(out, weights.contiguous(), maps, T)

@@ -359,7 +359,7 @@ int fma_b200_moe_gemm_wgrad(const void* dY, const void* X, void* dW, int32_t dty
                             int32_t OUT, int32_t IN, const int32_t* seg_offsets, int32_t n_seg, void* stream);
 /*
  * fma_b200_moe_gemm_wgrad (16-bit types, one segment per expert) for any number of rows: dY and X end at `rows`, and
- * seg_offsets [E+1] at the rows that count; a plain linear map is E = 1 with {0, rows}.  With several experts each
+ * seg_offsets [E+1] at the rows that count; a plain linear map is E = 1 with NULL, NULL.  With several experts each
  * segment starts on a multiple of 64 rows; seg_rows [E] (may be NULL: all of a segment's rows) is the number of rows to
  * reduce over in it, of which the last 64-row block is read whole: its rows behind them are zero.
  */

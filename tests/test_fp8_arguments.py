@@ -67,7 +67,8 @@ def test_entry_points_refuse_bad_arguments():
     v = lib.fma_b200_linear_wgrad
     assert v(at, at, at, 0, 4, 1, 16, 16, at, null, null) == UNSUPPORTED
     assert v(at, at, at, 1, 0, 1, 16, 16, at, null, null) == BAD
-    assert v(at, at, at, 1, 4, 1, 16, 16, null, null, null) == BAD
+    assert v(at, at, at, 1, 4, 2, 16, 16, null, null, null) == BAD  # several experts without offsets
+    assert v(at, null, at, 1, 4, 1, 16, 16, null, null, null) == BAD
     fw, bw = lib.fma_b200_swiglu_fp8_forward, lib.fma_b200_swiglu_fp8_backward
     assert fw(at, 16, at, 16, at, 16, 1, 4, 12, null, at, at, at, at, null, null, null) == BAD
     assert fw(at, 16, at, 16, at, 16, 1, 4, 16, null, at, null, at, at, null, null, null) == BAD  # values without scales
