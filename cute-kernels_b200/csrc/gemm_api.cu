@@ -23,7 +23,7 @@ int tc2_forward_swiglu(const void* X, const void* W, void* pre, void* act, int64
 int tc2_dgrad(const void* dY, const void* W, void* dX, const void* pre, int64_t rows_cap, int E, int OUT, int IN,
               const int32_t* mtile_expert, bool swiglu, bool f16, cudaStream_t s);
 int tc2_wgrad(const void* dY, const void* X, void* dW, int64_t rows_cap, int E, int OUT, int IN,
-              const int32_t* seg_offsets, int n_seg, const int32_t* seg_rows, bool f16, cudaStream_t s);
+              const int32_t* seg_offsets, int n_seg, bool f16, cudaStream_t s);
 int tc2_forward_peer(const void* X, const void* W, const uint64_t* dst_table, int64_t rows_cap, int E, int OUT, int IN,
                      const int32_t* mtile_expert, bool f16, cudaStream_t s);
 int tc2_dgrad_peer(const void* dY, const void* W, const uint64_t* dst_table, int64_t rows_cap, int E, int OUT, int IN,
@@ -106,21 +106,9 @@ int fma_b200_moe_gemm_wgrad(const void* dY, const void* X, void* dW, int32_t dty
     FMAB_REQUIRE(aligned16(dY) && aligned16(X) && aligned16(dW), FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool f16 = dtype == FMA_B200_F16;
-    if (dtype != FMA_B200_F32 && use_pairs(256)) return tc2_wgrad(dY, X, dW, rows_cap, E, OUT, IN, seg_offsets, n_seg, nullptr, f16, s);
+    if (dtype != FMA_B200_F32 && use_pairs(256)) return tc2_wgrad(dY, X, dW, rows_cap, E, OUT, IN, seg_offsets, n_seg, f16, s);
     if (dtype != FMA_B200_F32) return tc_wgrad(dY, X, dW, rows_cap, E, OUT, IN, seg_offsets, n_seg, f16, s);
     return simt_wgrad(dY, X, dW, rows_cap, E, OUT, IN, seg_offsets, n_seg, s);
-}
-
-int fma_b200_linear_wgrad(const void* dY, const void* X, void* dW, int32_t dtype, int64_t rows, int32_t E, int32_t OUT,
-                          int32_t IN, const int32_t* seg_offsets, const int32_t* seg_rows, void* stream) {
-    using namespace fmab;
-    FMAB_REQUIRE(dtype == FMA_B200_BF16 || dtype == FMA_B200_F16, FMA_B200_ERR_UNSUPPORTED, "dtype %d", dtype);
-    FMAB_REQUIRE(rows >= 1, FMA_B200_ERR_BAD_ARG, "rows=%lld", (long long)rows);
-    if (int rc = check_layer_gemm(dtype, (rows + 127) / 128 * 128, E, OUT, IN)) return rc;
-    FMAB_REQUIRE(dW && dY && X && (seg_offsets || (E == 1 && !seg_rows)), FMA_B200_ERR_BAD_ARG, "NULL pointer");
-    FMAB_REQUIRE(aligned16(dY) && aligned16(X) && aligned16(dW), FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
-    return tc2_wgrad(dY, X, dW, rows, E, OUT, IN, seg_offsets, 1, seg_rows, dtype == FMA_B200_F16,
-                     static_cast<cudaStream_t>(stream));
 }
 
 int fma_b200_moe_gemm_forward_swiglu(const void* X, const void* W, void* pre, void* act, int32_t dtype,

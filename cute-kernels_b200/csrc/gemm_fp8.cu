@@ -89,15 +89,6 @@ __device__ __forceinline__ void tc_mma_f8_pair(uint32_t d, uint64_t a, uint64_t 
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
         : "memory");
 }
-// One commit that arrives on the barrier at this offset in both CTAs.
-__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
-        ::"r"(bar), "h"(static_cast<uint16_t>(3))
-        : "memory");
-}
 // M = 256, e4m3 operands, ue8m0 scales; scale_byte = which byte of the scale words.
 __device__ __forceinline__ uint32_t f8_instr_desc(int n, uint32_t scale_byte) {
     return (scale_byte << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(256 >> 4) << 24) |

@@ -89,6 +89,15 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(peer_bar) : "memory");
 }
 
+// The same with one commit, issued by an elected lane of a converged warp.
+__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+        ::"r"(bar), "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
 // Bytes [outer, inner] with row pitch `pitch`, boxes of box_outer rows x 128 bytes, 128-byte swizzle.
 inline int encode_bytes(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_outer) {
     EncodeTiledFn fn = encode_fn();

@@ -133,16 +133,11 @@ __device__ __forceinline__ void decode_pair_segment(const GemmParams& p, const P
         a_k0 = 0;
         b_k0 = t.b_k_base;
         len = p.k_len;
-    } else if (p.seg_offsets == nullptr) {  // one expert, all rows
-        a_k0 = 0;
-        b_k0 = 0;
-        len = p.k_len;
     } else {
         const int32_t* o = p.seg_offsets + s * p.n_groups + t.group;
         a_k0 = o[0];
         b_k0 = o[0];
         len = o[1] - o[0];
-        if (p.seg_rows != nullptr) len = min(len, __ldg(p.seg_rows + t.group));
     }
 }
 
@@ -939,7 +934,7 @@ int tc2_dgrad_peer(const void* dY, const void* W, const uint64_t* dst_table, int
 }
 
 int tc2_wgrad(const void* dY, const void* X, void* dW, int64_t rows_cap, int E, int OUT, int IN,
-              const int32_t* seg_offsets, int n_seg, const int32_t* seg_rows, bool f16, cudaStream_t s) {
+              const int32_t* seg_offsets, int n_seg, bool f16, cudaStream_t s) {
     GemmParams p;
     if (int rc = fill_pair_common(p)) return rc;
     p.f16 = f16 ? 1 : 0;
@@ -947,8 +942,6 @@ int tc2_wgrad(const void* dY, const void* X, void* dW, int64_t rows_cap, int E, 
     if (int rc = encode_2d(&p.map_b, X, IN, rows_cap, IN, 64, BK, f16)) return rc;
     p.mode = MODE_WGRAD;
     p.seg_offsets = seg_offsets;
-    p.seg_rows = seg_rows;
-    p.k_len = static_cast<int32_t>(rows_cap);
     p.n_seg = n_seg;
     p.d = static_cast<__nv_bfloat16*>(dW);
     p.ldd = IN;

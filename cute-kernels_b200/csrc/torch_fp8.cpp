@@ -453,7 +453,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         .def_property_readonly("dtype", [](const Blocks& b) { return dtype_object(b.dtype); })
         .def_property_readonly("device", [](const Blocks& b) { return py::cast(b.held.buffer).attr("device"); })
         .def("dequantize", &Blocks::dequantized, py::arg("dtype") = py::none(),
-             "The values it stands for, rounded to `dtype` (default: the type it was made from).");
+             "The values it stands for, rounded to `dtype` (default: the type it was made from).")
+        .def(py::pickle(
+            [](const Blocks& b) { return py::make_tuple(b.held.buffer, b.held.rows, b.held.cols, b.shape, static_cast<int>(b.dtype)); },
+            [](const py::tuple& t) {
+                return std::make_shared<Blocks>(Blocks{Held(t[0].cast<Tensor>(), t[1].cast<int64_t>(), t[2].cast<int64_t>()),
+                                                       t[3].cast<std::vector<int64_t>>(), static_cast<at::ScalarType>(t[4].cast<int>())});
+            }));
     py::class_<Weight, WeightPtr>(m, "Fp8Weight",
                                   "A weight [N, K] or [E, N, K] held in 8 bits with a scale per 128 x 128 block: e4m3 `values` (row pitch: K "
                                   "rounded up to 16) and `scales` in the order in which the tensor cores read them.  `transposed` is the second "
@@ -473,7 +479,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         .def_property_readonly("dtype", [](const Weight& w) { return dtype_object(w.dtype); })
         .def_property_readonly("device", [](const Weight& w) { return py::cast(w.buffer).attr("device"); })
         .def("dequantize", &Weight::dequantized, py::arg("dtype") = py::none(),
-             "The values it stands for, rounded to `dtype` (default: the type it was made from).");
+             "The values it stands for, rounded to `dtype` (default: the type it was made from).")
+        .def(py::pickle(
+            [](const Weight& w) { return py::make_tuple(w.buffer, w.shape, static_cast<int>(w.dtype), w.E, w.N, w.K, w.turned); },
+            [](const py::tuple& t) {
+                return std::make_shared<Weight>(Weight{t[0].cast<Tensor>(), t[1].cast<std::vector<int64_t>>(),
+                                                       static_cast<at::ScalarType>(t[2].cast<int>()), t[3].cast<int64_t>(), t[4].cast<int64_t>(),
+                                                       t[5].cast<int64_t>(), t[6].cast<bool>()});
+            }));
+    for (const char* name : {"Fp8Blocks", "Fp8Weight"}) m.attr(name).attr("__module__") = "fma_b200";  // where pickle finds them
     m.def("few", &few, "Whether this many rows take the one-launch product (rows, experts, width).");
     m.def("quantize_fp8", &quantize_fp8);
     m.def("quantize_fp8_weight", &quantize_fp8_weight);

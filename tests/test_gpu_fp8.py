@@ -90,6 +90,30 @@ def test_weight(dtype, shape):
     assert bool((held.values.float()[..., K:] == 0).all()) and bool((held.transposed.float()[..., N:] == 0).all())
 
 
+def test_what_is_held_can_be_copied_and_saved(tmp_path):
+    import copy
+
+    import fma_b200 as fma
+
+    x, w = randn((9, 264), torch.bfloat16, 24).to(DEV), randn((2, 136, 264), torch.bfloat16, 25).to(DEV)
+    for held in (fma.quantize_fp8(x), fma.quantize_fp8_weight(w, transpose=True)):
+        torch.save(held, tmp_path / "held.pt")
+        for other in (copy.deepcopy(held), torch.load(tmp_path / "held.pt", weights_only=False)):
+            assert type(other) is type(held) and other.shape == held.shape and other.dtype == held.dtype
+            assert other.device == held.device and torch.equal(other.dequantize(), held.dequantize())
+    assert isinstance(held, fma.Fp8Weight) and isinstance(fma.quantize_fp8(x), fma.Fp8Blocks)
+    assert held.scales.data_ptr() != other.scales.data_ptr() and torch.equal(held.transposed_scales, other.transposed_scales)
+
+
+def test_second_derivatives_are_refused():
+    import fma_b200 as fma
+
+    x, w = randn((40, 16), torch.bfloat16, 26).to(DEV).requires_grad_(), randn((8, 16), torch.bfloat16, 27).to(DEV)
+    for y in (fma.linear_fp8(x, w), fma.swiglu_fp8_checkpoint(x, x)):
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 # ---- the linear map --------------------------------------------------------------------------------
 LINEAR = [(1, 8, 8), (1, 128, 16), (5, 1000, 1544), (16, 520, 136), (17, 392, 264), (127, 128, 128), (129, 264, 520), (300, 2056, 1032),
           (1025, 136, 392), (9, 4104, 264), (40, 2056, 392), (64, 1024, 2048), (90, 4104, 136), (120, 8200, 72), (33, 520, 8)]  # fmt: skip
