@@ -211,7 +211,7 @@ __device__ __forceinline__ uint32_t scale_word_of(uint32_t byte) {
     word |= __shfl_xor_sync(0xffffffffu, word, 8);
     return word | __shfl_xor_sync(0xffffffffu, word, 16);
 }
-// Scale byte of the 8 lanes' block and its 16 packed values per lane; returns the warp's scale word (all lanes).
+// The 16 packed values of a lane; returns the scale byte of its 8 lanes' block.
 __device__ __forceinline__ uint32_t quantize_lane_block(const float* x, uint32_t* w) {
     uint32_t m = 0;
 #pragma unroll
@@ -220,7 +220,7 @@ __device__ __forceinline__ uint32_t quantize_lane_block(const float* x, uint32_t
     const float inverse = fp8_inverse(byte);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = fp8_pack4(x + 4 * i, inverse);
-    return scale_word_of(byte);
+    return byte;
 }
 // The same from the lane's values as they were loaded.
 template <typename T>
@@ -236,7 +236,7 @@ __device__ __forceinline__ uint32_t quantize_lane_raw(const uint4* raw, uint32_t
             const float inverse = fp8_inverse(byte);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = fp8_pack4_finite(x + 4 * i, inverse);
-            return scale_word_of(byte);
+            return byte;
         }
     }
     return quantize_lane_block(x, w);

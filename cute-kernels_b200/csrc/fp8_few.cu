@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kFewThreads, 3) few_rows_kernel(const __grid_c
                 const int i = i0 + u * kFewWarps, q = i / rows, r = i - q * rows, kb = 4 * q + g;
                 if (i >= n) break;
                 uint32_t w[4];
-                const uint32_t word = quantize_lane_raw<T>(raw[u], w);
+                const uint32_t word = scale_word_of(quantize_lane_raw<T>(raw[u], w));
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int c = LaneBlock<T>::column(s, j);

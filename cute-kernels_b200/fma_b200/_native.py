@@ -99,7 +99,7 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "fma_b200_swiglu_fp8_backward": (
         ctypes.c_int,
-        [_P, _P, _P, _P, _P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _P, _P],
+        [_P, _P, _P, _P, _P, _I64, _P, _I64, _P, _I64, _I32, _I64, _I64, _P, _P, _P, _P],
     ),
 }
 

@@ -103,15 +103,17 @@ class Fp8SwigluExperts(torch.autograd.Function):
         out = _product(act8, *proj[:2], H, x.dtype, maps)
         y = K.combine(out, weights, maps, T)
         if keep:
-            ctx.save_for_backward(x8.buffer, up8.buffer, gate8.buffer, act8.buffer, out, weights)
-            ctx.held = held_fc, held_proj  # their transposed copies
+            # of the weights the transposed copies alone
+            ctx.save_for_backward(x8.buffer, up8.buffer, gate8.buffer, act8.buffer, out, weights, held_fc.transposed_buffer,
+                                  held_proj.transposed_buffer)  # fmt: skip
+            ctx.turned = fc[3] - fc[2], proj[3] - proj[2]  # where their scales begin
         ctx.maps, ctx.sizes, ctx.dtype = maps, (T, H, I), x.dtype
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x8, up8, gate8, act8, out, weights = ctx.saved_tensors
-        fc, proj = (h.addresses for h in ctx.held)
+        x8, up8, gate8, act8, out, weights, fc_t, proj_t = ctx.saved_tensors
+        fc_t, proj_t = ((b.data_ptr(), b.data_ptr() + at) for b, at in zip((fc_t, proj_t), ctx.turned))
         maps, (T, H, I), dtype, dev = ctx.maps, ctx.sizes, ctx.dtype, dy.device
         cap, used = maps.rows_cap, _used(maps)
         x8 = _Held(cap, H, dev, x8)
@@ -123,15 +125,18 @@ class Fp8SwigluExperts(torch.autograd.Function):
             if need_proj:
                 d_w_proj = _weight_gradient(d_out, act8, maps)
             if need_x or need_fc:
-                d_act = _product(_quantize_rows(d_out, used), *proj[2:], I, dtype, maps)
+                d_act = _product(_quantize_rows(d_out, used), *proj_t, I, dtype, maps)
                 d_pre = torch.empty(cap, 2 * I, dtype=dtype, device=dev)
+                # the same pass quantises d_pre where its blocks of 128 columns do not straddle up and gate
+                d_pre8 = _Held(cap, 2 * I, dev) if need_x and I % 128 == 0 else None
+                at = (d_pre8.values, d_pre8.scales) if d_pre8 else (None, None)
                 call("fma_b200_swiglu_fp8_backward", gate8.values, gate8.scales, up8.values, up8.scales, ptr(d_act), I,
-                     d_pre.data_ptr() + I * d_pre.element_size(), 2 * I, ptr(d_pre), 2 * I, dtype_code(dtype), cap, I, used,
+                     d_pre.data_ptr() + I * d_pre.element_size(), 2 * I, ptr(d_pre), 2 * I, dtype_code(dtype), cap, I, used, *at,
                      stream_ptr(dev))  # fmt: skip
                 if need_fc:
                     d_w_fc = _weight_gradient(d_pre, x8, maps)
                 if need_x:
-                    d_xg = _product(_quantize_rows(d_pre, used), *fc[2:], H, dtype, maps)
+                    d_xg = _product(d_pre8 or _quantize_rows(d_pre, used), *fc_t, H, dtype, maps)
                     d_x = K.scatter_backward(d_xg, maps, T)
         return d_x, d_w, d_w_fc, d_w_proj, None, None, None
 

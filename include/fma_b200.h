@@ -477,7 +477,8 @@ int fma_b200_fp8_few_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t
 /*
  * SwiGLU that keeps its inputs in 8 bits.  forward: out as fma_b200_swiglu_forward (may be NULL), and with gate8 / up8
  * / out8 (each may be NULL) the 8-bit form of gate, up and the rounded out in 1 x 128 blocks.  backward:
- * fma_b200_swiglu_backward on the values that gate8 and up8 stand for.
+ * fma_b200_swiglu_backward on the values that gate8 and up8 stand for; with grad8 (may be NULL; cols a multiple of 128)
+ * also the 8-bit form of the rows [up_grad | gate_grad] of 2 * cols columns.
  */
 int fma_b200_swiglu_fp8_forward(const void* gate, int64_t gate_pitch, const void* up, int64_t up_pitch, void* out,
                                 int64_t out_pitch, int32_t dtype, int64_t rows, int64_t cols, const int32_t* rows_used,
@@ -486,7 +487,7 @@ int fma_b200_swiglu_fp8_forward(const void* gate, int64_t gate_pitch, const void
 int fma_b200_swiglu_fp8_backward(const void* gate8, const void* gate_scales, const void* up8, const void* up_scales,
                                  const void* dy, int64_t dy_pitch, void* gate_grad, int64_t gate_grad_pitch,
                                  void* up_grad, int64_t up_grad_pitch, int32_t dtype, int64_t rows, int64_t cols,
-                                 const int32_t* rows_used, void* stream);
+                                 const int32_t* rows_used, void* grad8, void* grad_scales, void* stream);
 
 /* ======================================================================= */
 /* peer-memory transport of the expert-parallel layer                        */

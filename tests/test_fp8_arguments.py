@@ -73,8 +73,10 @@ def test_entry_points_refuse_bad_arguments():
     assert fw(at, 16, at, 16, at, 16, 1, 4, 12, null, at, at, at, at, null, null, null) == BAD
     assert fw(at, 16, at, 16, at, 16, 1, 4, 16, null, at, null, at, at, null, null, null) == BAD  # values without scales
     assert fw(at, 16, null, 16, at, 16, 1, 4, 16, null, at, at, at, at, null, null, null) == BAD
-    assert bw(at, at, at, null, at, 16, at, 16, at, 16, 1, 4, 16, null, null) == BAD
-    assert bw(at, at, at, at, at, 12, at, 16, at, 16, 1, 4, 16, null, null) == BAD
+    assert bw(at, at, at, null, at, 16, at, 16, at, 16, 1, 4, 16, null, null, null, null) == BAD
+    assert bw(at, at, at, at, at, 12, at, 16, at, 16, 1, 4, 16, null, null, null, null) == BAD
+    assert bw(at, at, at, at, at, 16, at, 16, at, 16, 1, 4, 16, null, at, at, null) == BAD  # grad8: width
+    assert bw(at, at, at, at, at, 128, at, 128, at, 128, 1, 4, 128, null, at, null, null) == BAD
 
 
 def test_operators_need_cuda_tensors():
