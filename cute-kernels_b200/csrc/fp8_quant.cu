@@ -518,9 +518,9 @@ __global__ void __launch_bounds__(kMapThreads) group_maps_kernel(const GroupMaps
     if (t == 0) pad[n + 1] = pad[n] + (rest + 255) / 256 * 256;
     __syncthreads();
     if (t < n) p.group_rows[t] = off[t + 1] - off[t];
-    if (t <= n) {
-        p.offsets[t] = off[t];
-        p.pad_offsets[t] = pad[t];
+    for (int i = t; i <= n; i += kMapThreads) {  // n + 1 entries: one more than threads with 1024 experts
+        p.offsets[i] = off[i];
+        p.pad_offsets[i] = pad[i];
     }
     if (t == 0) p.pad_offsets[n + 1] = pad[n + 1];
     for (int i = t; i < p.n_tiles; i += kMapThreads) {

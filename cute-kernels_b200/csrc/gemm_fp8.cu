@@ -72,7 +72,7 @@ struct GemmFp8Params {
     int64_t out_rows;
     int64_t layout_rows;
     int32_t n_cols, k_blocks, n_ntiles;
-    int32_t tile_n;              // columns per tile: a multiple of 16, at most 256
+    int32_t tile_n;              // columns per tile: a multiple of 32, at most 256
     int32_t a_tiles;             // scale tiles per quad of a
     int32_t b_tiles, b_tiles_expert;  // scale tiles per quad of w, and of one expert
     int32_t f16;
@@ -393,7 +393,7 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
 // where the number of row tiles is known (no experts) the width that makes waves * (width + 24) smallest is taken, 24
 // columns standing for what a tile costs besides its columns: a prompt of up to 256 rows spreads over all SMs (256 x
 // 4096 x 4096: 13.7 us, with 256 columns 15.7; 2048 x 2048 x 1536: 10.7 and 11.6; no difference from two waves on).
-// With experts only the waste at the right edge is known: the tiles share it (520 columns: three tiles of 176, not
+// With experts only the waste at the right edge is known: the tiles share it (520 columns: three tiles of 192, not
 // 256 + 256 + 8).
 static int tile_columns(int64_t layout_rows, int N, bool experts) {
     const int64_t pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, m = (layout_rows + 255) / 256;
@@ -401,7 +401,7 @@ static int tile_columns(int64_t layout_rows, int N, bool experts) {
     int best = 0;
     int64_t best_cost = 0;
     for (int n = fewest; n <= N / 64 + 1; ++n) {
-        const int width = ((N + n - 1) / n + 15) / 16 * 16;
+        const int width = ((N + n - 1) / n + 31) / 32 * 32;  // paired MMAs take whole 32 columns
         const int64_t tiles = (N + width - 1) / width;
         const int64_t cost = (m * tiles + pairs - 1) / pairs * (width + 24);
         if (best == 0 || cost < best_cost) {
@@ -434,7 +434,7 @@ static int launch_fp8(GemmFp8Params& p, cudaStream_t s) {
     }
     const int64_t total = (p.layout_rows + 255) / 256 * p.n_ntiles;
     FMAB_REQUIRE(total < (1LL << 31), FMA_B200_ERR_BAD_ARG, "too many tiles");
-    const int64_t max_pairs = sm_count() / 2;
+    const int64_t max_pairs = sm_count() >= 2 ? sm_count() / 2 : 1;
     const int pairs = static_cast<int>(total < max_pairs ? total : max_pairs);
     return launch_chained("8-bit grouped GEMM", gemm_fp8_kernel, dim3(2 * pairs), F8_THREADS, F8_SMEM, 0, s, p);
 }

@@ -291,7 +291,7 @@ int fma_b200_linear_wgrad(const void* dY, const void* X, void* dW, int32_t dtype
         FMAB_CUDA(cudaFuncSetAttribute(linear_wgrad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WG_SMEM));
         configured[dev] = true;
     }
-    const int64_t max_pairs = sm_count() / 2;
+    const int64_t max_pairs = sm_count() >= 2 ? sm_count() / 2 : 1;
     const int pairs = static_cast<int>(total < max_pairs ? total : max_pairs);
     return launch_chained("linear weight gradient", linear_wgrad_kernel, dim3(2 * pairs), WG_THREADS, WG_SMEM, 0,
                           static_cast<cudaStream_t>(stream), p);

@@ -116,7 +116,8 @@ def test_second_derivatives_are_refused():
 
 # ---- the linear map --------------------------------------------------------------------------------
 LINEAR = [(1, 8, 8), (1, 128, 16), (5, 1000, 1544), (16, 520, 136), (17, 392, 264), (127, 128, 128), (129, 264, 520), (300, 2056, 1032),
-          (1025, 136, 392), (9, 4104, 264), (40, 2056, 392), (64, 1024, 2048), (90, 4104, 136), (120, 8200, 72), (33, 520, 8)]  # fmt: skip
+          (1025, 136, 392), (9, 4104, 264), (40, 2056, 392), (64, 1024, 2048), (90, 4104, 136), (120, 8200, 72), (33, 520, 8), (200, 136, 8),
+          (130, 8, 40), (260, 40, 72)]  # fmt: skip
 
 
 @pytest.mark.parametrize("dtype", HALF)
@@ -296,6 +297,26 @@ def test_swiglu(dtype, shape, halves):
         off = (got.double() - ref).abs()
         assert bool((off <= half * ref.abs() + (1 + half) * fp32 * grow * size + tiny).all())
     check_device_status()
+
+
+def test_many_experts():
+    import fma_b200 as fma
+
+    E = 1024
+    counts = [0] * E
+    counts[0], counts[511], counts[512], counts[1022], counts[1023] = 3, 1, 20, 2, 130
+    rows = sum(counts) + 2
+    x, w = randn((rows, 16), torch.bfloat16, 28).to(DEV), randn((E, 8, 16), torch.bfloat16, 29).to(DEV)
+    d_out = randn((rows, 8), torch.bfloat16, 30).to(DEV)
+    (y, dx, dw), (sy, sx, sw) = R.grouped(x, w, counts, d_out)
+    count = torch.tensor(counts, device=DEV)
+    R.check_product(fma.grouped_linear_fp8(x, fma.quantize_fp8_weight(w), count), y, sy, 16)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = fma.grouped_linear_fp8(a, b, count)
+    out.backward(d_out)
+    R.check_product(out.detach(), y, sy, 16)
+    R.check_product(a.grad, dx, sx, 8)
+    R.check_product(b.grad, dw, sw, 130)
 
 
 def test_swiglu_keeps_half_the_memory():
