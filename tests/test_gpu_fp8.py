@@ -182,6 +182,30 @@ def test_linear_gradient_is_that_of_differences():
     assert float(moved.detach()) == float(a.grad[3, 5]) * float(step[3, 5])
 
 
+@pytest.mark.parametrize("rows", [9, 60, 150])
+def test_linear_far_scales(rows):
+    """Every row and every weight block with a scale of its own, far apart, rows and blocks of zeros among them."""
+    import fma_b200 as fma
+
+    K, N = 1544, 264
+    x, w = randn((rows, K), torch.bfloat16, 31).to(DEV), randn((N, K), torch.bfloat16, 32).to(DEV)
+    block = torch.arange(K, device=DEV) // 128
+    power = (torch.arange(rows, device=DEV)[:, None] * 7 + block * 5) % 81 - 40
+    x = (x.double() * torch.exp2(power.double())).to(torch.bfloat16)
+    power = ((torch.arange(N, device=DEV)[:, None] // 128) * 11 + block * 3) % 61 - 30
+    w = (w.double() * torch.exp2(power.double())).to(torch.bfloat16)
+    x[2], x[4, :256], w[:128, 384:512] = 0, 0, 0
+    d_out = randn((rows, N), torch.bfloat16, 33).to(DEV)
+    (y, dx, dw), (sy, sx, sw) = R.linear(x, w, d_out)
+    R.check_product(fma.linear_fp8(x, fma.quantize_fp8_weight(w)), y, sy, K)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = fma.linear_fp8(a, b)
+    out.backward(d_out)
+    R.check_product(out.detach(), y, sy, K)
+    R.check_product(a.grad, dx, sx, N)
+    R.check_product(b.grad, dw, sw, rows)
+
+
 @pytest.mark.parametrize("rows", [3, 200])
 def test_linear_keeps_a_bad_row_to_itself(rows):
     import fma_b200 as fma
