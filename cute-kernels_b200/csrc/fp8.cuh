@@ -1,5 +1,5 @@
 // The 8-bit format of this library, shared by the kernels that write it (fp8_quant.cu) and the products that read it
-// (gemm_fp8.cu).
+// (gemm_fp8.cu, fp8_few.cu).
 //
 // A tensor [rows, cols] is held as e4m3 values [rows, pitch] (pitch = cols rounded up to 16, the extra columns zero)
 // and one power-of-two scale per block of 128 columns of a row, or of 128 x 128 (weights).  With amax the largest
@@ -124,17 +124,7 @@ __device__ __forceinline__ uint32_t max_over_8_lanes(uint32_t v) {
     return v;
 }
 
-// Reads the lane's 16 values of columns [col0, cols); columns beyond are zero.
-template <typename T>
-__device__ __forceinline__ void load_lane_block(const T* row, int col0, int cols, int s, float* x) {
-    using B = LaneBlock<T>;
-#pragma unroll
-    for (int j = 0; j < B::N; ++j) {
-        const int c = col0 + B::column(s, j);
-        const uint4 v = c < cols ? ld_stream_16(row + c) : make_uint4(0, 0, 0, 0);
-        Elem<T>::unpack(v, x + j * B::V);
-    }
-}
+// The lane's 16 values to columns [col0, cols).
 template <typename T>
 __device__ __forceinline__ void store_lane_block(T* row, int col0, int cols, int s, const float* x) {
     using B = LaneBlock<T>;

@@ -24,9 +24,16 @@
 //   ring stages of 256 columns: eight MMAs per wait and commit instead of four             324 us  2.97
 // The library's 8-bit product without block scales takes 322 us on the same GPU.
 //
-// The pair tile is 256 rows x up to 256 columns.  Two 256-column accumulators and the scales do not fit into the 512
-// columns of tensor memory, so the accumulators overlap by 32 columns: the epilogue reads the overlap first and hands
-// it back at once, and the next tile's main loop starts while the rest is still being read and stored.
+// The pair tile is 256 weight rows (the instruction's rows) x up to 256 rows of a (its columns, in steps of 32): an
+// expert's last tile is as high as it has rows left.  With the operands the other way round every expert's rows were
+// padded to 256; 128 experts of 1536 x 2048 with 52 / 128 / 512 rows each on average took 104 / 108 / 201 us so and take
+// 94 / 100 / 193 now, 8 of 14336 x 4096 with 1024 rows 381 and 367; plain products are the same both ways.  A low tile
+// saves less than its MMAs: it loads 128 weight rows per CTA all the same, and a full one already loads near L2's rate.
+// The result lies in tensor memory a weight row per lane and is turned in shared memory on its way out.
+//
+// Two 256-column accumulators and the scales do not fit into the 512 columns of tensor memory, so the accumulators
+// overlap by 32 columns: the epilogue reads the overlap first and hands it back at once, and the next tile's main loop
+// starts while the rest is still being read and stored.
 #include "fp8.cuh"
 #include "gemm_pair.cuh"
 
@@ -43,38 +50,39 @@ constexpr int UMMA_K8 = 32;
 constexpr int F8_EPI_WARPS = 8;
 constexpr int F8_SCALE_WARPS = 4;
 constexpr int F8_THREADS = 32 * (2 + F8_EPI_WARPS + F8_SCALE_WARPS);
-constexpr int F8_TILE_N = 256;                    // widest tile
-constexpr int F8_A_BYTES = 128 * BK8;             // this CTA's 128 rows
-constexpr int F8_B_BYTES = F8_TILE_N / 2 * BK8;   // its half of the tile's columns
+constexpr int F8_TILE_ROWS = 256;                 // most rows of a per tile
+constexpr int F8_W_BYTES = 128 * BK8;             // this CTA's 128 weight rows
+constexpr int F8_X_BYTES = F8_TILE_ROWS / 2 * BK8;  // its half of the tile's rows of a
 constexpr int F8_STAGE_KB = 2;                    // k-blocks per ring stage
-constexpr int F8_STAGE_BYTES = F8_STAGE_KB * (F8_A_BYTES + F8_B_BYTES);
+constexpr int F8_STAGE_BYTES = F8_STAGE_KB * (F8_W_BYTES + F8_X_BYTES);
 constexpr int F8_STAGES = 3;
-constexpr int F8_PATCH_BYTES = 32 * 64;  // 32 rows x 32 columns of 16 bits per epilogue warp
+constexpr int F8_PATCH_BYTES = 32 * 64;  // 32 rows of a x 32 weight rows, 16 bits, per epilogue warp
 constexpr size_t F8_SMEM = static_cast<size_t>(F8_STAGES) * F8_STAGE_BYTES + F8_EPI_WARPS * F8_PATCH_BYTES + 1024;
-constexpr int F8_SUPER = 8;                       // pair m-tiles walked together (operand reuse in L2)
-// tensor memory: accumulator 0 in columns 0-255, accumulator 1 in 224-479, two scale buffers of 12 columns (A: 4,
-// B: 8) from 480 on
+constexpr int F8_SUPER = 8;                       // tiles of rows of a walked together (operand reuse in L2)
+constexpr int F8_BOXES = 4;                       // rows of a come in boxes of 16, 32, 64 or 128
+// tensor memory: accumulator 0 in columns 0-255, accumulator 1 in 224-479, two scale buffers of 12 columns (weights 4,
+// rows of a 8) from 480 on
 constexpr int F8_ACC1_COL = 224;
 constexpr int F8_SCALE_COL = 480;
 constexpr int F8_SCALE_COLS = 16;
 constexpr int F8_SCALE_BUFFERS = 2;
 
 struct GemmFp8Params {
-    CUtensorMap map_a, map_b;
+    CUtensorMap map_w, map_a[F8_BOXES];
     const uint8_t* a_scales;
-    const uint8_t* b_scales;
+    const uint8_t* w_scales;
     void* out;
-    const int32_t* tile_expert;  // per 128-row tile: expert, -1 = unused, -2 = rows of no expert (zeros); null: one expert
-    const int32_t* tile_row;     // per 128-row tile: first output row; null: tile * 128
-    const int32_t* tile_rows;    // per 128-row tile: output rows; null: up to out_rows
+    const int32_t* tile_expert;  // per 128 rows of a: expert, -1 = unused, -2 = rows of no expert (zeros); null: one expert
+    const int32_t* tile_row;     // per 128 rows of a: first output row; null: the same row
+    const int32_t* tile_rows;    // per 128 rows of a: output rows; null: up to out_rows
     const int32_t* rows_used;    // rows of the layout in use (device); null: layout_rows
     int32_t* status;
     int64_t out_rows;
     int64_t layout_rows;
-    int32_t n_cols, k_blocks, n_ntiles;
-    int32_t tile_n;              // columns per tile: a multiple of 32, at most 256
+    int32_t n_cols, k_blocks, w_ntiles;
+    int32_t tile_rows_most;      // rows of a per tile: a multiple of 32, at most 256; 256 where any tile_* is given
     int32_t a_tiles;             // scale tiles per quad of a
-    int32_t b_tiles, b_tiles_expert;  // scale tiles per quad of w, and of one expert
+    int32_t w_tiles, w_tiles_expert;  // scale tiles per quad of w, and of one expert
     int32_t f16;
 };
 
@@ -94,6 +102,9 @@ __device__ __forceinline__ uint32_t f8_instr_desc(int n, uint32_t scale_byte) {
     return (scale_byte << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(256 >> 4) << 24) |
            (scale_byte << 29);
 }
+__device__ __forceinline__ void st_shared_2(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
+}
 __device__ __forceinline__ void tc_store_4(uint32_t taddr, uint4 v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
                  ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
@@ -102,29 +113,40 @@ __device__ __forceinline__ void tc_store_4(uint32_t taddr, uint4 v) {
 
 struct F8PairTile {
     int32_t expert;
-    int32_t a_row;       // this CTA's first row of A
-    int32_t n0;
-    int32_t rows;        // output rows of this CTA
-    int64_t out_row;
+    int32_t w0;      // first weight row = output column of the pair
+    int32_t a_row;   // first row of a
+    int32_t n;       // rows of a in the MMAs: a multiple of 32
+    int32_t rows;    // output rows of this half of the tile (128 rows of a)
+    int64_t out_row; // and the first of them
 };
 
-__device__ __forceinline__ bool f8_decode(const GemmFp8Params& p, int tile, int n_pairs_m, uint32_t rank, F8PairTile& t) {
-    const int per_super = F8_SUPER * p.n_ntiles;
+__device__ __forceinline__ void f8_rows(const GemmFp8Params& p, int32_t a_row, int half, int64_t& out_row, int32_t& rows) {
+    const int mt = a_row / 128 + half;  // used where tiles start at multiples of 256
+    out_row = p.tile_row != nullptr ? __ldg(p.tile_row + mt) : a_row + 128LL * half;
+    const int64_t most = min(128, p.tile_rows_most - 128 * half);
+    const int64_t left = p.tile_rows != nullptr ? __ldg(p.tile_rows + mt) : p.out_rows - out_row;
+    rows = static_cast<int32_t>(left < 0 || most < 0 ? 0 : (left > most ? most : left));
+}
+
+// false: nothing to do for this tile
+__device__ __forceinline__ bool f8_decode(const GemmFp8Params& p, int tile, int a_ntiles, int half, F8PairTile& t) {
+    const int per_super = F8_SUPER * p.w_ntiles;
     const int super = tile / per_super;
-    const int m_first = super * F8_SUPER;
-    const int m_span = min(F8_SUPER, n_pairs_m - m_first);
+    const int first = super * F8_SUPER;
+    const int span = min(F8_SUPER, a_ntiles - first);
     const int r = tile - super * per_super;
-    const int nt = r / m_span;
-    const int pm = m_first + (r - nt * m_span);
-    const int mt = 2 * pm + static_cast<int>(rank);
-    t.expert = p.tile_expert != nullptr ? __ldg(p.tile_expert + 2 * pm) : 0;
+    const int wt = r / span;
+    t.w0 = wt * 256;
+    t.a_row = (first + (r - wt * span)) * p.tile_rows_most;
+    t.expert = p.tile_expert != nullptr ? __ldg(p.tile_expert + t.a_row / 128) : 0;
     if (t.expert == -1) return false;
-    t.a_row = mt * 128;
-    t.n0 = nt * p.tile_n;
-    t.out_row = p.tile_row != nullptr ? __ldg(p.tile_row + mt) : static_cast<int64_t>(mt) * 128;
-    const int64_t left = p.tile_rows != nullptr ? __ldg(p.tile_rows + mt) : p.out_rows - t.out_row;
-    t.rows = static_cast<int32_t>(left < 0 ? 0 : (left > 128 ? 128 : left));
-    return true;
+    int64_t other_row;
+    int32_t other;
+    f8_rows(p, t.a_row, half, t.out_row, t.rows);
+    f8_rows(p, t.a_row, half ^ 1, other_row, other);
+    const int32_t lower = half == 0 ? t.rows : other, upper = half == 0 ? other : t.rows;
+    t.n = ((upper > 0 ? 128 + upper : lower) + 31) / 32 * 32;
+    return t.n > 0;
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8_THREADS, 1)
@@ -174,8 +196,8 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
     volatile int* abort_ptr = &abort_flag;
 
     const int64_t rows_used = p.rows_used != nullptr ? min(p.layout_rows, static_cast<int64_t>(__ldg(p.rows_used))) : p.layout_rows;
-    const int n_pairs_m = static_cast<int>((rows_used + 255) / 256);
-    const int total_tiles = n_pairs_m * p.n_ntiles;
+    const int a_ntiles = static_cast<int>((rows_used + p.tile_rows_most - 1) / p.tile_rows_most);
+    const int total_tiles = a_ntiles * p.w_ntiles;
     const int pair_id = blockIdx.x >> 1;
     const int n_pairs = gridDim.x >> 1;
 
@@ -185,11 +207,13 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
             int stage = 0;
             uint32_t phase = 0;
             bool alive = true;
-            const uint32_t kb_bytes = F8_A_BYTES + p.tile_n / 2 * BK8;
             for (int tile = pair_id; tile < total_tiles && alive; tile += n_pairs) {
                 F8PairTile t;
-                if (!f8_decode(p, tile, n_pairs_m, rank, t) || t.expert < 0) continue;
-                const int b_row = t.expert * p.n_cols + t.n0 + static_cast<int>(rank) * (p.tile_n / 2);
+                if (!f8_decode(p, tile, a_ntiles, 0, t) || t.expert < 0) continue;
+                const int w_row = t.expert * p.n_cols + t.w0 + static_cast<int>(rank) * 128;
+                const int a_row = t.a_row + static_cast<int>(rank) * (t.n / 2);
+                const int box = t.n > 128 ? 3 : (t.n > 64 ? 2 : (t.n > 32 ? 1 : 0));  // the smallest that holds n / 2 rows
+                const uint32_t kb_bytes = F8_W_BYTES + (16 << box) * BK8;
                 for (int kb = 0; kb < p.k_blocks; kb += F8_STAGE_KB) {
                     if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, abort_ptr, p.status)) {
                         alive = false;
@@ -198,11 +222,11 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
                     const int n_kb = min(F8_STAGE_KB, p.k_blocks - kb);
                     const uint32_t leader_bar = map_to_rank(smem_u32(&full_bar[stage]), 0);
                     const uint32_t sa = ring + stage * F8_STAGE_BYTES;
-                    const uint32_t sb = sa + F8_STAGE_KB * F8_A_BYTES;
+                    const uint32_t sb = sa + F8_STAGE_KB * F8_W_BYTES;
                     if (leader) mbar_arrive_expect_tx(smem_u32(&full_bar[stage]), 2 * n_kb * kb_bytes);
                     for (int j = 0; j < n_kb; ++j) {
-                        tma_load_2d_pair(sa + j * F8_A_BYTES, &p.map_a, leader_bar, (kb + j) * BK8, t.a_row);
-                        tma_load_2d_pair(sb + j * F8_B_BYTES, &p.map_b, leader_bar, (kb + j) * BK8, b_row);
+                        tma_load_2d_pair(sa + j * F8_W_BYTES, &p.map_w, leader_bar, (kb + j) * BK8, w_row);
+                        tma_load_2d_pair(sb + j * F8_X_BYTES, &p.map_a[box], leader_bar, (kb + j) * BK8, a_row);
                     }
                     if (++stage == F8_STAGES) {
                         stage = 0;
@@ -225,7 +249,7 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
             bool alive = true;
             for (int tile = pair_id; tile < total_tiles && alive; tile += n_pairs) {
                 F8PairTile t;
-                if (!f8_decode(p, tile, n_pairs_m, rank, t) || t.expert < 0) continue;
+                if (!f8_decode(p, tile, a_ntiles, 0, t) || t.expert < 0) continue;
                 // the epilogues have read the columns that this accumulator shares with the previous one
                 if (n_done > 0 && !mbar_wait(smem_u32(&acc_empty_bar), (n_done - 1) & 1u, abort_ptr, p.status)) break;
                 tc_fence_after();
@@ -242,16 +266,16 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
                     tc_fence_after();
                     const uint32_t scales = tmem_base + F8_SCALE_COL + sbuf * F8_SCALE_COLS;
                     const uint32_t sa = ring + stage * F8_STAGE_BYTES;
-                    const uint64_t a_desc = make_smem_desc<false>(sa);
-                    const uint64_t b_desc = make_smem_desc<false>(sa + F8_STAGE_KB * F8_A_BYTES);
+                    const uint64_t w_desc = make_smem_desc<false>(sa);
+                    const uint64_t a_desc = make_smem_desc<false>(sa + F8_STAGE_KB * F8_W_BYTES);
 #pragma unroll
                     for (int j = 0; j < F8_STAGE_KB; ++j) {
                         if (kb + j >= p.k_blocks) continue;
-                        const uint32_t idesc = f8_instr_desc(p.tile_n, (kb + j) & 3);
+                        const uint32_t idesc = f8_instr_desc(t.n, (kb + j) & 3);
 #pragma unroll
                         for (int ks = 0; ks < BK8 / UMMA_K8; ++ks)
-                            tc_mma_f8_pair(acc, a_desc + (j * F8_A_BYTES + ks * UMMA_K8) / 16,
-                                           b_desc + (j * F8_B_BYTES + ks * UMMA_K8) / 16, idesc, scales, scales + 4,
+                            tc_mma_f8_pair(acc, w_desc + (j * F8_W_BYTES + ks * UMMA_K8) / 16,
+                                           a_desc + (j * F8_X_BYTES + ks * UMMA_K8) / 16, idesc, scales, scales + 4,
                                            (kb | j | ks) != 0);
                     }
                     tc_commit_both(smem_u32(&empty_bar[stage]));
@@ -274,14 +298,14 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
     } else if (warp < 2 + F8_EPI_WARPS) {
         // ------------------------------ epilogue (both CTAs) ------------------------------
         const int quad = warp & 3;               // tensor-memory lanes this warp may read
-        const int half = (warp - 2) >> 2;        // columns 0-127 or 128-255 of the tile
+        const int half = (warp - 2) >> 2;        // rows 0-127 or 128-255 of the tile
         const uint32_t patch = patches + (warp - 2) * F8_PATCH_BYTES;
         const bool f16 = p.f16 != 0;
         uint16_t* const out = static_cast<uint16_t*>(p.out);
         uint32_t n_done = 0;
         for (int tile = pair_id; tile < total_tiles; tile += n_pairs) {
             F8PairTile t;
-            if (!f8_decode(p, tile, n_pairs_m, rank, t)) continue;
+            if (!f8_decode(p, tile, a_ntiles, half, t)) continue;
             const uint32_t acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + (n_done & 1u) * F8_ACC1_COL;
             // the 32 columns of the overlap come first: the last ones of accumulator 0, the first ones of 1
             const bool backwards = half == 1 && (n_done & 1u) == 0;
@@ -289,12 +313,13 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
                 if (!mbar_wait(smem_u32(&acc_full_bar[n_done & 1u]), (n_done >> 1) & 1u, abort_ptr, p.status)) break;
                 tc_fence_after();
             }
+            const int col = t.w0 + static_cast<int>(rank) * 128 + quad * 32 + (lane & 3) * 8;
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {
-                const int c0 = half * 128 + (backwards ? 3 - i : i) * 32;
-                float v[32];
+                const int r0 = (backwards ? 3 - i : i) * 32;  // rows r0 .. r0 + 31 of this half
+                float v[32];                                  // one weight row, 32 rows of a
                 if (t.expert >= 0) {
-                    if (c0 < p.tile_n) tc_load_32(acc + c0, v);  // columns from tile_n on are never stored
+                    if (half * 128 + r0 < t.n) tc_load_32(acc + half * 128 + r0, v);
                     if (i == 0) {
                         tc_fence_before();
                         __syncwarp();
@@ -304,28 +329,36 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = 0.f;
                 }
-                if (c0 >= p.tile_n) continue;
-                // through the patch: 32 rows x 64 bytes, written a row per lane, read four lanes to a row
+                if (r0 >= t.rows) continue;
+                // turned in the patch: 32 rows of a x 64 bytes, written a weight row per lane (two bytes, 32 lanes next to
+                // each other), read four lanes to a row of a
                 __syncwarp();
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    st_shared_16(patch + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), pack8(v + 8 * q, f16));
+                for (int q = 0; q < 4; ++q) {
+                    const uint4 w = pack8(v + 8 * q, f16);
+                    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int row = 8 * q + 2 * k;
+                        const uint32_t at = patch + row * 64 + (((lane >> 3) ^ k) << 4) + (lane & 7) * 2;
+                        st_shared_2(at, words[k]);
+                        st_shared_2(at + 64, words[k] >> 16);
+                    }
+                }
                 __syncwarp();
-                const int cw = c0 + (lane & 3) * 8;
 #pragma unroll
                 for (int it = 0; it < 4; ++it) {
                     const int row = it * 8 + (lane >> 2);
                     const uint4 w = ld_shared_16(patch + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
-                    if (quad * 32 + row < t.rows && cw < p.tile_n && t.n0 + cw < p.n_cols)
-                        st_global_16(out + (t.out_row + quad * 32 + row) * p.n_cols + t.n0 + cw, w);
+                    if (r0 + row < t.rows && col < p.n_cols) st_global_16(out + (t.out_row + r0 + row) * p.n_cols + col, w);
                 }
             }
             if (t.expert >= 0) ++n_done;
         }
     } else {
         // ------------------------------ scales (both CTAs) ------------------------------
-        // All four warps bring the same words, each into its 32 lanes: word j of lane l is row j * 32 + l.  Rows of a
-        // weight block share one word, so a tile may start anywhere in it.
+        // All four warps bring the same words, each into its 32 lanes: word j of lane l is row j * 32 + l.  The 128 weight
+        // rows of a CTA are one block and share one word.
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         // A buffer is free again when the MMAs of two groups ago are complete, which the release of the last ring
         // stage of that group tells: these warps follow the stage numbers and watch that barrier.  It cannot run a
@@ -337,22 +370,22 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
         bool alive = true;
         for (int tile = pair_id; tile < total_tiles && alive; tile += n_pairs) {
             F8PairTile t;
-            if (!f8_decode(p, tile, n_pairs_m, rank, t) || t.expert < 0) continue;
-            const int a_tile = t.a_row / 128;
+            if (!f8_decode(p, tile, a_ntiles, 0, t) || t.expert < 0) continue;
+            const int block = t.w0 / FP8_BLOCK + static_cast<int>(rank);
+            const int piece = t.a_row / 32;  // in 32 rows: a scale tile holds four
             for (int kb = 0; kb < p.k_blocks; kb += 4) {
                 const int q = kb >> 2;
                 const uint32_t one = 0x01010101u * FP8_SCALE_ONE;
-                uint4 wa = make_uint4(one, one, one, one);
-                if (a_tile < p.a_tiles)
-                    wa = __ldg(reinterpret_cast<const uint4*>(p.a_scales + (static_cast<int64_t>(q) * p.a_tiles + a_tile) * FP8_TILE_BYTES) + lane);
-                uint32_t wb[8];
+                uint32_t ww = one, wa[8];
+                if (block < p.w_tiles_expert)
+                    ww = __ldg(reinterpret_cast<const uint32_t*>(
+                        p.w_scales + (static_cast<int64_t>(q) * p.w_tiles + t.expert * p.w_tiles_expert + block) * FP8_TILE_BYTES));
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int block = (t.n0 + j * 32 + lane) / FP8_BLOCK;
-                    wb[j] = one;
-                    if (block < p.b_tiles_expert)
-                        wb[j] = __ldg(reinterpret_cast<const uint32_t*>(
-                            p.b_scales + (static_cast<int64_t>(q) * p.b_tiles + t.expert * p.b_tiles_expert + block) * FP8_TILE_BYTES));
+                    wa[j] = one;
+                    if (j * 32 < t.n && (piece + j) / 4 < p.a_tiles)
+                        wa[j] = __ldg(reinterpret_cast<const uint32_t*>(
+                            p.a_scales + (static_cast<int64_t>(q) * p.a_tiles + (piece + j) / 4) * FP8_TILE_BYTES + lane * 16 + ((piece + j) & 3) * 4));
                 }
                 if (ends[buf] > 0) {
                     const uint32_t last = ends[buf] - 1;
@@ -366,9 +399,9 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
                 tc_fence_after();
                 __syncwarp();
                 const uint32_t at = tmem_base + lanes + F8_SCALE_COL + buf * F8_SCALE_COLS;
-                tc_store_4(at, wa);
-                tc_store_4(at + 4, make_uint4(wb[0], wb[1], wb[2], wb[3]));
-                tc_store_4(at + 8, make_uint4(wb[4], wb[5], wb[6], wb[7]));
+                tc_store_4(at, make_uint4(ww, ww, ww, ww));
+                tc_store_4(at + 4, make_uint4(wa[0], wa[1], wa[2], wa[3]));
+                tc_store_4(at + 8, make_uint4(wa[4], wa[5], wa[6], wa[7]));
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
@@ -389,37 +422,37 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
 }
 
 // ---- host side -------------------------------------------------------------------------------------
-// Columns per tile.  Few wide tiles read A least often; but the launch takes as long as its fullest pair of SMs, so
-// where the number of row tiles is known (no experts) the width that makes waves * (width + 24) smallest is taken, 24
-// columns standing for what a tile costs besides its columns: a prompt of up to 256 rows spreads over all SMs (256 x
-// 4096 x 4096: 13.7 us, with 256 columns 15.7; 2048 x 2048 x 1536: 10.7 and 11.6; no difference from two waves on).
-// With experts only the waste at the right edge is known: the tiles share it (520 columns: three tiles of 192, not
-// 256 + 256 + 8).
-static int tile_columns(int64_t layout_rows, int N, bool experts) {
-    const int64_t pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, m = (layout_rows + 255) / 256;
-    const int fewest = (N + F8_TILE_N - 1) / F8_TILE_N;
+// Rows of a per tile.  High tiles read the weights least often; but the launch takes as long as its fullest pair of SMs,
+// so where the number of rows is known (no experts) the height that makes waves * (height + 128) smallest is taken: a
+// tile costs its rows, and its loads of the weights as much as 128 rows more.  256 x 4096 x 4096: 13.5 us, with 256 rows
+// per tile 15.4; 256 x 2048 x 1536: 8.5 and 10.6; but 4096 x 4096 x 4096, where a rule that took the weights for 24 rows
+// split into tiles of 128: 51.5, against 75; 2048 x 4096 x 4096: 27.5 against 34.
+static int rows_per_tile(int64_t rows, int N) {
+    const int64_t pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1, w = (N + 255) / 256;
+    const int64_t fewest = (rows + F8_TILE_ROWS - 1) / F8_TILE_ROWS;
     int best = 0;
     int64_t best_cost = 0;
-    for (int n = fewest; n <= N / 64 + 1; ++n) {
-        const int width = ((N + n - 1) / n + 31) / 32 * 32;  // paired MMAs take whole 32 columns
-        const int64_t tiles = (N + width - 1) / width;
-        const int64_t cost = (m * tiles + pairs - 1) / pairs * (width + 24);
+    for (int64_t n = fewest; n <= rows / 64 + 1; ++n) {
+        const int64_t height = ((rows + n - 1) / n + 31) / 32 * 32;  // paired MMAs take whole 32 columns
+        const int64_t tiles = (rows + height - 1) / height;
+        const int64_t cost = (w * tiles + pairs - 1) / pairs * (height + 128);
         if (best == 0 || cost < best_cost) {
-            best = width;
+            best = static_cast<int>(height);
             best_cost = cost;
         }
-        if (experts || m * n > 16 * pairs) break;  // many waves: the widest tile
+        if (w * n > 16 * pairs) break;  // many waves: the highest tile
     }
     return best;
 }
 
-// Whether tiles of 128 weight rows and up to 128 rows of x, spread over clusters along k, are the faster way.  Measured,
-// x quantised in both: 4096 x 4096, 32 / 64 / 96 rows 8.7 / 10.1 / 11.3 us against 14.7 / 15.1 / 15.3 with pair tiles;
-// 14336 x 4096 (many tiles, little to split) 18.4 / 19.9 / 22.0 against 19.3 / 19.6 / 19.9; 4096 x 14336 18.2 / 20.1 / 22.6
-// and 25.1 for 128 rows against 36.2 to 37.3; 128 experts of 1536 x 2048, 16 / 32 / 64 rows each 95 / 100 / 116 against
-// 105 / 107 / 115.
+// Whether tiles of 128 weight rows and up to 128 rows of x, spread over clusters along k, are the faster way: with few
+// rows, where the pair tiles leave at least half of the pairs without work.  Measured (this way / pair tiles): one matrix
+// of 4096 x 4096 (16 tiles), 16 / 32 / 48 rows 7.9 / 8.7 / 9.1 us against 12.9 / 13.0 / 13.3, 4096 x 14336 (16) 20.5 / 21.3 /
+// 22.2 against 33.9 to 34.5, two experts of 4096 x 4096 (32) 13.4 / 14.1 / 14.9 against 13.9 / 14.3 / 14.5, of 4096 x 14336
+// 27.7 / 28.7 / 29.5 against 36.4 to 37.3; but 14336 x 4096 (56) 16.4 / 17.3 / 18.3 against 16.0 / 16.2 / 16.5, eight
+// experts of 4096 x 4096 (128) 31 to 32 against 30 to 31, 128 of 1536 x 2048 80 / 84 / 89 against 76 / 77 / 79.
 static bool some_rows_suit(int64_t layout_rows, int64_t out_rows, int32_t E, int32_t N, int32_t K, bool experts, bool tile_rows) {
-    if (!fp8_some_rows_fits(K)) return false;
+    if (!fp8_some_rows_fits(K) || E * ((N + 255LL) / 256) * 2 > sm_count() / 2) return false;
     if (!experts) return layout_rows <= 64 || (layout_rows <= 96 && K >= N) || (layout_rows <= 128 && K >= 2LL * N);
     return tile_rows && out_rows <= 48LL * E;  // without tile_rows the rows of a layout are not known here
 }
@@ -432,7 +465,7 @@ static int launch_fp8(GemmFp8Params& p, cudaStream_t s) {
         FMAB_CUDA(cudaFuncSetAttribute(gemm_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)F8_SMEM));
         configured[dev] = true;
     }
-    const int64_t total = (p.layout_rows + 255) / 256 * p.n_ntiles;
+    const int64_t total = (p.layout_rows + p.tile_rows_most - 1) / p.tile_rows_most * p.w_ntiles;
     FMAB_REQUIRE(total < (1LL << 31), FMA_B200_ERR_BAD_ARG, "too many tiles");
     const int64_t max_pairs = sm_count() >= 2 ? sm_count() / 2 : 1;
     const int pairs = static_cast<int>(total < max_pairs ? total : max_pairs);
@@ -477,16 +510,17 @@ int fma_b200_fp8_gemm(const void* a, const void* a_scales, int64_t layout_rows, 
     p.layout_rows = layout_rows;
     p.n_cols = N;
     p.k_blocks = (K + BK8 - 1) / BK8;
-    p.tile_n = tile_columns(layout_rows, N, tile_expert != nullptr);
-    p.n_ntiles = (N + p.tile_n - 1) / p.tile_n;
+    p.tile_rows_most = tile_expert || tile_row || tile_rows ? F8_TILE_ROWS : rows_per_tile(layout_rows, N);
+    p.w_ntiles = (N + 255) / 256;
     p.a_scales = static_cast<const uint8_t*>(a_scales);
-    p.b_scales = static_cast<const uint8_t*>(w_scales);
+    p.w_scales = static_cast<const uint8_t*>(w_scales);
     p.a_tiles = static_cast<int32_t>(fp8_row_tiles(layout_rows));
-    p.b_tiles_expert = static_cast<int32_t>(fp8_row_tiles(N));
-    p.b_tiles = E * p.b_tiles_expert;
+    p.w_tiles_expert = static_cast<int32_t>(fp8_row_tiles(N));
+    p.w_tiles = E * p.w_tiles_expert;
     p.f16 = dtype == FMA_B200_F16 ? 1 : 0;
-    if (int rc = encode_bytes(&p.map_a, a, K, layout_rows, fp8_pitch(K), 128)) return rc;
-    if (int rc = encode_bytes(&p.map_b, w, K, static_cast<uint64_t>(E) * N, fp8_pitch(K), p.tile_n / 2)) return rc;
+    for (int b = 0; b < F8_BOXES; ++b)
+        if (int rc = encode_bytes(&p.map_a[b], a, K, layout_rows, fp8_pitch(K), 16 << b)) return rc;
+    if (int rc = encode_bytes(&p.map_w, w, K, static_cast<uint64_t>(E) * N, fp8_pitch(K), 128)) return rc;
     return launch_fp8(p, static_cast<cudaStream_t>(stream));
 }
 

@@ -459,8 +459,10 @@ int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, 
  * out[r, :] = a[r, :] . w[e(r)]^T for 8-bit a [layout_rows, K] (1 x 128 blocks) and w [E, N, K] (128 x 128 blocks),
  * fp32 sums, out bfloat16 or half with row pitch N.  tile_expert / tile_row / tile_rows as from group_maps (or the
  * mtile_expert of fma_b200_moe_sort with NULL, NULL); all NULL: one expert, row for row.  Tiles of expert -2 get
- * zeros.  rows_used (device, may be NULL): layout rows in use.  N and K are multiples of 8.  Runs on 256 x 256 tiles of
- * CTA pairs, or, with few rows per expert, on tiles of 128 weight rows that clusters share along K.
+ * zeros.  rows_used (device, may be NULL): layout rows in use.  N and K are multiples of 8.  Runs on tiles of 256
+ * weight rows x up to 256 rows of CTA pairs, or, with few rows and few such tiles, on tiles of 128 weight rows that
+ * clusters share along K.  Where tile_rows is given, tiles are as high as their rows; rows of the layout that it leaves
+ * out are not written.
  */
 int fma_b200_fp8_gemm(const void* a, const void* a_scales, int64_t layout_rows, const void* w, const void* w_scales,
                       int32_t E, int32_t N, int32_t K, void* out, int32_t dtype, int64_t out_rows,
