@@ -1,5 +1,5 @@
 // Kernels around the 8-bit format of fp8.cuh: quantising rows (plain, grouped by expert, or scattered to the expert
-// layout of the MoE layer), quantising weights with their transposed copy, dequantising, and SwiGLU that keeps its
+// layout of the MoE layer), quantising weights, dequantising, and SwiGLU that keeps its
 // inputs in 8 bits for the backward pass.  All are bound by HBM traffic: one pass over the data, 128-bit reads, every
 // value read once and written once; the block maximum lives in registers between the two.
 #include "fp8.cuh"
@@ -149,28 +149,17 @@ __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRow
 }
 
 // ---- weights ---------------------------------------------------------------------------------------
-// One CTA per block of 128 x 128.  A thread holds 8 rows x 8 columns: its rows leave as 8-byte pieces, and the 8 x 8
-// bytes transposed in registers go through shared memory into the transposed copy, whose rows also leave whole.
-__device__ __forceinline__ void transpose_4x4(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
-    const uint32_t ab_lo = __byte_perm(a, b, 0x5140), ab_hi = __byte_perm(a, b, 0x7362);
-    const uint32_t cd_lo = __byte_perm(c, d, 0x5140), cd_hi = __byte_perm(c, d, 0x7362);
-    a = __byte_perm(ab_lo, cd_lo, 0x5410);
-    b = __byte_perm(ab_lo, cd_lo, 0x7632);
-    c = __byte_perm(ab_hi, cd_hi, 0x5410);
-    d = __byte_perm(ab_hi, cd_hi, 0x7632);
-}
-
+// One CTA per block of 128 x 128.  A thread holds 8 rows x 8 columns; its rows leave as 8-byte pieces.
 struct QuantWeight {
     const void* w;
-    uint8_t *values, *scales, *values_t, *scales_t;
-    int32_t E, N, K, pitch, pitch_t;  // pitch_t: of the transposed copy [E, K, pitch_t]
-    int32_t n_blocks, k_blocks;       // per expert
+    uint8_t *values, *scales;
+    int32_t E, N, K, pitch;
+    int32_t n_blocks, k_blocks;  // per expert
 };
 
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_weight_kernel(const QuantWeight p) {
     __shared__ uint32_t warp_max[8];
-    __shared__ __align__(16) uint8_t turned[FP8_BLOCK][FP8_BLOCK];  // 8-byte pieces of column c at piece ^ (c / 8 % 16): no bank conflicts
     allow_next();
     wait_for_previous();
     constexpr int V = Elem<T>::kPerVec;
@@ -220,44 +209,19 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const QuantWeight 
     }
     const uint32_t byte = fp8_scale_byte(m);
     const float inverse = fp8_inverse(byte);
-    uint32_t lo[8], hi[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8 / V; ++j) Elem<T>::unpack(raw[i][j], x + j * V);
-        lo[i] = finite ? fp8_pack4_finite(x, inverse) : fp8_pack4(x, inverse);
-        hi[i] = finite ? fp8_pack4_finite(x + 4, inverse) : fp8_pack4(x + 4, inverse);
+        const uint32_t lo = finite ? fp8_pack4_finite(x, inverse) : fp8_pack4(x, inverse);
+        const uint32_t hi = finite ? fp8_pack4_finite(x + 4, inverse) : fp8_pack4(x + 4, inverse);
         if (r0 + i < p.N && c0 < p.pitch)
-            *reinterpret_cast<uint2*>(p.values + (static_cast<int64_t>(e) * p.N + r0 + i) * p.pitch + c0) = make_uint2(lo[i], hi[i]);
+            *reinterpret_cast<uint2*>(p.values + (static_cast<int64_t>(e) * p.N + r0 + i) * p.pitch + c0) = make_uint2(lo, hi);
     }
     if (tid < FP8_BLOCK)
         p.scales[fp8_scale_word((static_cast<int64_t>(e) * p.n_blocks + nb) * FP8_BLOCK + tid, kb >> 2,
                                 static_cast<int64_t>(p.E) * p.n_blocks) + (kb & 3)] = static_cast<uint8_t>(byte);
-    if (p.values_t == nullptr) return;
-    if (tid < FP8_BLOCK)
-        p.scales_t[fp8_scale_word((static_cast<int64_t>(e) * p.k_blocks + kb) * FP8_BLOCK + tid, nb >> 2,
-                                  static_cast<int64_t>(p.E) * p.k_blocks) + (nb & 3)] = static_cast<uint8_t>(byte);
-    transpose_4x4(lo[0], lo[1], lo[2], lo[3]);  // lo[j] = rows 0-3 of column j
-    transpose_4x4(lo[4], lo[5], lo[6], lo[7]);  // lo[4 + j] = rows 4-7 of column j
-    transpose_4x4(hi[0], hi[1], hi[2], hi[3]);
-    transpose_4x4(hi[4], hi[5], hi[6], hi[7]);
-    const int tc = (tid & 15) * 8, tr = (tid >> 4) * 8;
-    const int to = tr ^ ((tid & 15) * 8);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        *reinterpret_cast<uint2*>(&turned[tc + j][to]) = make_uint2(lo[j], lo[4 + j]);
-        *reinterpret_cast<uint2*>(&turned[tc + 4 + j][to]) = make_uint2(hi[j], hi[4 + j]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int piece = i * 256 + tid, col = piece >> 3, at = (piece & 7) * 16, key = (col >> 3) & 15;
-        const int k = kb * FP8_BLOCK + col, n = nb * FP8_BLOCK + at;
-        uint4 v = *reinterpret_cast<const uint4*>(&turned[col][at ^ ((key & 14) * 8)]);
-        if (key & 1) v = make_uint4(v.z, v.w, v.x, v.y);
-        if (k < p.K && n < p.pitch_t) st_global_16(p.values_t + (static_cast<int64_t>(e) * p.K + k) * p.pitch_t + n, v);
-    }
 }
 
 // ---- back to 16 or 32 bits -------------------------------------------------------------------------
@@ -664,27 +628,23 @@ int fma_b200_fp8_quantize_scatter(const void* x, int32_t dtype, int64_t T, int64
 }
 
 int fma_b200_fp8_quantize_weight(const void* w, int32_t dtype, int32_t E, int32_t N, int32_t K, void* values,
-                                 void* scales, void* values_t, void* scales_t, void* stream) {
+                                 void* scales, void* stream) {
     using namespace fmab;
     if (int rc = check_rows_cols(dtype, N, K)) return rc;
     FMAB_REQUIRE(E >= 1 && E <= 1024, FMA_B200_ERR_BAD_ARG, "E=%d not in [1,1024]", E);
     FMAB_REQUIRE(N >= 8 && N % 8 == 0, FMA_B200_ERR_BAD_ARG, "N=%d must be a positive multiple of 8", N);
     FMAB_REQUIRE(static_cast<int64_t>(E) * N < (1LL << 31) - 1024 && static_cast<int64_t>(E) * K < (1LL << 31) - 1024,
                  FMA_B200_ERR_BAD_ARG, "E*N or E*K overflows");
-    FMAB_REQUIRE(w && values && scales && (values_t == nullptr) == (scales_t == nullptr), FMA_B200_ERR_BAD_ARG, "NULL pointer");
-    FMAB_REQUIRE(aligned16(w) && aligned16(values) && aligned16(scales) && aligned16(values_t) && aligned16(scales_t),
-                 FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
+    FMAB_REQUIRE(w && values && scales, FMA_B200_ERR_BAD_ARG, "NULL pointer");
+    FMAB_REQUIRE(aligned16(w) && aligned16(values) && aligned16(scales), FMA_B200_ERR_BAD_ARG, "pointers not 16-byte aligned");
     QuantWeight p;
     p.w = w;
     p.values = static_cast<uint8_t*>(values);
     p.scales = static_cast<uint8_t*>(scales);
-    p.values_t = static_cast<uint8_t*>(values_t);
-    p.scales_t = static_cast<uint8_t*>(scales_t);
     p.E = E;
     p.N = N;
     p.K = K;
     p.pitch = static_cast<int32_t>(fp8_pitch(K));
-    p.pitch_t = static_cast<int32_t>(fp8_pitch(N));
     p.n_blocks = (N + FP8_BLOCK - 1) / FP8_BLOCK;
     p.k_blocks = (K + FP8_BLOCK - 1) / FP8_BLOCK;
     FMAB_REQUIRE(static_cast<int64_t>(p.n_blocks) * p.k_blocks < (1LL << 31), FMA_B200_ERR_BAD_ARG, "N*K overflows");

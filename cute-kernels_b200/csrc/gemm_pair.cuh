@@ -73,6 +73,12 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar), "r"(c0), "r"(c1)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t leader_bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
 __device__ __forceinline__ void tc_mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -98,19 +104,24 @@ __device__ __forceinline__ void tc_commit_both(uint32_t bar) {
         ::"r"(bar), "h"(static_cast<uint16_t>(3))
         : "memory");
 }
-// Bytes [outer, inner] with row pitch `pitch`, boxes of box_outer rows x 128 bytes, 128-byte swizzle.
-inline int encode_bytes(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_outer) {
+// Bytes [batch, outer, inner] with row pitch `pitch`, boxes of box_outer rows x 128 bytes, 128-byte swizzle.  Boxes that
+// reach beyond `outer` read zeros there, not the next batch.
+inline int encode_bytes_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t batch, uint64_t pitch, uint32_t box_outer,
+                           uint32_t rank = 3) {
     EncodeTiledFn fn = encode_fn();
     FMAB_REQUIRE(fn != nullptr, FMA_B200_ERR_LAUNCH, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint64_t dims[2] = {inner, outer};
-    const cuuint64_t strides[1] = {pitch};
-    const cuuint32_t box[2] = {128, box_outer};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+    const cuuint64_t dims[3] = {inner, outer, batch};
+    const cuuint64_t strides[2] = {pitch, outer * pitch};
+    const cuuint32_t box[3] = {128, box_outer, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     FMAB_REQUIRE(r == CUDA_SUCCESS, FMA_B200_ERR_LAUNCH, "cuTensorMapEncodeTiled (8-bit operand) failed with CUresult %d", (int)r);
     return FMA_B200_OK;
+}
+inline int encode_bytes(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_outer) {
+    return encode_bytes_3d(map, base, inner, outer, 1, pitch, box_outer, 2);
 }
 
 }  // namespace fmab

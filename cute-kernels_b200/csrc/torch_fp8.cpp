@@ -131,33 +131,19 @@ std::shared_ptr<Blocks> quantize_fp8(const Tensor& x) {
     return std::make_shared<Blocks>(Blocks{quantize_rows(rows_2d(x)), x.sizes().vec(), x.scalar_type()});
 }
 
-// What quantize_fp8_weight returns: values then scales in one buffer, and with `transpose` those of the transposed copy in
-// another, so that a backward pass keeps that one alone alive.
+// What quantize_fp8_weight returns: values, then scales, in one buffer.
 struct Weight {
-    Tensor buffer, buffer_t;
+    Tensor buffer;
     std::vector<int64_t> shape;
     at::ScalarType dtype;
     int64_t E, N, K;
-    bool turned() const { return buffer_t.defined(); }
     int64_t tiles_rows(int64_t n) const { return E * ((n + 127) / 128) * 128; }
     int64_t value_bytes() const { return E * N * pitch_of(K); }
     int64_t scale_bytes() const { return fma_b200_fp8_scale_bytes(tiles_rows(N), K); }
-    int64_t value_bytes_t() const { return E * K * pitch_of(N); }
-    int64_t scale_bytes_t() const { return fma_b200_fp8_scale_bytes(tiles_rows(K), N); }
     uint8_t* values() const { return buffer.data_ptr<uint8_t>(); }
     uint8_t* scales() const { return values() + value_bytes(); }
-    uint8_t* values_t() const { return buffer_t.data_ptr<uint8_t>(); }
-    uint8_t* scales_t() const { return values_t() + value_bytes_t(); }
     Tensor values_tensor() const { return buffer.narrow(0, 0, value_bytes()).view(at::kFloat8_e4m3fn).view({E, N, pitch_of(K)}); }
     Tensor scales_tensor() const { return buffer.narrow(0, value_bytes(), scale_bytes()); }
-    py::object transposed() const {
-        if (!turned()) return py::none();
-        return py::cast(buffer_t.narrow(0, 0, value_bytes_t()).view(at::kFloat8_e4m3fn).view({E, K, pitch_of(N)}));
-    }
-    py::object transposed_scales() const {
-        if (!turned()) return py::none();
-        return py::cast(buffer_t.narrow(0, value_bytes_t(), scale_bytes_t()));
-    }
     Tensor dequantized(const py::object& to) const {
         const c10::cuda::CUDAGuard guard(buffer.device());
         return dequantize(values(), scales(), E, N, shape, scalar_type_or(to, dtype), buffer, nullptr);
@@ -165,7 +151,7 @@ struct Weight {
 };
 using WeightPtr = std::shared_ptr<Weight>;
 
-WeightPtr quantize_fp8_weight(const Tensor& weight, bool transpose) {
+WeightPtr quantize_fp8_weight(const Tensor& weight) {
     require_cuda(weight);
     const int32_t code = dtype_code(weight.scalar_type());
     TORCH_CHECK(weight.dim() == 2 || weight.dim() == 3, "quantize_fp8_weight: weight must be [N, K] or [experts, N, K], got ", weight.sizes());
@@ -176,12 +162,10 @@ WeightPtr quantize_fp8_weight(const Tensor& weight, bool transpose) {
     Tensor w = weight.contiguous();
     if (!aligned(w)) w = w.clone();
     auto held = std::make_shared<Weight>(
-        Weight{Tensor(), Tensor(), weight.sizes().vec(), weight.scalar_type(), w.dim() == 3 ? w.size(0) : 1, w.size(-2), w.size(-1)});
+        Weight{Tensor(), weight.sizes().vec(), weight.scalar_type(), w.dim() == 3 ? w.size(0) : 1, w.size(-2), w.size(-1)});
     held->buffer = bytes(held->value_bytes() + held->scale_bytes(), w);
-    if (transpose) held->buffer_t = bytes(held->value_bytes_t() + held->scale_bytes_t(), w);
     check(fma_b200_fp8_quantize_weight(w.data_ptr(), code, static_cast<int32_t>(held->E), static_cast<int32_t>(held->N),
-                                       static_cast<int32_t>(held->K), held->values(), held->scales(), transpose ? held->values_t() : nullptr,
-                                       transpose ? held->scales_t() : nullptr, stream_of(w)),
+                                       static_cast<int32_t>(held->K), held->values(), held->scales(), stream_of(w)),
           "fma_b200_fp8_quantize_weight");
     return held;
 }
@@ -221,14 +205,14 @@ Held quantize_groups(const Tensor& x, const GroupMaps& m, void* copy) {
     return held;
 }
 
-// [rows, N] = rows of `a` times the rows of a weight copy, both reduced over a's columns.
-Tensor product(const Held& a, const uint8_t* w_values, const uint8_t* w_scales, int64_t E, int64_t N, at::ScalarType dtype, int64_t rows,
-               const GroupMaps* m) {
-    Tensor out = at::empty({rows, N}, a.buffer.options().dtype(dtype));
-    check(fma_b200_fp8_gemm(a.values(), a.scales(), a.rows, w_values, w_scales, static_cast<int32_t>(E), static_cast<int32_t>(N),
-                            static_cast<int32_t>(a.cols), out.data_ptr(), dtype_code(dtype), rows, m ? m->tile_expert() : nullptr,
-                            m ? m->tile_row() : nullptr, m ? m->tile_rows() : nullptr, m ? m->used_all() : nullptr, stream_of(out)),
-          "fma_b200_fp8_gemm");
+// [rows, N] = a . w^T, or with `turned` [rows, K] = a . w.
+Tensor product(const Held& a, const Weight& w, bool turned, at::ScalarType dtype, int64_t rows, const GroupMaps* m) {
+    Tensor out = at::empty({rows, turned ? w.K : w.N}, a.buffer.options().dtype(dtype));
+    check((turned ? fma_b200_fp8_gemm_dgrad : fma_b200_fp8_gemm)(
+              a.values(), a.scales(), a.rows, w.values(), w.scales(), static_cast<int32_t>(w.E), static_cast<int32_t>(w.N), static_cast<int32_t>(w.K),
+              out.data_ptr(), dtype_code(dtype), rows, m ? m->tile_expert() : nullptr, m ? m->tile_row() : nullptr,
+              m ? m->tile_rows() : nullptr, m ? m->used_all() : nullptr, stream_of(out)),
+          turned ? "fma_b200_fp8_gemm_dgrad" : "fma_b200_fp8_gemm");
     return out;
 }
 
@@ -255,8 +239,8 @@ struct Linear : torch::autograd::Function<Linear> {
         GroupMaps maps;
         if (grouped) maps = make_maps(*counts, x.size(0));
         const Held rows = grouped ? quantize_groups(x, maps, nullptr) : quantize_rows(x);
-        Tensor out = product(rows, held->values(), held->scales(), held->E, held->N, x.scalar_type(), x.size(0), grouped ? &maps : nullptr);
-        ctx->save_for_backward({want_w ? rows.buffer : Tensor(), want_x ? held->buffer_t : Tensor(), maps.buffer});
+        Tensor out = product(rows, *held, false, x.scalar_type(), x.size(0), grouped ? &maps : nullptr);
+        ctx->save_for_backward({want_w ? rows.buffer : Tensor(), want_x ? held->buffer : Tensor(), maps.buffer});
         ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), held->E, held->N, held->K, grouped, want_x, want_w};
         return out;
     }
@@ -283,8 +267,8 @@ struct Linear : torch::autograd::Function<Linear> {
             d8 = quantize_groups(d_out, maps, want_w ? d_rows.data_ptr() : nullptr);
         }
         if (want_x) {
-            const Weight w{Tensor(), saved[1], {}, dtype, E, N, K};
-            d_x = product(d8, w.values_t(), w.scales_t(), E, K, dtype, rows, grouped ? &maps : nullptr);
+            const Weight w{saved[1], {}, dtype, E, N, K};
+            d_x = product(d8, w, true, dtype, rows, grouped ? &maps : nullptr);
         }
         if (want_w) {
             const Held x8(saved[0], layout, K);
@@ -339,7 +323,6 @@ Tensor linear(const char* name, const Tensor& x, const py::object& weight, const
     check_cols(name, K);
     const bool grad = at::GradMode::is_enabled();
     const bool want_x = grad && x.requires_grad(), want_w = grad && parameter.defined() && parameter.requires_grad();
-    TORCH_CHECK(!want_x || !held || held->turned(), name, ": the gradient of x needs quantize_fp8_weight(weight, transpose=True)");
     std::vector<int64_t> out_shape = x.sizes().vec();
     out_shape.back() = N;
     const int64_t rows = x.numel() / K;
@@ -351,7 +334,7 @@ Tensor linear(const char* name, const Tensor& x, const py::object& weight, const
         return out;
     }
     const c10::cuda::CUDAGuard guard(x.device());
-    if (!held) held = quantize_fp8_weight(parameter, want_x);
+    if (!held) held = quantize_fp8_weight(parameter);
     const Tensor x2 = rows_2d(x);
     if (grouped) counts = counts.contiguous();
     Tensor out;
@@ -364,7 +347,7 @@ Tensor linear(const char* name, const Tensor& x, const py::object& weight, const
         GroupMaps maps;
         if (grouped) maps = make_maps(counts, rows);
         const Held a = grouped ? quantize_groups(x2, maps, nullptr) : quantize_rows(x2);
-        out = product(a, held->values(), held->scales(), held->E, N, x.scalar_type(), rows, grouped ? &maps : nullptr);
+        out = product(a, *held, false, x.scalar_type(), rows, grouped ? &maps : nullptr);
     }
     return x.dim() == 2 ? out : out.view(out_shape);
 }
@@ -464,36 +447,28 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             }));
     py::class_<Weight, WeightPtr>(m, "Fp8Weight",
                                   "A weight [N, K] or [E, N, K] held in 8 bits with a scale per 128 x 128 block: e4m3 `values` (row pitch: K "
-                                  "rounded up to 16) and `scales` in the order in which the tensor cores read them.  `transposed` is the second "
-                                  "copy that input gradients read, or None.")
+                                  "rounded up to 16) and `scales` in the order in which the tensor cores read them.")
         .def_property_readonly("values", &Weight::values_tensor)
         .def_property_readonly("scales", &Weight::scales_tensor)
-        .def_property_readonly("transposed", &Weight::transposed)
-        .def_property_readonly("transposed_scales", &Weight::transposed_scales)
-        .def_property_readonly("forward_buffer", [](const Weight& w) { return w.buffer; }, "What values and scales lie in.")
-        .def_property_readonly("transposed_buffer", [](const Weight& w) { return w.turned() ? py::cast(w.buffer_t) : py::object(py::none()); },
-                               "What the transposed copy and its scales lie in, or None.")
+        .def_property_readonly("buffer", [](const Weight& w) { return w.buffer; }, "What values and scales lie in.")
         .def_property_readonly(
             "addresses",
             [](const Weight& w) {
                 auto at = [](uint8_t* p) { return reinterpret_cast<uintptr_t>(p); };
-                return py::make_tuple(at(w.values()), at(w.scales()), w.turned() ? at(w.values_t()) : 0, w.turned() ? at(w.scales_t()) : 0);
+                return py::make_tuple(at(w.values()), at(w.scales()));
             },
-            "Device addresses of values, scales, transposed and transposed_scales (0: not there).")
+            "Device addresses of values and scales.")
         .def_property_readonly("shape", [](const Weight& w) { return shape_object(w.shape); })
         .def_property_readonly("dtype", [](const Weight& w) { return dtype_object(w.dtype); })
         .def_property_readonly("device", [](const Weight& w) { return py::cast(w.buffer).attr("device"); })
         .def("dequantize", &Weight::dequantized, py::arg("dtype") = py::none(),
              "The values it stands for, rounded to `dtype` (default: the type it was made from).")
         .def(py::pickle(
-            [](const Weight& w) {
-                return py::make_tuple(w.buffer, w.turned() ? py::cast(w.buffer_t) : py::object(py::none()), w.shape, static_cast<int>(w.dtype),
-                                      w.E, w.N, w.K);
-            },
+            [](const Weight& w) { return py::make_tuple(w.buffer, w.shape, static_cast<int>(w.dtype), w.E, w.N, w.K); },
             [](const py::tuple& t) {
-                return std::make_shared<Weight>(Weight{t[0].cast<Tensor>(), t[1].is_none() ? Tensor() : t[1].cast<Tensor>(),
-                                                       t[2].cast<std::vector<int64_t>>(), static_cast<at::ScalarType>(t[3].cast<int>()),
-                                                       t[4].cast<int64_t>(), t[5].cast<int64_t>(), t[6].cast<int64_t>()});
+                return std::make_shared<Weight>(Weight{t[0].cast<Tensor>(), t[1].cast<std::vector<int64_t>>(),
+                                                       static_cast<at::ScalarType>(t[2].cast<int>()), t[3].cast<int64_t>(), t[4].cast<int64_t>(),
+                                                       t[5].cast<int64_t>()});
             }));
     for (const char* name : {"Fp8Blocks", "Fp8Weight"}) m.attr(name).attr("__module__") = "fma_b200";  // where pickle finds them
     m.def("few", &few, "Whether this many rows take the one-launch product (rows, experts, width).");

@@ -43,7 +43,7 @@ def _quantize_rows(x: torch.Tensor, rows_used: int) -> _Held:
 
 def _few_rows(x: torch.Tensor, held, counts: torch.Tensor) -> torch.Tensor:
     E, N, K_ = held.shape
-    values, scales, _, _ = held.addresses
+    values, scales = held.addresses
     out = torch.empty(x.size(0), N, dtype=x.dtype, device=x.device)
     call("fma_b200_fp8_few_rows", ptr(x), x.stride(0), dtype_code(x.dtype), x.size(0), values, scales, E, N, K_, ptr(counts),
          counts.element_size(), ptr(out), stream_ptr(x.device))  # fmt: skip
@@ -64,10 +64,12 @@ def _used(maps: K.RowMaps) -> int:
     return maps.pad_offsets.data_ptr() + 4 * maps.num_experts
 
 
-def _product(a: _Held, w_values: int, w_scales: int, N: int, dtype, maps: K.RowMaps) -> torch.Tensor:
+def _product(a: _Held, w_values: int, w_scales: int, cols: int, dtype, maps: K.RowMaps, dgrad: bool = False) -> torch.Tensor:
+    """a . w^T per expert, or with `dgrad` a . w; `cols` of the result."""
     dev = a.buffer.device
-    out = torch.empty(maps.rows_cap, N, dtype=dtype, device=dev)
-    call("fma_b200_fp8_gemm", a.values, a.scales, maps.rows_cap, w_values, w_scales, maps.num_experts, N, a.cols,
+    out = torch.empty(maps.rows_cap, cols, dtype=dtype, device=dev)
+    name, N, K_ = ("fma_b200_fp8_gemm_dgrad", a.cols, cols) if dgrad else ("fma_b200_fp8_gemm", cols, a.cols)
+    call(name, a.values, a.scales, maps.rows_cap, w_values, w_scales, maps.num_experts, N, K_,
          ptr(out), dtype_code(dtype), maps.rows_cap, ptr(maps.mtile_expert), None, None, _used(maps),
          stream_ptr(dev))  # fmt: skip
     return out
@@ -93,27 +95,25 @@ class Fp8SwigluExperts(torch.autograd.Function):
         I, dev, cap = held_proj.shape[-1], x.device, maps.rows_cap
         x8 = _quantize_scatter(x, maps)
         fc, proj = held_fc.addresses, held_proj.addresses
-        pre = _product(x8, *fc[:2], 2 * I, x.dtype, maps)
+        pre = _product(x8, *fc, 2 * I, x.dtype, maps)
         keep = any(ctx.needs_input_grad)
         act8, up8, gate8 = _Held(cap, I, dev), *((_Held(cap, I, dev) if keep else None) for _ in range(2))
         at = (gate8.values, gate8.scales, up8.values, up8.scales) if keep else (None,) * 4
         call("fma_b200_swiglu_fp8_forward", pre.data_ptr() + I * pre.element_size(), 2 * I, ptr(pre), 2 * I, None, I,
              dtype_code(x.dtype), cap, I, _used(maps), *at, act8.values, act8.scales, stream_ptr(dev))  # fmt: skip
         del pre
-        out = _product(act8, *proj[:2], H, x.dtype, maps)
+        out = _product(act8, *proj, H, x.dtype, maps)
         y = K.combine(out, weights, maps, T)
         if keep:
-            # of the weights the transposed copies alone
-            ctx.save_for_backward(x8.buffer, up8.buffer, gate8.buffer, act8.buffer, out, weights, held_fc.transposed_buffer,
-                                  held_proj.transposed_buffer)  # fmt: skip
-            ctx.turned = fc[3] - fc[2], proj[3] - proj[2]  # where their scales begin
+            ctx.save_for_backward(x8.buffer, up8.buffer, gate8.buffer, act8.buffer, out, weights, held_fc.buffer, held_proj.buffer)
+            ctx.scales_at = fc[1] - fc[0], proj[1] - proj[0]  # where the weights' scales begin
         ctx.maps, ctx.sizes, ctx.dtype = maps, (T, H, I), x.dtype
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x8, up8, gate8, act8, out, weights, fc_t, proj_t = ctx.saved_tensors
-        fc_t, proj_t = ((b.data_ptr(), b.data_ptr() + at) for b, at in zip((fc_t, proj_t), ctx.turned))
+        x8, up8, gate8, act8, out, weights, fc, proj = ctx.saved_tensors
+        fc, proj = ((b.data_ptr(), b.data_ptr() + at) for b, at in zip((fc, proj), ctx.scales_at))
         maps, (T, H, I), dtype, dev = ctx.maps, ctx.sizes, ctx.dtype, dy.device
         cap, used = maps.rows_cap, _used(maps)
         x8 = _Held(cap, H, dev, x8)
@@ -125,7 +125,7 @@ class Fp8SwigluExperts(torch.autograd.Function):
             if need_proj:
                 d_w_proj = _weight_gradient(d_out, act8, maps)
             if need_x or need_fc:
-                d_act = _product(_quantize_rows(d_out, used), *proj_t, I, dtype, maps)
+                d_act = _product(_quantize_rows(d_out, used), *proj, I, dtype, maps, dgrad=True)
                 d_pre = torch.empty(cap, 2 * I, dtype=dtype, device=dev)
                 # the same pass quantises d_pre where its blocks of 128 columns do not straddle up and gate
                 d_pre8 = _Held(cap, 2 * I, dev) if need_x and I % 128 == 0 else None
@@ -136,7 +136,7 @@ class Fp8SwigluExperts(torch.autograd.Function):
                 if need_fc:
                     d_w_fc = _weight_gradient(d_pre, x8, maps)
                 if need_x:
-                    d_xg = _product(d_pre8 or _quantize_rows(d_pre, used), *fc_t, H, dtype, maps)
+                    d_xg = _product(d_pre8 or _quantize_rows(d_pre, used), *fc, H, dtype, maps, dgrad=True)
                     d_x = K.scatter_backward(d_xg, maps, T)
         return d_x, d_w, d_w_fc, d_w_proj, None, None, None
 

@@ -411,8 +411,8 @@ class MoE(nn.Module):
         return _Combine.apply(grouped, router_weights, maps, T)
 
     # ---- experts on 8-bit operands ------------------------------------------------------------------
-    def _experts_in_8_bits(self, transpose: bool):
-        return tuple(quantize_fp8_weight(w, transpose) for w in (self.c_fc.weight, self.c_proj.weight))
+    def _experts_in_8_bits(self):
+        return tuple(quantize_fp8_weight(w) for w in (self.c_fc.weight, self.c_proj.weight))
 
     def _expert_weights_seen(self):
         return tuple((w._version, w.data_ptr(), w.dtype, w.device) for w in (self.c_fc.weight, self.c_proj.weight))
@@ -423,7 +423,7 @@ class MoE(nn.Module):
         (otherwise, and whenever gradients are recorded, every forward quantises the weights it finds).  After the
         weights have changed, call it again; until then such a forward raises an error."""
         with torch.cuda.device(self.c_fc.weight.device):
-            self._held_experts = (*self._experts_in_8_bits(False), self._expert_weights_seen())
+            self._held_experts = (*self._experts_in_8_bits(), self._expert_weights_seen())
 
     def _compute_experts_fp8(self, hidden_states, router_weights, selected_experts):
         if not (self.is_glu and _is_swiglu_packed(self.act) and self.c_fc.bias is None and self.c_proj.bias is None):
@@ -440,7 +440,7 @@ class MoE(nn.Module):
                 raise RuntimeError("the expert weights have changed since quantize_experts(): call it again")
             held = self._held_experts[:2]
         if held is None:
-            held = self._experts_in_8_bits(graph)
+            held = self._experts_in_8_bits()
         if not graph and _fp8_experts.few(T * self.top_k, held[1]):
             maps = self._sort_selected(selected_experts, row_align=1)
             self.last_row_maps = maps

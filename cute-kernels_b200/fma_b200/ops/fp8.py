@@ -33,10 +33,10 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Blocks:
     return _native.binding().quantize_fp8(x)
 
 
-def quantize_fp8_weight(weight: torch.Tensor, transpose: bool = False) -> Fp8Weight:
-    """Holds weight [N, K] or [E, N, K] in 8 bits with a scale per 128 x 128 block.  With `transpose` also the
-    transposed copy that the input gradient of a linear map needs.  N and K must be multiples of 8."""
-    return _native.binding().quantize_fp8_weight(weight, transpose)
+def quantize_fp8_weight(weight: torch.Tensor) -> Fp8Weight:
+    """Holds weight [N, K] or [E, N, K] in 8 bits with a scale per 128 x 128 block, for a linear map and for its
+    input gradient.  N and K must be multiples of 8."""
+    return _native.binding().quantize_fp8_weight(weight)
 
 
 def linear_fp8(x: torch.Tensor, weight: torch.Tensor | Fp8Weight, quantized: Fp8Weight | None = None) -> torch.Tensor:

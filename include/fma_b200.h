@@ -426,8 +426,7 @@ int fma_b200_grouped_gemm(const void* A, const void* B, void* D, const uint32_t*
  *                    receives the rows themselves, unquantised, in the same layout [layout_rows, cols].
  * quantize_scatter   token t goes to the k rows row_of_slot[t*k..] of the layout of fma_b200_moe_sort (negative:
  *                    nowhere), padding rows below pad_offsets[E] become zeros: fma_b200_moe_scatter in 8 bits
- * quantize_weight    w [E, N, K] -> values [E, N, pitch(K)] and scales of 128 x 128 blocks; with values_t also the
- *                    transposed copy [E, K, pitch(N)].  Scale tiles count ceil(N/128) (transposed: ceil(K/128))
+ * quantize_weight    w [E, N, K] -> values [E, N, pitch(K)] and scales of 128 x 128 blocks, which count ceil(N/128)
  *                    row tiles per expert, so their size is scale_bytes(E * ceil(N/128) * 128, K)
  * dequantize         batch matrices [rows, cols] with 1 x 128 or 128 x 128 blocks -> out, contiguous; what a rounding
  *                    to e4m3 lifted above the type's range becomes its largest finite value
@@ -442,7 +441,7 @@ int fma_b200_fp8_quantize_scatter(const void* x, int32_t dtype, int64_t T, int64
                                   const int32_t* row_of_slot, const int32_t* slot_of_row, const int32_t* pad_offsets,
                                   int32_t E, int64_t layout_rows, void* values, void* scales, void* stream);
 int fma_b200_fp8_quantize_weight(const void* w, int32_t dtype, int32_t E, int32_t N, int32_t K, void* values,
-                                 void* scales, void* values_t, void* scales_t, void* stream);
+                                 void* scales, void* stream);
 int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batch, int64_t rows, int64_t cols,
                             const int32_t* rows_used, void* out, int32_t dtype, void* stream);
 /*
@@ -468,6 +467,14 @@ int fma_b200_fp8_gemm(const void* a, const void* a_scales, int64_t layout_rows, 
                       int32_t E, int32_t N, int32_t K, void* out, int32_t dtype, int64_t out_rows,
                       const int32_t* tile_expert, const int32_t* tile_row, const int32_t* tile_rows,
                       const int32_t* rows_used, void* stream);
+/*
+ * Its input gradient: dx[r, :] = dy[r, :] . w[e(r)] for 8-bit dy [layout_rows, N] and the same w [E, N, K]; dx has row
+ * pitch K.  Always on the pair tiles, which read the weights as they lie.
+ */
+int fma_b200_fp8_gemm_dgrad(const void* dy, const void* dy_scales, int64_t layout_rows, const void* w, const void* w_scales,
+                            int32_t E, int32_t N, int32_t K, void* dx, int32_t dtype, int64_t out_rows,
+                            const int32_t* tile_expert, const int32_t* tile_row, const int32_t* tile_rows,
+                            const int32_t* rows_used, void* stream);
 /*
  * The same product for a few rows, in one launch: x [rows, K] in bfloat16 or half is quantised on the way in; counts
  * [E] (4- or 8-byte integers on the device, NULL: one expert) consecutive rows per expert, rows behind the last

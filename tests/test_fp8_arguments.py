@@ -37,10 +37,10 @@ def test_entry_points_refuse_bad_arguments():
     assert s(at, 1, 4, 16, 0, at, at, at, 2, 256, at, at, null) == BAD  # k
     assert s(at, 1, 4, 16, 2, at, null, at, 2, 256, at, at, null) == BAD
     w = lib.fma_b200_fp8_quantize_weight
-    assert w(at, 1, 1, 12, 16, at, at, null, null, null) == BAD  # N
-    assert w(at, 1, 2000, 16, 16, at, at, null, null, null) == BAD  # E
-    assert w(at, 1, 1, 16, 16, at, at, at, null, null) == BAD  # transposed values without scales
-    assert w(at, 1, 1024, 1 << 22, 16, at, at, null, null, null) == BAD  # E * N
+    assert w(at, 1, 1, 12, 16, at, at, null) == BAD  # N
+    assert w(at, 1, 2000, 16, 16, at, at, null) == BAD  # E
+    assert w(at, 1, 1, 16, 16, at, null, null) == BAD
+    assert w(at, 1, 1024, 1 << 22, 16, at, at, null) == BAD  # E * N
     d = lib.fma_b200_fp8_dequantize
     assert d(at, at, 0, 4, 16, null, at, 1, null) == BAD
     assert d(at, at, 1, 4, 16, null, at, 5, null) == UNSUPPORTED
@@ -57,6 +57,12 @@ def test_entry_points_refuse_bad_arguments():
     assert p(at, at, 256, at, at, 1, 16, 20, at, 1, 256, null, null, null, null, null) == BAD
     assert p(at, null, 256, at, at, 1, 16, 16, at, 1, 256, null, null, null, null, null) == BAD
     assert p(null, null, 0, null, null, 1, 16, 16, null, 1, 0, null, null, null, null, null) == OK
+    g = lib.fma_b200_fp8_gemm_dgrad
+    assert g(at, at, 256, at, at, 1, 16, 16, at, 0, 256, null, null, null, null, null) == UNSUPPORTED  # fp32 result
+    assert g(at, at, 256, at, at, 2, 16, 16, at, 1, 256, null, null, null, null, null) == BAD  # experts without a table
+    assert g(at, at, 256, at, odd, 1, 16, 16, at, 1, 256, null, null, null, null, null) == BAD
+    assert g(at, at, 256, at, at, 1024, 1 << 22, 16, at, 1, 256, at, null, null, null, null) == BAD  # E * N
+    assert g(null, null, 0, null, null, 1, 16, 16, null, 1, 0, null, null, null, null, null) == OK
     f = lib.fma_b200_fp8_few_rows
     assert f(at, 16, 0, 4, at, at, 1, 16, 16, null, 4, at, null) == UNSUPPORTED
     assert f(at, 8, 1, 4, at, at, 1, 16, 16, null, 4, at, null) == BAD

@@ -82,12 +82,10 @@ def test_weight(dtype, shape):
     import fma_b200 as fma
 
     w = randn(shape, dtype, 4, scale=0.02).to(DEV)
-    held = fma.quantize_fp8_weight(w, transpose=True)
+    held = fma.quantize_fp8_weight(w)
     _same(held.dequantize(), R.hold_weight(w))
     N, K = shape[-2:]
-    values, turned = held.values.float()[..., :K], held.transposed.float()[..., :N]
-    assert torch.equal(values.transpose(-1, -2).contiguous(), turned)
-    assert bool((held.values.float()[..., K:] == 0).all()) and bool((held.transposed.float()[..., N:] == 0).all())
+    assert held.values.shape[-2] == N and bool((held.values.float()[..., K:] == 0).all())
 
 
 def test_what_is_held_can_be_copied_and_saved(tmp_path):
@@ -96,13 +94,13 @@ def test_what_is_held_can_be_copied_and_saved(tmp_path):
     import fma_b200 as fma
 
     x, w = randn((9, 264), torch.bfloat16, 24).to(DEV), randn((2, 136, 264), torch.bfloat16, 25).to(DEV)
-    for held in (fma.quantize_fp8(x), fma.quantize_fp8_weight(w, transpose=True)):
+    for held in (fma.quantize_fp8(x), fma.quantize_fp8_weight(w)):
         torch.save(held, tmp_path / "held.pt")
         for other in (copy.deepcopy(held), torch.load(tmp_path / "held.pt", weights_only=False)):
             assert type(other) is type(held) and other.shape == held.shape and other.dtype == held.dtype
             assert other.device == held.device and torch.equal(other.dequantize(), held.dequantize())
     assert isinstance(held, fma.Fp8Weight) and isinstance(fma.quantize_fp8(x), fma.Fp8Blocks)
-    assert held.scales.data_ptr() != other.scales.data_ptr() and torch.equal(held.transposed_scales, other.transposed_scales)
+    assert held.scales.data_ptr() != other.scales.data_ptr() and torch.equal(held.scales, other.scales)
 
 
 def test_second_derivatives_are_refused():
@@ -145,7 +143,7 @@ def test_linear_gradients_one_at_a_time_and_kept_weights(rows):
     x, w = randn((2, rows // 2, 264), torch.bfloat16, 8).to(DEV), randn((136, 264), torch.bfloat16, 9, scale=0.05).to(DEV)
     d = randn((2, rows // 2, 136), torch.bfloat16, 10).to(DEV)
     (y, dx, dw), (sy, sx, sw) = R.linear(x.reshape(rows, 264), w, d.reshape(rows, 136))
-    held = fma.quantize_fp8_weight(w, transpose=True)
+    held = fma.quantize_fp8_weight(w)
     a = x.clone().requires_grad_()
     out = fma.linear_fp8(a, held)
     out.backward(d)
@@ -275,7 +273,7 @@ def test_grouped_counts_that_do_not_fit(dtype, rows):
     import fma_b200 as fma
 
     x, w = randn((rows, 128), torch.bfloat16, 17).to(DEV), randn((4, 64, 128), torch.bfloat16, 18).to(DEV)
-    held = fma.quantize_fp8_weight(w, transpose=True)
+    held = fma.quantize_fp8_weight(w)
     wild = [rows - 9, 20, 2**31 - 1, 5] if dtype != torch.uint32 else [rows - 9, 20, 2**30, 5]
     want = R.grouped(x, w, [rows - 9, 9, 0, 0], torch.zeros(rows, 64, device=DEV))
     got = fma.grouped_linear_fp8(x, held, torch.tensor(wild, dtype=dtype).to(DEV))
@@ -321,6 +319,27 @@ def test_swiglu(dtype, shape, halves):
         off = (got.double() - ref).abs()
         assert bool((off <= half * ref.abs() + (1 + half) * fp32 * grow * size + tiny).all())
     check_device_status()
+
+
+@pytest.mark.parametrize("N,K", [(8, 8), (200, 136), (136, 520), (392, 128)])
+def test_an_expert_without_a_number_stays_alone(N, K):
+    """Tiles and k-blocks that reach into the next expert's weights, and rows behind an expert's, spoil nothing."""
+    import fma_b200 as fma
+
+    counts = [70, 0, 33, 300]
+    x, w = randn((sum(counts), K), torch.bfloat16, 31).to(DEV), randn((4, N, K), torch.bfloat16, 32).to(DEV)
+    d_out = randn((sum(counts), N), torch.bfloat16, 33).to(DEV)
+    w[1], w[3] = float("nan"), float("inf")
+    x[70 + 33 + 5] = float("nan")
+    (y, dx, dw), (sy, sx, sw) = R.grouped(x, w, counts, d_out)
+    count = torch.tensor(counts, device=DEV)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = fma.grouped_linear_fp8(a, b, count)
+    out.backward(d_out)
+    R.check_product(out.detach()[:103], y[:103], sy[:103], K)
+    R.check_product(a.grad[:103], dx[:103], sx[:103], N)
+    R.check_product(b.grad[:3], dw[:3], sw[:3], 70)
+    assert bool(torch.isnan(out[103:]).all()) and bool(torch.isnan(a.grad[103:]).all())
 
 
 def test_many_experts():
@@ -473,7 +492,6 @@ def test_refusals():
     refused("CUDA", fma.grouped_linear_fp8, x, w3, count.cpu())
     refused("quantize_fp8_weight", fma.linear_fp8, x, w, w)
     refused("shape", fma.linear_fp8, x, w, fma.quantize_fp8_weight(w3))
-    refused("transpose=True", fma.linear_fp8, x.clone().requires_grad_(), fma.quantize_fp8_weight(w))
     refused("same shape", fma.swiglu_fp8_checkpoint, x, x[:2])
     refused("multiple of 8", fma.swiglu_fp8_checkpoint, x[:, :4], x[:, :4])
     refused("same shape, dtype", fma.swiglu_fp8_checkpoint, x, x.half())
