@@ -4,11 +4,14 @@
 //
 // The reduction of a tile is as long as its expert has rows, a few hundred for experts, so what a tile costs besides its
 // MMAs counts.  Hence 256 x 256 pair tiles with two accumulators that fill tensor memory: reading and storing a result
-// overlaps the next tile's main loop whole.  Ring stages of 128 rows make it eight MMAs per wait and commit, and the
-// whole issuing warp walks the loop (gemm_fp8.cu says what these two are worth).
-// Measured, bfloat16: 128 experts of 1536 x 2048 with 512 rows each on average 352 us
-// (417 with the 256 x 512 tiles of gemm_tc2.cu, whose single accumulator waits for its epilogue), 14336 x 4096 over 8192 rows 631 us, 1.53 PFLOP/s (651 there; the
-// library takes 608).  What bounds it now is the tensor pipe, and with short reductions the last wave.
+// overlaps the next tile's main loop whole.  Ring stages of 128 rows make it eight MMAs per commit, and the whole issuing
+// warp walks the loop (gemm_fp8.cu says what these two are worth); the MMAs start when half a stage has landed (experts of
+// 256 / 1024 rows 231 / 619 -> 225 / 606 us).  Results leave through the copy engine, in boxes of 32 rows x 64 columns that
+// end with their expert (128 rows per expert, where writing the result is most of the work: 195 us with stores from
+// registers, 175 so).
+// Measured, bfloat16: 128 experts of 1536 x 2048 with 512 rows each on average 348 us (417 with the 256 x 512 tiles of
+// gemm_tc2.cu, whose single accumulator waits for its epilogue), 14336 x 4096 over 8192 rows 631 us, 1.53 PFLOP/s (651
+// there; the library takes 608).  What bounds it now is the tensor pipe, and with short reductions writing the result.
 #include "fp8.cuh"
 #include "gemm_pair.cuh"
 
@@ -20,13 +23,12 @@ constexpr int WG_STAGE_BYTES = 4 * WG_SLAB;             // both operands, two ha
 constexpr int WG_STAGES = 3;
 constexpr int WG_EPI_WARPS = 8;
 constexpr int WG_THREADS = 32 * (2 + WG_EPI_WARPS);
-constexpr int WG_PATCH_BYTES = 32 * 64;
+constexpr int WG_PATCH_BYTES = 32 * 128;             // 32 rows x 64 columns of the result per epilogue warp
 constexpr size_t WG_SMEM = static_cast<size_t>(WG_STAGES) * WG_STAGE_BYTES + WG_EPI_WARPS * WG_PATCH_BYTES + 1024;
 constexpr int WG_SUPER = 8;                             // tiles along OUT walked together (operand reuse in L2)
 
 struct WgradParams {
-    CUtensorMap map_a, map_b;
-    void* out;
+    CUtensorMap map_a, map_b, map_out;
     const int32_t* offsets;  // [E + 1] first row of each expert; null: one expert, all rows
     const int32_t* counts;   // rows to reduce over per expert; null: up to the next offset
     int32_t* status;
@@ -68,9 +70,24 @@ __device__ __forceinline__ void tc_mma_pair_elected(uint32_t d, uint64_t a, uint
         : "memory");
 }
 
+// The result [E, OUT, IN]: boxes of 32 rows x 64 columns that end with their expert, 128-byte swizzle.
+static int encode_result(CUtensorMap* map, void* base, uint64_t E, uint64_t OUT, uint64_t IN, bool f16) {
+    EncodeTiledFn fn = encode_fn();
+    FMAB_REQUIRE(fn != nullptr, FMA_B200_ERR_LAUNCH, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[3] = {IN, OUT, E};
+    const cuuint64_t strides[2] = {IN * 2, OUT * IN * 2};
+    const cuuint32_t box[3] = {64, 32, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    FMAB_REQUIRE(r == CUDA_SUCCESS, FMA_B200_ERR_LAUNCH, "cuTensorMapEncodeTiled (weight gradient) failed with CUresult %d", (int)r);
+    return FMA_B200_OK;
+}
+
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linear_wgrad_kernel(const __grid_constant__ WgradParams p) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[WG_STAGES];   // used in the leader only
+    __shared__ __align__(8) uint64_t full_bar[WG_STAGES][2];  // per half of 64 rows; used in the leader only
     __shared__ __align__(8) uint64_t empty_bar[WG_STAGES];  // each CTA waits on its own copy
     __shared__ __align__(8) uint64_t acc_full_bar[2];       // each CTA waits on its own copy
     __shared__ __align__(8) uint64_t acc_empty_bar[2];      // used in the leader only
@@ -86,7 +103,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < WG_STAGES; ++s) {
-            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&full_bar[s][0]), 1);
+            mbar_init(smem_u32(&full_bar[s][1]), 1);
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -128,10 +146,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
                         break;
                     }
                     const int n_halves = min(2, t.halves - h0);
-                    const uint32_t leader_bar = map_to_rank(smem_u32(&full_bar[stage]), 0);
                     const uint32_t sa = ring + stage * WG_STAGE_BYTES, sb = sa + 2 * WG_SLAB;
-                    if (leader) mbar_arrive_expect_tx(smem_u32(&full_bar[stage]), 2 * n_halves * 2 * WG_SLAB);
                     for (int h = 0; h < n_halves; ++h) {
+                        const uint32_t leader_bar = map_to_rank(smem_u32(&full_bar[stage][h]), 0);
+                        if (leader) mbar_arrive_expect_tx(smem_u32(&full_bar[stage][h]), 2 * 2 * WG_SLAB);
                         const int row = t.row0 + (h0 + h) * WG_HALF_ROWS;
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
@@ -156,7 +174,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
             const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (1u << 16) |
                                    (static_cast<uint32_t>(256 >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
             int stage = 0;
-            uint32_t phase = 0;
+            uint32_t phases[2] = {0, 0};  // of the halves' barriers, a bit per stage
             uint32_t n_done = 0;  // tiles with MMAs so far: accumulator n_done % 2
             bool alive = true;
             for (int tile = pair_id; tile < total_tiles && alive; tile += n_pairs) {
@@ -165,17 +183,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
                 if (n_done >= 2 && !mbar_wait(smem_u32(&acc_empty_bar[n_done & 1u]), ((n_done >> 1) - 1) & 1u, abort_ptr, p.status)) break;
                 tc_fence_after();
                 const uint32_t acc = tmem_base + (n_done & 1u) * 256;
-                for (int h0 = 0; h0 < t.halves; h0 += 2) {
-                    if (!mbar_wait(smem_u32(&full_bar[stage]), phase, abort_ptr, p.status)) {
-                        alive = false;
-                        break;
-                    }
-                    tc_fence_after();
+                for (int h0 = 0; h0 < t.halves && alive; h0 += 2) {
                     const uint32_t sa = ring + stage * WG_STAGE_BYTES;
                     const uint64_t a_desc = make_smem_desc<true>(sa), b_desc = make_smem_desc<true>(sa + 2 * WG_SLAB);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if (h0 + h >= t.halves) continue;
+                        if (h0 + h >= t.halves || !alive) continue;
+                        alive = mbar_wait(smem_u32(&full_bar[stage][h]), (phases[h] >> stage) & 1u, abort_ptr, p.status);
+                        if (!alive) continue;
+                        phases[h] ^= 1u << stage;
+                        tc_fence_after();
 #pragma unroll
                         for (int ks = 0; ks < WG_HALF_ROWS / UMMA_K; ++ks) {
                             const uint32_t at = (h * WG_SLAB + ks * desc_k_step<true>()) / 16;
@@ -183,10 +200,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
                         }
                     }
                     tc_commit_both(smem_u32(&empty_bar[stage]));
-                    if (++stage == WG_STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                    if (++stage == WG_STAGES) stage = 0;
                 }
                 // published last: once the epilogues have seen it no other signal of the tile is outstanding
                 if (alive) tc_commit_both(smem_u32(&acc_full_bar[n_done & 1u]));
@@ -199,7 +213,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
         const int half = (warp - 2) >> 2;  // columns 0-127 or 128-255 of the tile
         const uint32_t patch = patches + (warp - 2) * WG_PATCH_BYTES;
         const bool f16 = p.f16 != 0;
-        uint16_t* const out = static_cast<uint16_t*>(p.out);
         uint32_t n_done = 0;
         for (int tile = pair_id; tile < total_tiles; tile += n_pairs) {
             const WgradTile t = wgrad_decode(p, tile);
@@ -209,9 +222,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
                 tc_fence_after();
             }
             const int first_row = t.m0 + static_cast<int>(rank) * 128 + quad * 32;
-            const int64_t base = static_cast<int64_t>(t.expert) * p.OUT + first_row;
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 4; ++i) {  // 32 columns each; two make a box
                 const int c0 = half * 128 + i * 32;
                 float v[32];
                 if (t.halves > 0) {
@@ -225,21 +237,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = 0.f;
                 }
-                // through the patch: 32 rows x 64 bytes, written a row per lane, read four lanes to a row
-                __syncwarp();
+                if ((i & 1) == 0) {
+                    if (lane == 0) bulk_wait_read_all();  // the previous box has left the patch
+                    __syncwarp();
+                }
 #pragma unroll
-                for (int q = 0; q < 4; ++q) st_shared_16(patch + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4), pack8(v + 8 * q, f16));
-                __syncwarp();
-                const int col = t.n0 + c0 + (lane & 3) * 8;
-#pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    const int row = it * 8 + (lane >> 2);
-                    const uint4 w = ld_shared_16(patch + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
-                    if (first_row + row < p.OUT && col < p.IN) st_global_16(out + (base + row) * p.IN + col, w);
+                for (int q = 0; q < 4; ++q) st_shared_16(patch_addr(patch, lane, (i & 1) * 4 + q), pack8(v + 8 * q, f16));
+                if ((i & 1) == 1) {
+                    fence_smem_to_async();
+                    __syncwarp();
+                    const int col = t.n0 + c0 - 32;
+                    if (lane == 0 && first_row < p.OUT && col < p.IN) {
+                        tma_store_3d(&p.map_out, patch, col, first_row, t.expert);
+                        bulk_commit();
+                    }
                 }
             }
             if (t.halves > 0) ++n_done;
         }
+        if (lane == 0) bulk_wait_all();
     }
 
     __syncwarp();
@@ -273,7 +289,7 @@ int fma_b200_linear_wgrad(const void* dY, const void* X, void* dW, int32_t dtype
     p.f16 = dtype == FMA_B200_F16 ? 1 : 0;
     if (int rc = encode_2d(&p.map_a, dY, OUT, rows, OUT, 64, WG_HALF_ROWS, p.f16 != 0)) return rc;
     if (int rc = encode_2d(&p.map_b, X, IN, rows, IN, 64, WG_HALF_ROWS, p.f16 != 0)) return rc;
-    p.out = dW;
+    if (int rc = encode_result(&p.map_out, dW, E, OUT, IN, p.f16 != 0)) return rc;
     p.offsets = seg_offsets;
     p.counts = seg_rows;
     p.rows = rows;
