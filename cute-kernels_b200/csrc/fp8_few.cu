@@ -122,8 +122,6 @@ __global__ void __launch_bounds__(kFewThreads, 3) few_rows_kernel(const __grid_c
     const int item = blockIdx.x / p.split;
     const int chunk = item / p.tiles, n0 = (item - chunk * p.tiles) * 128;
     int expert, row0, rows;
-    allow_next();
-    wait_for_previous();
     if (!few_locate(p, chunk, expert, row0, rows)) return;  // the whole cluster
     T* const out = static_cast<T*>(p.out) + static_cast<int64_t>(row0) * p.N + n0;
     if (expert < 0) {
@@ -327,8 +325,6 @@ __global__ void __launch_bounds__(kSomeThreads) some_rows_kernel(const __grid_co
     const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
     const int item = blockIdx.x / p.split;
     const int x_tile = item / p.tiles, tile = item - x_tile * p.tiles, n0 = tile * 128;
-    allow_next();
-    wait_for_previous();
     if (p.rows_used != nullptr && static_cast<int64_t>(x_tile) * 128 >= __ldg(p.rows_used)) return;  // the whole cluster
     const int expert = p.tile_expert != nullptr ? __ldg(p.tile_expert + x_tile) : 0;
     const int64_t out_row = p.tile_row != nullptr ? __ldg(p.tile_row + x_tile) : static_cast<int64_t>(x_tile) * 128;
@@ -522,7 +518,7 @@ static int allow_smem(Kernel kernel) {
 template <typename T>
 static int launch_few(const FewRows& p, int64_t items, cudaStream_t s) {
     if (int rc = allow_smem(few_rows_kernel<T>)) return rc;
-    return launch_chained("fp8_few_rows", few_rows_kernel<T>, dim3(static_cast<unsigned>(items * p.split)), kFewThreads,
+    return launch_kernel("fp8_few_rows", few_rows_kernel<T>, dim3(static_cast<unsigned>(items * p.split)), kFewThreads,
                           static_cast<size_t>(few_smem(p.quads_most)), static_cast<unsigned>(p.split), s, p);
 }
 
@@ -530,7 +526,7 @@ template <typename T>
 static int launch_some(const SomeRows& p, int64_t items, cudaStream_t s) {
     if (int rc = allow_smem(some_rows_kernel<T>)) return rc;
     const size_t smem = static_cast<size_t>(p.stages) * (kFewStageBytes + p.cols_most * FP8_BLOCK) + 1024;
-    return launch_chained("fp8_some_rows", some_rows_kernel<T>, dim3(static_cast<unsigned>(items * p.split)), kSomeThreads, smem,
+    return launch_kernel("fp8_some_rows", some_rows_kernel<T>, dim3(static_cast<unsigned>(items * p.split)), kSomeThreads, smem,
                           static_cast<unsigned>(p.split), s, p);
 }
 

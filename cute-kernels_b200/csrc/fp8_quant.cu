@@ -91,8 +91,6 @@ __device__ void zero_padding_rows(const QuantRows& p, uint32_t warp_id, uint32_t
 template <typename T, int TO>
 __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRows p) {
     constexpr int N = LaneBlock<T>::N, AHEAD = kAhead<T>;
-    allow_next();
-    wait_for_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     if (TO != TO_ROWS && blockIdx.x >= p.row_blocks) {
         zero_padding_rows<T, TO>(p, (blockIdx.x - p.row_blocks) * kQWarps + warp, (gridDim.x - p.row_blocks) * kQWarps);
@@ -160,8 +158,6 @@ struct QuantWeight {
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_weight_kernel(const QuantWeight p) {
     __shared__ uint32_t warp_max[8];
-    allow_next();
-    wait_for_previous();
     constexpr int V = Elem<T>::kPerVec;
     const int tid = threadIdx.x;
     const int kb = blockIdx.x % p.k_blocks;
@@ -246,8 +242,6 @@ struct Dequant {
 
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) dequantize_rows_kernel(const Dequant p) {
-    allow_next();
-    wait_for_previous();
     constexpr int AHEAD = 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
@@ -358,8 +352,6 @@ __device__ __forceinline__ void store_lane_raw(const uint4* raw, void* base, int
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) swiglu_fp8_forward_kernel(const SwigluFp8 p) {
     constexpr int N = LaneBlock<T>::N, V = LaneBlock<T>::V;
-    allow_next();
-    wait_for_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
     const int64_t units = rows * p.blocks;
@@ -388,8 +380,6 @@ __global__ void __launch_bounds__(kQThreads) swiglu_fp8_forward_kernel(const Swi
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) swiglu_fp8_backward_kernel(const SwigluFp8 p) {
     constexpr int N = LaneBlock<T>::N, V = LaneBlock<T>::V;
-    allow_next();
-    wait_for_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
     const int64_t units = rows * p.blocks;
@@ -443,8 +433,6 @@ struct GroupMaps {
 __global__ void __launch_bounds__(kMapThreads) group_maps_kernel(const GroupMaps p) {
     __shared__ int32_t off[1024 + 2], pad[1024 + 3];
     __shared__ long long scan[kMapThreads];
-    allow_next();
-    wait_for_previous();
     const int t = threadIdx.x;
     long long c = 0;
     if (t < p.E) {
@@ -547,7 +535,7 @@ static int launch_quantize(QuantRows& p, int32_t dtype, int64_t extra_rows, cuda
     const uint32_t grid = p.row_blocks + (TO != TO_ROWS ? row_grid(extra_rows) : 0);
     int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        rc = launch_chained("fp8_quantize", quantize_rows_kernel<decltype(tag), TO>, dim3(grid), kQThreads, 0, 0, s, p);
+        rc = launch_kernel("fp8_quantize", quantize_rows_kernel<decltype(tag), TO>, dim3(grid), kQThreads, 0, 0, s, p);
     });
     return rc;
 }
@@ -651,7 +639,7 @@ int fma_b200_fp8_quantize_weight(const void* w, int32_t dtype, int32_t E, int32_
     const dim3 grid(static_cast<unsigned>(p.n_blocks * p.k_blocks), static_cast<unsigned>(E));
     int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        rc = launch_chained("fp8_quantize_weight", quantize_weight_kernel<decltype(tag)>, grid, 256, 0, 0,
+        rc = launch_kernel("fp8_quantize_weight", quantize_weight_kernel<decltype(tag)>, grid, 256, 0, 0,
                             static_cast<cudaStream_t>(stream), p);
     });
     return rc;
@@ -680,7 +668,7 @@ int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batc
     if (int rc = make_items(p.work, p.rows, cols, 8)) return rc;
     int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        rc = launch_chained("fp8_dequantize", dequantize_rows_kernel<decltype(tag)>, dim3(row_grid(p.work.items)), kQThreads, 0, 0,
+        rc = launch_kernel("fp8_dequantize", dequantize_rows_kernel<decltype(tag)>, dim3(row_grid(p.work.items)), kQThreads, 0, 0,
                             static_cast<cudaStream_t>(stream), p);
     });
     return rc;
@@ -709,7 +697,7 @@ int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, 
     p.tile_expert = tile_expert;
     p.tile_row = tile_row;
     p.tile_rows = tile_rows;
-    return launch_chained("fp8_group_maps", group_maps_kernel, dim3(1), kMapThreads, 0, 0, static_cast<cudaStream_t>(stream), p);
+    return launch_kernel("fp8_group_maps", group_maps_kernel, dim3(1), kMapThreads, 0, 0, static_cast<cudaStream_t>(stream), p);
 }
 
 int fma_b200_swiglu_fp8_forward(const void* gate, int64_t gate_pitch, const void* up, int64_t up_pitch, void* out,
@@ -751,7 +739,7 @@ int fma_b200_swiglu_fp8_forward(const void* gate, int64_t gate_pitch, const void
     p.blocks = static_cast<int32_t>((cols + FP8_BLOCK - 1) / FP8_BLOCK);
     int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        rc = launch_chained("swiglu_fp8_forward", swiglu_fp8_forward_kernel<decltype(tag)>, dim3(row_grid((rows * p.blocks + 3) / 4)), kQThreads, 0, 0,
+        rc = launch_kernel("swiglu_fp8_forward", swiglu_fp8_forward_kernel<decltype(tag)>, dim3(row_grid((rows * p.blocks + 3) / 4)), kQThreads, 0, 0,
                             static_cast<cudaStream_t>(stream), p);
     });
     return rc;
@@ -795,7 +783,7 @@ int fma_b200_swiglu_fp8_backward(const void* gate8, const void* gate_scales, con
     p.blocks = static_cast<int32_t>((cols + FP8_BLOCK - 1) / FP8_BLOCK);
     int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        rc = launch_chained("swiglu_fp8_backward", swiglu_fp8_backward_kernel<decltype(tag)>, dim3(row_grid((rows * p.blocks + 3) / 4)), kQThreads, 0, 0,
+        rc = launch_kernel("swiglu_fp8_backward", swiglu_fp8_backward_kernel<decltype(tag)>, dim3(row_grid((rows * p.blocks + 3) / 4)), kQThreads, 0, 0,
                             static_cast<cudaStream_t>(stream), p);
     });
     return rc;

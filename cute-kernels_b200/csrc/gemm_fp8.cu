@@ -199,8 +199,6 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
     __syncthreads();
     cluster_sync_all();  // the peer's barriers exist before anything is signalled across CTAs
     tc_fence_after();
-    allow_next();
-    wait_for_previous();
     const uint32_t tmem_base = tmem_slot;
     volatile int* abort_ptr = &abort_flag;
 
@@ -492,7 +490,7 @@ static int launch_fp8(GemmFp8Params& p, cudaStream_t s) {
     FMAB_REQUIRE(total < (1LL << 31), FMA_B200_ERR_BAD_ARG, "too many tiles");
     const int64_t max_pairs = sm_count() >= 2 ? sm_count() / 2 : 1;
     const int pairs = static_cast<int>(total < max_pairs ? total : max_pairs);
-    return launch_chained("8-bit grouped GEMM", gemm_fp8_kernel<TURNED>, dim3(2 * pairs), F8_THREADS, F8_SMEM, 0, s, p);
+    return launch_kernel("8-bit grouped GEMM", gemm_fp8_kernel<TURNED>, dim3(2 * pairs), F8_THREADS, F8_SMEM, 0, s, p);
 }
 
 template <bool TURNED>

@@ -124,8 +124,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
     __syncthreads();
     cluster_sync_all();  // the peer's barriers exist before anything is signalled across CTAs
     tc_fence_after();
-    allow_next();
-    wait_for_previous();
     const uint32_t tmem_base = tmem_slot;
     volatile int* abort_ptr = &abort_flag;
     const int total_tiles = p.E * p.m_tiles * p.n_tiles;
@@ -309,7 +307,7 @@ int fma_b200_linear_wgrad(const void* dY, const void* X, void* dW, int32_t dtype
     }
     const int64_t max_pairs = sm_count() >= 2 ? sm_count() / 2 : 1;
     const int pairs = static_cast<int>(total < max_pairs ? total : max_pairs);
-    return launch_chained("linear weight gradient", linear_wgrad_kernel, dim3(2 * pairs), WG_THREADS, WG_SMEM, 0,
+    return launch_kernel("linear weight gradient", linear_wgrad_kernel, dim3(2 * pairs), WG_THREADS, WG_SMEM, 0,
                           static_cast<cudaStream_t>(stream), p);
 }
 
