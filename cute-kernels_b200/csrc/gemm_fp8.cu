@@ -81,6 +81,8 @@ struct GemmFp8Params {
     const int32_t* tile_row;     // per 128 rows of a: first output row; null: the same row
     const int32_t* tile_rows;    // per 128 rows of a: output rows; null: up to out_rows
     const int32_t* rows_used;    // rows of the layout in use (device); null: layout_rows
+    const int32_t* row_offsets;  // first row and number of rows of each expert in the layout, instead of tile_row and
+    const int32_t* row_counts;   // tile_rows: rows up to a multiple of 64 are computed; null: not known
     int32_t* status;
     int64_t out_rows;
     int64_t layout_rows;
@@ -127,11 +129,13 @@ struct F8PairTile {
     int64_t out_row; // and the first of them
 };
 
-__device__ __forceinline__ void f8_rows(const GemmFp8Params& p, int32_t a_row, int half, int64_t& out_row, int32_t& rows) {
+__device__ __forceinline__ void f8_rows(const GemmFp8Params& p, int32_t expert, int32_t a_row, int half, int64_t& out_row, int32_t& rows) {
     const int mt = a_row / 128 + half;  // used where tiles start at multiples of 256
     out_row = p.tile_row != nullptr ? __ldg(p.tile_row + mt) : a_row + 128LL * half;
     const int64_t most = min(128, p.tile_rows_most - 128 * half);
-    const int64_t left = p.tile_rows != nullptr ? __ldg(p.tile_rows + mt) : p.out_rows - out_row;
+    int64_t left = p.tile_rows != nullptr ? __ldg(p.tile_rows + mt) : p.out_rows - out_row;
+    if (p.row_counts != nullptr && expert >= 0)
+        left = min(left, __ldg(p.row_offsets + expert) + (static_cast<int64_t>(__ldg(p.row_counts + expert)) + 63) / 64 * 64 - out_row);
     rows = static_cast<int32_t>(left < 0 || most < 0 ? 0 : (left > most ? most : left));
 }
 
@@ -149,8 +153,8 @@ __device__ __forceinline__ bool f8_decode(const GemmFp8Params& p, int tile, int 
     if (t.expert == -1) return false;
     int64_t other_row;
     int32_t other;
-    f8_rows(p, t.a_row, half, t.out_row, t.rows);
-    f8_rows(p, t.a_row, half ^ 1, other_row, other);
+    f8_rows(p, t.expert, t.a_row, half, t.out_row, t.rows);
+    f8_rows(p, t.expert, t.a_row, half ^ 1, other_row, other);
     const int32_t lower = half == 0 ? t.rows : other, upper = half == 0 ? other : t.rows;
     t.n = ((upper > 0 ? 128 + upper : lower) + 31) / 32 * 32;
     return t.n > 0;
@@ -496,7 +500,8 @@ static int launch_fp8(GemmFp8Params& p, cudaStream_t s) {
 template <bool TURNED>
 static int fp8_product(const void* a, const void* a_scales, int64_t layout_rows, const void* w, const void* w_scales, int32_t E, int32_t N,
                        int32_t K, void* out, int32_t dtype, int64_t out_rows, const int32_t* tile_expert, const int32_t* tile_row,
-                       const int32_t* tile_rows, const int32_t* rows_used, cudaStream_t s) {
+                       const int32_t* tile_rows, const int32_t* rows_used, const int32_t* row_offsets, const int32_t* row_counts,
+                       cudaStream_t s) {
     FMAB_REQUIRE(dtype == FMA_B200_BF16 || dtype == FMA_B200_F16, FMA_B200_ERR_UNSUPPORTED,
                  "dtype %d: the 8-bit product returns bfloat16 or half", dtype);
     FMAB_REQUIRE(layout_rows >= 0 && layout_rows < (1LL << 31) - 256 && out_rows >= 0, FMA_B200_ERR_BAD_ARG,
@@ -506,6 +511,8 @@ static int fp8_product(const void* a, const void* a_scales, int64_t layout_rows,
                  "N=%d and K=%d must be positive multiples of 8", N, K);
     FMAB_REQUIRE(static_cast<int64_t>(E) * (TURNED ? K : N) < (1LL << 31) - 1024, FMA_B200_ERR_BAD_ARG, "E*%s overflows", TURNED ? "K" : "N");
     FMAB_REQUIRE(E == 1 || tile_expert != nullptr, FMA_B200_ERR_BAD_ARG, "several experts need tile_expert");
+    FMAB_REQUIRE((row_offsets == nullptr) == (row_counts == nullptr) && !(row_counts && (tile_row || tile_rows || !tile_expert)),
+                 FMA_B200_ERR_BAD_ARG, "row_offsets and row_counts come together, beside tile_expert, without tile_row and tile_rows");
     if (layout_rows == 0 || out_rows == 0) return FMA_B200_OK;
     FMAB_REQUIRE(a && a_scales && w && w_scales && out, FMA_B200_ERR_BAD_ARG, "NULL pointer");
     FMAB_REQUIRE(aligned16(a) && aligned16(a_scales) && aligned16(w) && aligned16(w_scales) && aligned16(out),
@@ -522,6 +529,8 @@ static int fp8_product(const void* a, const void* a_scales, int64_t layout_rows,
     p.tile_row = tile_row;
     p.tile_rows = tile_rows;
     p.rows_used = rows_used;
+    p.row_offsets = row_offsets;
+    p.row_counts = row_counts;
     p.out_rows = out_rows;
     p.layout_rows = layout_rows;
     p.n_cols = N;
@@ -552,17 +561,17 @@ extern "C" {
 int fma_b200_fp8_gemm(const void* a, const void* a_scales, int64_t layout_rows, const void* w, const void* w_scales,
                       int32_t E, int32_t N, int32_t K, void* out, int32_t dtype, int64_t out_rows,
                       const int32_t* tile_expert, const int32_t* tile_row, const int32_t* tile_rows,
-                      const int32_t* rows_used, void* stream) {
+                      const int32_t* rows_used, const int32_t* row_offsets, const int32_t* row_counts, void* stream) {
     return fmab::fp8_product<false>(a, a_scales, layout_rows, w, w_scales, E, N, K, out, dtype, out_rows, tile_expert, tile_row, tile_rows,
-                                    rows_used, static_cast<cudaStream_t>(stream));
+                                    rows_used, row_offsets, row_counts, static_cast<cudaStream_t>(stream));
 }
 
 int fma_b200_fp8_gemm_dgrad(const void* dy, const void* dy_scales, int64_t layout_rows, const void* w, const void* w_scales,
                             int32_t E, int32_t N, int32_t K, void* dx, int32_t dtype, int64_t out_rows,
                             const int32_t* tile_expert, const int32_t* tile_row, const int32_t* tile_rows,
-                            const int32_t* rows_used, void* stream) {
+                            const int32_t* rows_used, const int32_t* row_offsets, const int32_t* row_counts, void* stream) {
     return fmab::fp8_product<true>(dy, dy_scales, layout_rows, w, w_scales, E, K, N, dx, dtype, out_rows, tile_expert, tile_row, tile_rows,
-                                   rows_used, static_cast<cudaStream_t>(stream));
+                                   rows_used, row_offsets, row_counts, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

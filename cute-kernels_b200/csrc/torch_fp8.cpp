@@ -211,7 +211,7 @@ Tensor product(const Held& a, const Weight& w, bool turned, at::ScalarType dtype
     check((turned ? fma_b200_fp8_gemm_dgrad : fma_b200_fp8_gemm)(
               a.values(), a.scales(), a.rows, w.values(), w.scales(), static_cast<int32_t>(w.E), static_cast<int32_t>(w.N), static_cast<int32_t>(w.K),
               out.data_ptr(), dtype_code(dtype), rows, m ? m->tile_expert() : nullptr, m ? m->tile_row() : nullptr,
-              m ? m->tile_rows() : nullptr, m ? m->used_all() : nullptr, stream_of(out)),
+              m ? m->tile_rows() : nullptr, m ? m->used_all() : nullptr, nullptr, nullptr, stream_of(out)),
           turned ? "fma_b200_fp8_gemm_dgrad" : "fma_b200_fp8_gemm");
     return out;
 }

@@ -90,11 +90,11 @@ SIGNATURES: dict[str, tuple] = {
     "fma_b200_fp8_group_maps": (ctypes.c_int, [_P, _I32, _I32, _I64, _I64, _P, _P, _P, _P, _P, _P, _P]),
     "fma_b200_fp8_gemm": (
         ctypes.c_int,
-        [_P, _P, _I64, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _P, _P],
+        [_P, _P, _I64, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _P, _P, _P, _P],
     ),
     "fma_b200_fp8_gemm_dgrad": (
         ctypes.c_int,
-        [_P, _P, _I64, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _P, _P],
+        [_P, _P, _I64, _P, _P, _I32, _I32, _I32, _P, _I32, _I64, _P, _P, _P, _P, _P, _P, _P],
     ),
     "fma_b200_fp8_few_rows": (ctypes.c_int, [_P, _I64, _I32, _I64, _P, _P, _I32, _I32, _I32, _P, _I32, _P, _P]),
     "fma_b200_swiglu_fp8_forward": (

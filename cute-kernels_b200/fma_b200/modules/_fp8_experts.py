@@ -65,13 +65,14 @@ def _used(maps: K.RowMaps) -> int:
 
 
 def _product(a: _Held, w_values: int, w_scales: int, cols: int, dtype, maps: K.RowMaps, dgrad: bool = False) -> torch.Tensor:
-    """a . w^T per expert, or with `dgrad` a . w; `cols` of the result."""
+    """a . w^T per expert, or with `dgrad` a . w; `cols` of the result.  Its rows behind an expert's are written up to a
+    multiple of 64 only, which is as far as anything reads them."""
     dev = a.buffer.device
     out = torch.empty(maps.rows_cap, cols, dtype=dtype, device=dev)
     name, N, K_ = ("fma_b200_fp8_gemm_dgrad", a.cols, cols) if dgrad else ("fma_b200_fp8_gemm", cols, a.cols)
     call(name, a.values, a.scales, maps.rows_cap, w_values, w_scales, maps.num_experts, N, K_,
          ptr(out), dtype_code(dtype), maps.rows_cap, ptr(maps.mtile_expert), None, None, _used(maps),
-         stream_ptr(dev))  # fmt: skip
+         ptr(maps.pad_offsets), ptr(maps.expert_count), stream_ptr(dev))  # fmt: skip
     return out
 
 

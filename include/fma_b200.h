@@ -461,12 +461,13 @@ int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, 
  * zeros.  rows_used (device, may be NULL): layout rows in use.  N and K are multiples of 8.  Runs on tiles of 256
  * weight rows x up to 256 rows of CTA pairs, or, with few rows and few such tiles, on tiles of 128 weight rows that
  * clusters share along K.  Where tile_rows is given, tiles are as high as their rows; rows of the layout that it leaves
- * out are not written.
+ * out are not written.  The same for row_offsets and row_counts (instead of tile_row and tile_rows: first layout row and
+ * number of rows of each expert), which computes whole 64 rows, the step of fma_b200_linear_wgrad.
  */
 int fma_b200_fp8_gemm(const void* a, const void* a_scales, int64_t layout_rows, const void* w, const void* w_scales,
                       int32_t E, int32_t N, int32_t K, void* out, int32_t dtype, int64_t out_rows,
                       const int32_t* tile_expert, const int32_t* tile_row, const int32_t* tile_rows,
-                      const int32_t* rows_used, void* stream);
+                      const int32_t* rows_used, const int32_t* row_offsets, const int32_t* row_counts, void* stream);
 /*
  * Its input gradient: dx[r, :] = dy[r, :] . w[e(r)] for 8-bit dy [layout_rows, N] and the same w [E, N, K]; dx has row
  * pitch K.  Always on the pair tiles, which read the weights as they lie.
@@ -474,7 +475,7 @@ int fma_b200_fp8_gemm(const void* a, const void* a_scales, int64_t layout_rows, 
 int fma_b200_fp8_gemm_dgrad(const void* dy, const void* dy_scales, int64_t layout_rows, const void* w, const void* w_scales,
                             int32_t E, int32_t N, int32_t K, void* dx, int32_t dtype, int64_t out_rows,
                             const int32_t* tile_expert, const int32_t* tile_row, const int32_t* tile_rows,
-                            const int32_t* rows_used, void* stream);
+                            const int32_t* rows_used, const int32_t* row_offsets, const int32_t* row_counts, void* stream);
 /*
  * The same product for a few rows, in one launch: x [rows, K] in bfloat16 or half is quantised on the way in; counts
  * [E] (4- or 8-byte integers on the device, NULL: one expert) consecutive rows per expert, rows behind the last

@@ -51,18 +51,22 @@ def test_entry_points_refuse_bad_arguments():
     assert m(at, 4, 1025, 100, 1 << 20, at, at, at, at, at, at, null) == BAD
     assert m(null, 4, 4, 100, 2048, at, at, at, at, at, at, null) == BAD
     p = lib.fma_b200_fp8_gemm
-    assert p(at, at, 256, at, at, 1, 16, 16, at, 0, 256, null, null, null, null, null) == UNSUPPORTED  # fp32 result
-    assert p(at, at, 256, at, at, 2, 16, 16, at, 1, 256, null, null, null, null, null) == BAD  # experts without a table
-    assert p(at, at, 256, at, at, 1, 12, 16, at, 1, 256, null, null, null, null, null) == BAD
-    assert p(at, at, 256, at, at, 1, 16, 20, at, 1, 256, null, null, null, null, null) == BAD
-    assert p(at, null, 256, at, at, 1, 16, 16, at, 1, 256, null, null, null, null, null) == BAD
-    assert p(null, null, 0, null, null, 1, 16, 16, null, 1, 0, null, null, null, null, null) == OK
+    assert p(at, at, 256, at, at, 1, 16, 16, at, 0, 256, null, null, null, null, null, null, null) == UNSUPPORTED  # fp32 result
+    assert p(at, at, 256, at, at, 2, 16, 16, at, 1, 256, null, null, null, null, null, null, null) == BAD  # experts without a table
+    assert p(at, at, 256, at, at, 1, 12, 16, at, 1, 256, null, null, null, null, null, null, null) == BAD
+    assert p(at, at, 256, at, at, 1, 16, 20, at, 1, 256, null, null, null, null, null, null, null) == BAD
+    assert p(at, null, 256, at, at, 1, 16, 16, at, 1, 256, null, null, null, null, null, null, null) == BAD
+    assert p(null, null, 0, null, null, 1, 16, 16, null, 1, 0, null, null, null, null, null, null, null) == OK
     g = lib.fma_b200_fp8_gemm_dgrad
-    assert g(at, at, 256, at, at, 1, 16, 16, at, 0, 256, null, null, null, null, null) == UNSUPPORTED  # fp32 result
-    assert g(at, at, 256, at, at, 2, 16, 16, at, 1, 256, null, null, null, null, null) == BAD  # experts without a table
-    assert g(at, at, 256, at, odd, 1, 16, 16, at, 1, 256, null, null, null, null, null) == BAD
-    assert g(at, at, 256, at, at, 1024, 1 << 22, 16, at, 1, 256, at, null, null, null, null) == BAD  # E * N
-    assert g(null, null, 0, null, null, 1, 16, 16, null, 1, 0, null, null, null, null, null) == OK
+    assert g(at, at, 256, at, at, 1, 16, 16, at, 0, 256, null, null, null, null, null, null, null) == UNSUPPORTED  # fp32 result
+    assert g(at, at, 256, at, at, 2, 16, 16, at, 1, 256, null, null, null, null, null, null, null) == BAD  # experts without a table
+    assert g(at, at, 256, at, odd, 1, 16, 16, at, 1, 256, null, null, null, null, null, null, null) == BAD
+    assert g(at, at, 256, at, at, 1024, 1 << 22, 16, at, 1, 256, at, null, null, null, null, null, null) == BAD  # E * N
+    assert g(null, null, 0, null, null, 1, 16, 16, null, 1, 0, null, null, null, null, null, null, null) == OK
+    for call in (p, g):
+        assert call(at, at, 256, at, at, 2, 16, 16, at, 1, 256, at, null, null, null, at, null, null) == BAD  # offsets without counts
+        assert call(at, at, 256, at, at, 2, 16, 16, at, 1, 256, at, at, at, null, at, at, null) == BAD  # both kinds
+        assert call(at, at, 256, at, at, 1, 16, 16, at, 1, 256, null, null, null, null, at, at, null) == BAD
     f = lib.fma_b200_fp8_few_rows
     assert f(at, 16, 0, 4, at, at, 1, 16, 16, null, 4, at, null) == UNSUPPORTED
     assert f(at, 8, 1, 4, at, at, 1, 16, 16, null, 4, at, null) == BAD
