@@ -185,9 +185,10 @@ __device__ __forceinline__ uint32_t max_magnitudes16(uint32_t m, const uint4& v)
 }
 // Four finite values, scaled, as e4m3 bytes.
 __device__ __forceinline__ uint32_t fp8_pack4_finite(const float* x, float inverse) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inverse, x[1] * inverse), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inverse, x[3] * inverse), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
+    const float2 by = make_float2(inverse, inverse);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(__fmul2_rn(make_float2(x[0], x[1]), by), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(__fmul2_rn(make_float2(x[2], x[3]), by), __NV_SATFINITE, __NV_E4M3);
+    return __byte_perm(lo, hi, 0x5410);
 }
 // The warp's scale word (all lanes) from each lane's scale byte.
 __device__ __forceinline__ uint32_t scale_word_of(uint32_t byte) {
