@@ -111,8 +111,29 @@ __device__ __forceinline__ uint32_t f8_instr_desc(int n, uint32_t scale_byte) {
     return (scale_byte << 4) | ((TURNED ? 1u : 0u) << 15) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(256 >> 4) << 24) |
            (scale_byte << 29);
 }
-__device__ __forceinline__ void st_shared_2(uint32_t addr, uint32_t v) {
-    asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
+// 32 tensor-memory lanes x 32 columns in the fragments of 8 x 8 matrices: v[16 h + 4 i ..] = (lane 16 h + l/4: columns
+// 8 i + 2 (l%4) and the next; lane 16 h + l/4 + 8: the same), l = lane of the warp.
+__device__ __forceinline__ void tc_load_32x32_fragments(uint32_t taddr, float* v) {
+    uint32_t u[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(taddr), "r"(taddr + (16u << 16))
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
+}
+// Four matrices of 8 x 8 values of 16 bits, turned: thread l holds of matrix m (word m) row l / 4, columns 2 (l % 4) and the
+// next; lane 8 m + c gives the address of the 16 bytes that column c becomes.
+__device__ __forceinline__ void st_matrix_turned(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared::cta.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ void tc_store_4(uint32_t taddr, uint4 v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
@@ -331,9 +352,9 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {
                 const int r0 = (backwards ? 3 - i : i) * 32;  // rows r0 .. r0 + 31 of this half
-                float v[32];                                  // one weight row, 32 rows of a
+                float v[32];                                  // 16 weight rows x 32 rows of a, and the next 16
                 if (t.expert >= 0) {
-                    if (half * 128 + r0 < t.n) tc_load_32(acc + half * 128 + r0, v);
+                    if (half * 128 + r0 < t.n) tc_load_32x32_fragments(acc + half * 128 + r0, v);
                     if (i == 0) {
                         tc_fence_before();
                         __syncwarp();
@@ -344,19 +365,17 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
                     for (int j = 0; j < 32; ++j) v[j] = 0.f;
                 }
                 if (r0 >= t.rows) continue;
-                // turned in the patch: 32 rows of a x 64 bytes, written a weight row per lane (two bytes, 32 lanes next to
-                // each other), read four lanes to a row of a
+                // turned on the way into the patch: 32 rows of a x 64 bytes, read four lanes to a row of a
                 __syncwarp();
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint4 w = pack8(v + 8 * q, f16);
-                    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int row = 8 * q + 2 * k;
-                        const uint32_t at = patch + row * 64 + (((lane >> 3) ^ k) << 4) + (lane & 7) * 2;
-                        st_shared_2(at, words[k]);
-                        st_shared_2(at + 64, words[k] >> 16);
+                    for (int q = 0; q < 4; q += 2) {
+                        // matrices: weight rows 16 h + 0-7 and 8-15, for rows of a 8 q .. 8 q + 7 and the next eight
+                        const float* m = v + 16 * h + 4 * q;
+                        const uint4 w = pack8(m, f16);
+                        const int row = 8 * q + ((lane >> 4) << 3) + (lane & 7), piece = 2 * h + ((lane >> 3) & 1);
+                        st_matrix_turned(patch + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4), w.x, w.y, w.z, w.w);
                     }
                 }
                 __syncwarp();
