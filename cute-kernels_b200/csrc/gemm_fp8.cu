@@ -33,7 +33,12 @@
 // padded to 256; 128 experts of 1536 x 2048 with 52 / 128 / 512 rows each on average took 104 / 108 / 201 us so and take
 // 94 / 100 / 193 now, 8 of 14336 x 4096 with 1024 rows 381 and 367; plain products are the same both ways.  A low tile
 // saves less than its MMAs: it loads 128 weight rows per CTA all the same, and a full one already loads near L2's rate.
-// The result lies in tensor memory a weight row per lane and is turned in shared memory on its way out.
+//
+// The result lies in tensor memory a weight row per lane.  It is read as fragments of 8 x 8 matrices, turned by the matrix
+// store into shared memory and leaves through the copy engine in boxes of 32 rows x 32 columns; only where an expert ends
+// inside a box the rows are stored one by one.  128 experts of 2048 x 768 (short sums, so the way out counts) with 512 / 2048
+// rows each: 150 / 487 us with two-byte stores into the patch, 135 / 437 with matrix stores, 128 / 415 with the copy engine;
+// 1536 x 2048 193 / 658 and 189 / 642.
 //
 // Two 256-column accumulators and the scales do not fit into the 512 columns of tensor memory, so the accumulators
 // overlap by 32 columns: the epilogue reads the overlap first and hands it back at once, and the next tile's main loop
@@ -60,8 +65,8 @@ constexpr int F8_X_BYTES = F8_TILE_ROWS / 2 * BK8;  // its half of the tile's ro
 constexpr int F8_STAGE_KB = 2;                    // k-blocks per ring stage
 constexpr int F8_STAGE_BYTES = F8_STAGE_KB * (F8_W_BYTES + F8_X_BYTES);
 constexpr int F8_STAGES = 3;
-constexpr int F8_PATCH_BYTES = 32 * 64;  // 32 rows of a x 32 weight rows, 16 bits, per epilogue warp
-constexpr size_t F8_SMEM = static_cast<size_t>(F8_STAGES) * F8_STAGE_BYTES + F8_EPI_WARPS * F8_PATCH_BYTES + 1024;
+constexpr int F8_PATCH_BYTES = 32 * 64;  // two per epilogue warp:  // 32 rows of a x 32 weight rows, 16 bits, per epilogue warp
+constexpr size_t F8_SMEM = static_cast<size_t>(F8_STAGES) * F8_STAGE_BYTES + 2 * F8_EPI_WARPS * F8_PATCH_BYTES + 1024;
 constexpr int F8_SUPER = 8;                       // tiles of rows of a walked together (operand reuse in L2)
 constexpr int F8_BOXES = 4;                       // rows of a come in boxes of 16, 32, 64 or 128
 // tensor memory: accumulator 0 in columns 0-255, accumulator 1 in 224-479, two scale buffers of 12 columns (weights 4,
@@ -74,6 +79,7 @@ constexpr int F8_SCALE_BUFFERS = 2;
 struct GemmFp8Params {
     CUtensorMap map_w;            // TURNED: [expert, reduction, columns], so that a box does not reach into the next expert
     CUtensorMap map_a[F8_BOXES];
+    CUtensorMap map_out;          // boxes of 32 rows x 32 columns
     const uint8_t* a_scales;
     const uint8_t* w_scales;
     void* out;
@@ -334,7 +340,7 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
         // ------------------------------ epilogue (both CTAs) ------------------------------
         const int quad = warp & 3;               // tensor-memory lanes this warp may read
         const int half = (warp - 2) >> 2;        // rows 0-127 or 128-255 of the tile
-        const uint32_t patch = patches + (warp - 2) * F8_PATCH_BYTES;
+        uint32_t n_chunks = 0;
         const bool f16 = p.f16 != 0;
         uint16_t* const out = static_cast<uint16_t*>(p.out);
         uint32_t n_done = 0;
@@ -366,6 +372,8 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
                 }
                 if (r0 >= t.rows) continue;
                 // turned on the way into the patch: 32 rows of a x 64 bytes, read four lanes to a row of a
+                const uint32_t patch = patches + (2 * (warp - 2) + (n_chunks++ & 1u)) * F8_PATCH_BYTES;
+                if (lane == 0) bulk_wait_read_but_one();  // what left from this patch has been read
                 __syncwarp();
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -378,16 +386,28 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
                         st_matrix_turned(patch + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4), w.x, w.y, w.z, w.w);
                     }
                 }
-                __syncwarp();
+                if (r0 + 32 <= t.rows) {
+                    fence_smem_to_async();
+                    __syncwarp();
+                    const int first = t.w0 + static_cast<int>(rank) * 128 + quad * 32;
+                    if (lane == 0) {
+                        if (first < p.n_cols) tma_store_3d(&p.map_out, patch, first, static_cast<int>(t.out_row) + r0, 0);
+                        bulk_commit();
+                    }
+                } else {  // a box would reach into the next expert's rows
+                    __syncwarp();
 #pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    const int row = it * 8 + (lane >> 2);
-                    const uint4 w = ld_shared_16(patch + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
-                    if (r0 + row < t.rows && col < p.n_cols) st_global_16(out + (t.out_row + r0 + row) * p.n_cols + col, w);
+                    for (int it = 0; it < 4; ++it) {
+                        const int row = it * 8 + (lane >> 2);
+                        const uint4 w = ld_shared_16(patch + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
+                        if (r0 + row < t.rows && col < p.n_cols) st_global_16(out + (t.out_row + r0 + row) * p.n_cols + col, w);
+                    }
+                    if (lane == 0) bulk_commit();  // an empty group, so that groups count the patches
                 }
             }
             if (t.expert >= 0) ++n_done;
         }
+        if (lane == 0) bulk_wait_all();
     } else {
         // ------------------------------ scales (both CTAs) ------------------------------
         // All four warps bring the same words, each into its 32 lanes: word j of lane l is row j * 32 + l.  The 128 weight
@@ -570,6 +590,7 @@ static int fp8_product(const void* a, const void* a_scales, int64_t layout_rows,
     } else {
         if (int rc = encode_bytes(&p.map_w, w, K, static_cast<uint64_t>(E) * N, fp8_pitch(K), 128)) return rc;
     }
+    if (int rc = encode_3d(&p.map_out, out, N, out_rows, 1, N, static_cast<uint64_t>(out_rows) * N, 32, 32, p.f16 != 0)) return rc;
     return launch_fp8<TURNED>(p, s);
 }
 
