@@ -104,12 +104,6 @@ __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRow
         p.work.decode(i, row, q0, q1);
         if (row >= rows) break;
         int64_t to = row;
-        if (TO == TO_GROUPS) {
-            if (row >= __ldg(p.offsets + p.n_groups)) break;  // from here on: rows of no expert
-            const int e = group_of_row(p.offsets, p.n_groups, static_cast<int32_t>(row));
-            to = __ldg(p.pad_offsets + e) + (row - __ldg(p.offsets + e));
-            if (to >= p.layout_rows) continue;
-        }
         const T* const src = static_cast<const T*>(p.x) + row * p.x_pitch;
         for (int qa = q0; qa < q1; qa += AHEAD) {
             uint4 raw[AHEAD][N];
@@ -120,6 +114,12 @@ __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRow
                     const int c = (qa + u) * FP8_QUAD + g * FP8_BLOCK + LaneBlock<T>::column(s, j);
                     raw[u][j] = qa + u < q1 && c < p.cols ? ld_stream_16(src + c) : make_uint4(0, 0, 0, 0);
                 }
+            if (TO == TO_GROUPS && qa == q0) {  // found while the loads are on their way
+                if (row >= __ldg(p.offsets + p.n_groups)) return;  // from here on: rows of no expert
+                const int e = group_of_row(p.offsets, p.n_groups, static_cast<int32_t>(row));
+                to = __ldg(p.pad_offsets + e) + (row - __ldg(p.offsets + e));
+                if (to >= p.layout_rows) break;
+            }
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const int q = qa + u, col0 = q * FP8_QUAD + g * FP8_BLOCK;

@@ -65,7 +65,7 @@ constexpr int F8_X_BYTES = F8_TILE_ROWS / 2 * BK8;  // its half of the tile's ro
 constexpr int F8_STAGE_KB = 2;                    // k-blocks per ring stage
 constexpr int F8_STAGE_BYTES = F8_STAGE_KB * (F8_W_BYTES + F8_X_BYTES);
 constexpr int F8_STAGES = 3;
-constexpr int F8_PATCH_BYTES = 32 * 64;  // two per epilogue warp:  // 32 rows of a x 32 weight rows, 16 bits, per epilogue warp
+constexpr int F8_PATCH_BYTES = 32 * 64;           // 32 rows of a x 32 weight rows, 16 bits; two per epilogue warp
 constexpr size_t F8_SMEM = static_cast<size_t>(F8_STAGES) * F8_STAGE_BYTES + 2 * F8_EPI_WARPS * F8_PATCH_BYTES + 1024;
 constexpr int F8_SUPER = 8;                       // tiles of rows of a walked together (operand reuse in L2)
 constexpr int F8_BOXES = 4;                       // rows of a come in boxes of 16, 32, 64 or 128

@@ -1,4 +1,4 @@
-// Pieces shared by the kernels that run on CTA pairs (gemm_tc2.cu, gemm_fp8.cu): cluster addressing, barriers across
+// Pieces shared by the kernels that run on CTA pairs (gemm_tc2.cu, gemm_fp8.cu, gemm_wgrad.cu): cluster addressing, barriers across
 // the pair, paired loads, MMAs and commits, and the epilogue's staging patch.
 #pragma once
 
