@@ -10,17 +10,25 @@ namespace fmab {
 constexpr int kQThreads = 256;
 constexpr int kQWarps = kQThreads / 32;
 
-// Work of the row kernels: an item is a row, or a part of one (`per_item` groups of 512 columns) where there are few
-// rows; a warp has the loads of AHEAD groups in flight before it touches the first.  (One group per item, the row found
-// by a 64-bit division each time, ran at 70 % of the copy rate.)
+// Work of the row kernels: blocks of 128 columns, row after row; 8 lanes have a block each, a warp four in a row, and the
+// loads of several such steps are in flight before the first is touched, one where there are few blocks.  With rows as the unit (four groups of 512 columns
+// in flight) widths that are no multiple of 2048 left lanes or loads idle: 65536 rows of 768 / 1536 / 2048 columns took 47 /
+// 59 / 71.7 us and take 32 / 55 / 70.7 (6.4 TB/s at 4096), back to 16 bits 41 / 56 / 69 and 32 / 54 / 69.
 struct RowItems {
-    uint32_t items, parts;  // items; parts of a row
-    int32_t quads, per_item;
-    __device__ __forceinline__ void decode(uint32_t i, int64_t& row, int& q0, int& q1) const {
-        const uint32_t r = parts == 1 ? i : i / parts;
-        row = r;
-        q0 = static_cast<int>(i - r * parts) * per_item;
-        q1 = min(quads, q0 + per_item);
+    uint32_t units, blocks;            // blocks in all, and in a row
+    uint32_t step_rows, step_blocks;   // four blocks further
+    int32_t ahead;                     // steps of a warp at a time: a template argument of the kernels
+};
+struct RowPlace {
+    uint32_t row, block;
+    __device__ __forceinline__ RowPlace(const RowItems& w, uint32_t unit) : row(unit / w.blocks), block(unit - row * w.blocks) {}
+    __device__ __forceinline__ void next(const RowItems& w) {
+        row += w.step_rows;
+        block += w.step_blocks;
+        if (block >= w.blocks) {
+            block -= w.blocks;
+            ++row;
+        }
     }
 };
 template <typename T>
@@ -63,7 +71,7 @@ template <typename T>
 __device__ __forceinline__ void zero_row(const QuantRows& p, int64_t row) {
     const int lane = threadIdx.x & 31;
     for (int c = lane * 16; c < p.pitch; c += 512) st_global_16(p.values + row * p.pitch + c, make_uint4(0, 0, 0, 0));
-    for (int q = lane; q < p.work.quads; q += 32)
+    for (int q = lane; q * 4 < static_cast<int>(p.work.blocks); q += 32)
         *reinterpret_cast<uint32_t*>(p.scales + fp8_scale_word(row, q, p.row_tiles)) = 0x01010101u * FP8_SCALE_ONE;
     if (p.copy != nullptr) {
         constexpr int V = Elem<T>::kPerVec;
@@ -89,58 +97,66 @@ __device__ void zero_padding_rows(const QuantRows& p, uint32_t warp_id, uint32_t
     }
 }
 
-template <typename T, int TO>
+template <typename T, int TO, int AHEAD>
 __global__ void __launch_bounds__(kQThreads) quantize_rows_kernel(const QuantRows p) {
-    constexpr int N = LaneBlock<T>::N, AHEAD = kAhead<T>;
+    constexpr int N = LaneBlock<T>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     if (TO != TO_ROWS && blockIdx.x >= p.row_blocks) {
         zero_padding_rows<T, TO>(p, (blockIdx.x - p.row_blocks) * kQWarps + warp, (gridDim.x - p.row_blocks) * kQWarps);
         return;
     }
     const int64_t rows = TO == TO_ROWS && p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
-    for (uint32_t i = blockIdx.x * kQWarps + warp; i < p.work.items; i += p.row_blocks * kQWarps) {
-        int64_t row;
-        int q0, q1;
-        p.work.decode(i, row, q0, q1);
-        if (row >= rows) break;
-        int64_t to = row;
-        const T* const src = static_cast<const T*>(p.x) + row * p.x_pitch;
-        for (int qa = q0; qa < q1; qa += AHEAD) {
-            uint4 raw[AHEAD][N];
+    const int64_t known = TO == TO_GROUPS ? min(rows, static_cast<int64_t>(__ldg(p.offsets + p.n_groups))) : rows;  // the others: no expert
+    const uint32_t n_warps = p.row_blocks * kQWarps;
+    for (uint64_t first = (blockIdx.x * kQWarps + warp) * 4ull * AHEAD; first < p.work.units; first += n_warps * 4ull * AHEAD) {
+        RowPlace at(p.work, static_cast<uint32_t>(first) + g);  // units stay below 2^32 by more than a step
+        uint32_t row[AHEAD], block[AHEAD];
+        uint4 raw[AHEAD][N];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
+        for (int u = 0; u < AHEAD; ++u) {
+            row[u] = at.row;
+            block[u] = at.block;
+            const T* const src = static_cast<const T*>(p.x) + at.row * p.x_pitch;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int c = static_cast<int>(at.block) * FP8_BLOCK + LaneBlock<T>::column(s, j);
+                raw[u][j] = row[u] < known && c < p.cols ? ld_stream_16(src + c) : make_uint4(0, 0, 0, 0);
+            }
+            at.next(p.work);
+        }
+        int64_t layout_row = -1;  // groups: lane s finds where row[s] goes, while the loads are on their way
+        if (TO == TO_GROUPS) {
+            uint32_t mine = row[0];
+#pragma unroll
+            for (int u = 1; u < AHEAD; ++u) mine = s == u ? row[u] : mine;
+            if (mine < known) {
+                const int e = group_of_row(p.offsets, p.n_groups, static_cast<int32_t>(mine));
+                layout_row = __ldg(p.pad_offsets + e) + (static_cast<int64_t>(mine) - __ldg(p.offsets + e));
+                if (layout_row >= p.layout_rows) layout_row = -1;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int col0 = static_cast<int>(block[u]) * FP8_BLOCK;
+            uint32_t w[4];
+            const uint32_t byte = quantize_lane_raw<T>(raw[u], w);
+            int64_t to = row[u];
+            if (TO == TO_GROUPS) to = __shfl_sync(0xffffffffu, layout_row, (lane & 24) | u);
+            if (row[u] >= known || to < 0) continue;
+            const int copies = TO == TO_SLOTS ? p.k : 1;
+            for (int j = 0; j < copies; ++j) {
+                if (TO == TO_SLOTS) {
+                    to = __ldg(p.row_of_slot + static_cast<int64_t>(row[u]) * p.k + j);
+                    if (to < 0 || to >= p.layout_rows) continue;
+                }
+                store_lane_bytes<T>(p.values + to * p.pitch, col0, p.pitch, s, w);
+                if (s == 0) p.scales[fp8_scale_word(to, block[u] >> 2, p.row_tiles) + (block[u] & 3)] = static_cast<uint8_t>(byte);
+            }
+            if (TO == TO_GROUPS && p.copy != nullptr) {
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    const int c = (qa + u) * FP8_QUAD + g * FP8_BLOCK + LaneBlock<T>::column(s, j);
-                    raw[u][j] = qa + u < q1 && c < p.cols ? ld_stream_16(src + c) : make_uint4(0, 0, 0, 0);
-                }
-            if (TO == TO_GROUPS && qa == q0) {  // found while the loads are on their way
-                if (row >= __ldg(p.offsets + p.n_groups)) return;  // from here on: rows of no expert
-                const int e = group_of_row(p.offsets, p.n_groups, static_cast<int32_t>(row));
-                to = __ldg(p.pad_offsets + e) + (row - __ldg(p.offsets + e));
-                if (to >= p.layout_rows) break;
-            }
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int q = qa + u, col0 = q * FP8_QUAD + g * FP8_BLOCK;
-                if (q >= q1) break;
-                uint32_t w[4];
-                const uint32_t word = scale_word_of(quantize_lane_raw<T>(raw[u], w));
-                const int copies = TO == TO_SLOTS ? p.k : 1;
-                for (int j = 0; j < copies; ++j) {
-                    if (TO == TO_SLOTS) {
-                        to = __ldg(p.row_of_slot + row * p.k + j);
-                        if (to < 0 || to >= p.layout_rows) continue;
-                    }
-                    store_lane_bytes<T>(p.values + to * p.pitch, col0, p.pitch, s, w);
-                    if (lane == 0) *reinterpret_cast<uint32_t*>(p.scales + fp8_scale_word(to, q, p.row_tiles)) = word;
-                }
-                if (TO == TO_GROUPS && p.copy != nullptr) {
-#pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        const int c = col0 + LaneBlock<T>::column(s, j);
-                        if (c < p.cols) st_global_16(static_cast<T*>(p.copy) + to * p.cols + c, raw[u][j]);
-                    }
+                    const int c = col0 + LaneBlock<T>::column(s, j);
+                    if (c < p.cols) st_global_16(static_cast<T*>(p.copy) + to * p.cols + c, raw[u][j]);
                 }
             }
         }
@@ -241,40 +257,40 @@ struct Dequant {
     int32_t batch, rows_per, tiles_per, cols, pitch;  // of one matrix of the batch
 };
 
-template <typename T>
+template <typename T, int AHEAD>
 __global__ void __launch_bounds__(kQThreads) dequantize_rows_kernel(const Dequant p) {
-    constexpr int AHEAD = 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, s = lane & 7, g = lane >> 3;
     const int64_t rows = p.rows_used != nullptr ? min(p.rows, static_cast<int64_t>(*p.rows_used)) : p.rows;
-    for (uint32_t i = blockIdx.x * kQWarps + warp; i < p.work.items; i += gridDim.x * kQWarps) {
-        int64_t row;
-        int q0, q1;
-        p.work.decode(i, row, q0, q1);
-        if (row >= rows) break;
-        int64_t scale_row = row;
-        if (p.batch > 1) {
-            const uint32_t b = static_cast<uint32_t>(row) / static_cast<uint32_t>(p.rows_per);
-            scale_row = static_cast<int64_t>(b) * p.tiles_per * FP8_TILE_ROWS + (row - static_cast<int64_t>(b) * p.rows_per);
+    for (uint64_t first = (blockIdx.x * kQWarps + warp) * 4ull * AHEAD; first < p.work.units; first += gridDim.x * kQWarps * 4ull * AHEAD) {
+        RowPlace at(p.work, static_cast<uint32_t>(first) + g);
+        uint32_t row[AHEAD], block[AHEAD], w[AHEAD][4];
+        uint8_t byte[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            row[u] = at.row;
+            block[u] = at.block;
+            byte[u] = FP8_SCALE_ONE;
+            if (row[u] < rows) {
+                int64_t scale_row = at.row;
+                if (p.batch > 1) {
+                    const uint32_t b = at.row / static_cast<uint32_t>(p.rows_per);
+                    scale_row = static_cast<int64_t>(b) * p.tiles_per * FP8_TILE_ROWS + (at.row - static_cast<int64_t>(b) * p.rows_per);
+                }
+                load_lane_bytes<T>(p.values + static_cast<int64_t>(at.row) * p.pitch, static_cast<int>(at.block) * FP8_BLOCK, p.pitch, s, w[u]);
+                byte[u] = p.scales[fp8_scale_word(scale_row, at.block >> 2, p.row_tiles) + (at.block & 3)];
+            }
+            at.next(p.work);
         }
-        for (int qa = q0; qa < q1; qa += AHEAD) {
-            uint32_t w[AHEAD][4], word[AHEAD];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                if (qa + u >= q1) break;
-                load_lane_bytes<T>(p.values + row * p.pitch, (qa + u) * FP8_QUAD + g * FP8_BLOCK, p.pitch, s, w[u]);
-                word[u] = *reinterpret_cast<const uint32_t*>(p.scales + fp8_scale_word(scale_row, qa + u, p.row_tiles));
-            }
+        for (int u = 0; u < AHEAD; ++u) {
+            if (row[u] >= rows) continue;
+            const float factor = fp8_factor(byte[u]);
+            float x[16];
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                if (qa + u >= q1) break;
-                const float factor = fp8_factor((word[u] >> (8 * g)) & 0xffu);
-                float x[16];
+            for (int j = 0; j < 4; ++j) fp8_unpack4(w[u][j], factor, x + 4 * j);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) fp8_unpack4(w[u][j], factor, x + 4 * j);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = finite_in<T>(x[j]);
-                store_lane_block<T>(static_cast<T*>(p.out) + row * p.cols, (qa + u) * FP8_QUAD + g * FP8_BLOCK, p.cols, s, x);
-            }
+            for (int j = 0; j < 16; ++j) x[j] = finite_in<T>(x[j]);
+            store_lane_block<T>(static_cast<T*>(p.out) + static_cast<int64_t>(row[u]) * p.cols, static_cast<int>(block[u]) * FP8_BLOCK, p.cols, s, x);
         }
     }
 }
@@ -547,17 +563,16 @@ static uint32_t row_grid(int64_t items) {
     const int64_t cap = static_cast<int64_t>(sm_count()) * 64;
     return static_cast<uint32_t>(want < 1 ? 1 : (want > cap ? cap : want));
 }
-// `most` groups of 512 columns per item at most; fewer where the rows alone would not give every SM 16 warps.
-static int make_items(RowItems& w, int64_t rows, int64_t cols, int most) {
-    w.quads = static_cast<int32_t>(fp8_quads(cols));
-    const int64_t warps = 16LL * sm_count();
-    w.per_item = w.quads < most ? w.quads : most;
-    while (w.per_item > 1 && rows * ((w.quads + w.per_item - 1) / w.per_item) < warps) w.per_item = (w.per_item + 1) / 2;
-    w.parts = static_cast<uint32_t>((w.quads + w.per_item - 1) / w.per_item);
-    const int64_t items = rows * w.parts;
-    FMAB_REQUIRE(items < (1LL << 32) - (1LL << 24), FMA_B200_ERR_BAD_ARG, "rows=%lld of %lld columns are too many", (long long)rows,
+static int make_items(RowItems& w, int64_t rows, int64_t cols, int32_t most) {
+    w.blocks = static_cast<uint32_t>((cols + FP8_BLOCK - 1) / FP8_BLOCK);
+    w.step_rows = 4 / w.blocks;
+    w.step_blocks = 4 % w.blocks;
+    const int64_t units = rows * w.blocks;
+    FMAB_REQUIRE(units < (1LL << 32) - (1LL << 10), FMA_B200_ERR_BAD_ARG, "rows=%lld of %lld columns are too many", (long long)rows,
                  (long long)cols);
-    w.items = static_cast<uint32_t>(items);
+    w.units = static_cast<uint32_t>(units);
+    w.ahead = most;
+    if (units < 16LL * sm_count() * 4 * most) w.ahead = 1;  // 16 warps on every SM come first
     return FMA_B200_OK;
 }
 
@@ -576,11 +591,13 @@ static int check_pitch(const char* what, int32_t dtype, int64_t pitch, int64_t c
 
 template <int TO>
 static int launch_quantize(QuantRows& p, int32_t dtype, int64_t extra_rows, cudaStream_t s) {
-    p.row_blocks = row_grid(p.work.items);
+    p.row_blocks = row_grid((p.work.units + 4LL * p.work.ahead - 1) / (4 * p.work.ahead));
     const uint32_t grid = p.row_blocks + (TO != TO_ROWS ? row_grid(extra_rows) : 0);
     int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        rc = launch_kernel("fp8_quantize", quantize_rows_kernel<decltype(tag), TO>, dim3(grid), kQThreads, 0, 0, s, p);
+        using T = decltype(tag);
+        rc = launch_kernel("fp8_quantize", p.work.ahead == 1 ? quantize_rows_kernel<T, TO, 1> : quantize_rows_kernel<T, TO, kAhead<T>>,
+                           dim3(grid), kQThreads, 0, 0, s, p);
     });
     return rc;
 }
@@ -598,7 +615,7 @@ static int fill_quantize(QuantRows& p, const void* x, int64_t x_pitch, int32_t d
     p.row_tiles = fp8_row_tiles(layout_rows);
     p.cols = static_cast<int32_t>(cols);
     p.pitch = static_cast<int32_t>(fp8_pitch(cols));
-    if (int rc = make_items(p.work, rows, cols, 8)) return rc;
+    if (int rc = make_items(p.work, rows, cols, dtype == FMA_B200_F32 ? kAhead<float> : kAhead<__nv_bfloat16>)) return rc;
     p.values = static_cast<uint8_t*>(values);
     p.scales = static_cast<uint8_t*>(scales);
     if (rows == 0) return FMA_B200_OK;
@@ -710,10 +727,11 @@ int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batc
     p.batch = batch;
     p.cols = static_cast<int32_t>(cols);
     p.pitch = static_cast<int32_t>(fp8_pitch(cols));
-    if (int rc = make_items(p.work, p.rows, cols, 8)) return rc;
+    if (int rc = make_items(p.work, p.rows, cols, 2)) return rc;
     int rc = FMA_B200_OK;
     dispatch_dtype(dtype, [&](auto tag) {
-        rc = launch_kernel("fp8_dequantize", dequantize_rows_kernel<decltype(tag)>, dim3(row_grid(p.work.items)), kQThreads, 0, 0,
+        rc = launch_kernel("fp8_dequantize", p.work.ahead == 1 ? dequantize_rows_kernel<decltype(tag), 1> : dequantize_rows_kernel<decltype(tag), 2>,
+                           dim3(row_grid((p.work.units + 4LL * p.work.ahead - 1) / (4 * p.work.ahead))), kQThreads, 0, 0,
                             static_cast<cudaStream_t>(stream), p);
     });
     return rc;
