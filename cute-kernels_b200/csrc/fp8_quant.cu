@@ -1,7 +1,7 @@
 // Kernels around the 8-bit format of fp8.cuh: quantising rows (plain, grouped by expert, or scattered to the expert
-// layout of the MoE layer), quantising weights, dequantising, and SwiGLU that keeps its
-// inputs in 8 bits for the backward pass.  All are bound by HBM traffic: one pass over the data, 128-bit reads, every
-// value read once and written once; the block maximum lives in registers between the two.
+// layout of the MoE layer), quantising weights, dequantising, and SwiGLU that keeps its inputs in 8 bits for the backward
+// pass.  All are bound by HBM traffic: one pass over the data, 128-bit reads, every value read once and written once; the
+// block maximum lives in registers between the two.
 #include "fp8.cuh"
 #include "gemm_tc.cuh"
 
@@ -11,9 +11,10 @@ constexpr int kQThreads = 256;
 constexpr int kQWarps = kQThreads / 32;
 
 // Work of the row kernels: blocks of 128 columns, row after row; 8 lanes have a block each, a warp four in a row, and the
-// loads of several such steps are in flight before the first is touched, one where there are few blocks.  With rows as the unit (four groups of 512 columns
-// in flight) widths that are no multiple of 2048 left lanes or loads idle: 65536 rows of 768 / 1536 / 2048 columns took 47 /
-// 59 / 71.7 us and take 32 / 55 / 70.7 (6.4 TB/s at 4096), back to 16 bits 41 / 56 / 69 and 32 / 54 / 69.
+// loads of several such steps are in flight before the first is touched, one where there are few blocks.  With rows as the
+// unit (four groups of 512 columns in flight) widths that are no multiple of 2048 left lanes or loads idle: 65536 rows of
+// 768 / 1536 / 2048 columns took 47 / 59 / 71.7 us and take 32 / 55 / 70.7 (4096: 131 us, 6.1 TB/s), back to 16 bits 41 / 56 /
+// 69 and 32 / 54 / 69.
 struct RowItems {
     uint32_t units, blocks;            // blocks in all, and in a row
     uint32_t step_rows, step_blocks;   // four blocks further

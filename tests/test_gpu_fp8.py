@@ -321,6 +321,27 @@ def test_swiglu(dtype, shape, halves):
     check_device_status()
 
 
+@pytest.mark.parametrize("rows", [40, 700])
+def test_grouped_rows_that_nothing_writes_are_not_read(rows):
+    import fma_b200 as fma
+
+    x, w = randn((rows, 264), torch.bfloat16, 34).to(DEV), randn((3, 136, 264), torch.bfloat16, 35).to(DEV)
+    d_out, count = randn((rows, 136), torch.bfloat16, 36).to(DEV), torch.tensor([rows // 2, 3, rows // 4], device=DEV)
+    results = []
+    for byte in (0, 0xFF):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        blocks = [torch.full((n,), byte, dtype=torch.uint8, device=DEV) for n in [1 << 26] * 2 + [1 << 20] * 32 + [1 << 13] * 128]
+        torch.cuda.synchronize()
+        del blocks
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        out = fma.grouped_linear_fp8(a, b, count)
+        out.backward(d_out)
+        results.append((out.detach(), a.grad, b.grad))
+    for one, other in zip(*results):
+        assert bool(torch.isfinite(one).all()) and torch.equal(one, other)
+
+
 @pytest.mark.parametrize("N,K", [(8, 8), (200, 136), (136, 520), (392, 128)])
 def test_an_expert_without_a_number_stays_alone(N, K):
     """Tiles and k-blocks that reach into the next expert's weights, and rows behind an expert's, spoil nothing."""

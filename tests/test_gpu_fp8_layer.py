@@ -62,6 +62,32 @@ def _chain(x, weights, selected, w_fc, w_proj, dy):
     return y, dx, d_weights, d_fc, d_proj
 
 
+def _fill_free_memory(byte):
+    """The allocator's free blocks, small ones and large ones, hold this byte."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    blocks = [torch.full((n,), byte, dtype=torch.uint8, device=DEV) for n in [1 << 28] * 2 + [1 << 20] * 64 + [1 << 13] * 256]
+    torch.cuda.synchronize()
+    del blocks
+
+
+@pytest.mark.parametrize("T,E,k,H,I", [(300, 4, 2, 264, 136), (2000, 5, 3, 256, 128)])
+def test_rows_that_nothing_writes_are_not_read(T, E, k, H, I):
+    """Padding rows of the grouped layout that stay as the allocator left them do not reach a result."""
+    moe = _layer(E, k, H, I, torch.bfloat16)
+    x, dy = randn((T, H), torch.bfloat16, 10).to(DEV), randn((T, H), torch.bfloat16, 11).to(DEV)
+    results = []
+    for byte in (0, 0xFF):  # zeros, and NaN in every type and scale
+        a = x.clone().requires_grad_()
+        moe.zero_grad(set_to_none=True)
+        _fill_free_memory(byte)
+        y, _ = moe(a)
+        y.backward(dy)
+        results.append([t.detach().clone() for t in (y, a.grad, moe.c_fc.weight.grad, moe.c_proj.weight.grad, moe.gate.weight.grad)])
+    for one, other in zip(*results):
+        assert bool(torch.isfinite(one).all()) and torch.equal(one, other)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,E,k,H,I", [(300, 4, 2, 264, 136), (37, 8, 3, 128, 256), (1, 4, 2, 136, 8), (700, 3, 1, 520, 392)])
 def test_layer(dtype, T, E, k, H, I):
