@@ -559,9 +559,11 @@ __global__ void __launch_bounds__(kMapThreads) group_maps_kernel(const GroupMaps
 }
 
 // ---- host side -------------------------------------------------------------------------------------
+// At most 32 blocks of 256 threads per SM, about six rounds of them: 16384 x 4096 to 8 bits and back 71.7 us (64: 73.5, 8:
+// 73.5), SwiGLU of 32781 x 1536 forward and backward 134 us (137, 144).
 static uint32_t row_grid(int64_t items) {
     const int64_t want = (items + kQWarps - 1) / kQWarps;
-    const int64_t cap = static_cast<int64_t>(sm_count()) * 64;
+    const int64_t cap = static_cast<int64_t>(sm_count()) * 32;
     return static_cast<uint32_t>(want < 1 ? 1 : (want > cap ? cap : want));
 }
 static int make_items(RowItems& w, int64_t rows, int64_t cols, int32_t most) {
