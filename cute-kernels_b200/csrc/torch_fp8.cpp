@@ -217,9 +217,15 @@ Tensor product(const Held& a, const Weight& w, bool turned, at::ScalarType dtype
 }
 
 // Whether the product that reads x itself, in one launch, is the faster way.  Above, x is quantised by a launch of its own.
-// Measured with weights of 4096 x 4096: 5.8 us against 7.4 for one row, 7.6 / 7.9 for 16, 12.0 / 8.7 for 32; of 14336 x 4096:
-// 13.8 / 16.6, 17.9 / 17.4, 34.2 / 18.4; 128 experts of 1536 x 2048: 81 / 94 for 8 rows each, 101 / 95 for 16.
-bool few(int64_t rows, int64_t E, int64_t K) { return rows <= (E == 1 ? 16 : 12 * E) && K <= (1 << 16); }
+// Measured with weights of 4096 x 4096: 8.3 us against 9.7 for one row, 9.8 / 10.1 for 16, 12.1 / 10.5 for 24; of 14336 x 4096:
+// 14.7 / 19.3, 18.9 / 19.5, 31.1 / 19.6; 128 experts of 1536 x 2048: 83 / 90 for 8 rows each, 92 / 91 for 12, 102 / 93 for 16;
+// eight of 4096 x 4096: 36 / 40 for 4, 42 / 39 for 12.  Every tile of the weights quantises x again, which counts where there
+// are several experts with many tiles or long rows: eight of 4096 x 14336 86 / 102 for one row each, 106 / 103 for two, 127 /
+// 107 for eight; of 14336 x 4096 80 / 75, 92 / 86, 110 / 97.
+bool few(int64_t rows, int64_t E, int64_t N, int64_t K) {
+    if (K > (1 << 16)) return false;
+    return rows <= (E == 1 ? 16 : (N * K <= (1 << 25) ? 12 * E : E));
+}
 
 Tensor few_rows(const Tensor& x, const Weight& w, const Tensor& counts) {
     Tensor out = at::empty({x.size(0), w.N}, x.options());
@@ -341,7 +347,7 @@ Tensor linear(const char* name, const Tensor& x, const py::object& weight, const
     if (want_x || want_w) {
         using Maybe = std::optional<Tensor>;
         out = Linear::apply(x2, parameter.defined() ? Maybe(parameter) : Maybe(), held, grouped ? Maybe(counts) : Maybe(), want_x, want_w);
-    } else if (few(rows, held->E, K)) {
+    } else if (few(rows, held->E, N, K)) {
         out = few_rows(x2, *held, counts);
     } else {
         GroupMaps maps;
@@ -471,7 +477,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                                        t[5].cast<int64_t>()});
             }));
     for (const char* name : {"Fp8Blocks", "Fp8Weight"}) m.attr(name).attr("__module__") = "fma_b200";  // where pickle finds them
-    m.def("few", &few, "Whether this many rows take the one-launch product (rows, experts, width).");
+    m.def("few", &few, "Whether this many rows take the one-launch product (rows, experts, N, K).");
     m.def("quantize_fp8", &quantize_fp8);
     m.def("quantize_fp8_weight", &quantize_fp8_weight);
     m.def("linear_fp8", &linear_fp8);
