@@ -292,12 +292,11 @@ __global__ void __launch_bounds__(kFewThreads, 3) few_rows_kernel(const __grid_c
 }
 
 // ---- tiles of up to 128 rows, quantised before ------------------------------------------------------------
-// The same shape of product where experts have tens of rows (a batch in flight): 128 weight rows against a 128-row tile of
-// x, of which the 16, 32, 64 or 128 rows that cover its rows are the columns of the MMA and are streamed beside the
-// weights.  With few tiles a cluster shares each along the reduction.  Weights are still what moves: the 256 x 256 pair
-// tiles of gemm_fp8.cu would load as much of x as of w and cannot spread one tile over more than two SMs.  Quantising on
-// the way in would be repeated by every tile of weights (1 us per row of 4096 columns, measured), so it is a launch of
-// its own here.
+// The same shape of product for tens of rows, where the pair tiles of gemm_fp8.cu are too few for the GPU (its rule has
+// the figures): 128 weight rows against a 128-row tile of x, of which the 16, 32, 64 or 128 rows that cover its rows are the
+// columns of the MMA and are streamed beside the weights.  A cluster shares each tile along the reduction, which is what
+// pair tiles cannot do.  Weights are still what moves.  Quantising on the way in would be repeated by every tile of
+// weights (1 us per row of 4096 columns, measured), so it is a launch of its own here.
 constexpr int kSomeThreads = 192;
 constexpr int kSomeStagesMost = 5;
 constexpr int kSomeBoxes = 4;  // loads of 16, 32, 64, 128 rows of x
