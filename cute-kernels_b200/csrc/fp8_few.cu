@@ -208,10 +208,10 @@ __global__ void __launch_bounds__(kFewThreads, 3) few_rows_kernel(const __grid_c
             }
         }
     } else if (warp == 1) {
-        bool alive = mbar_wait(smem_u32(&scale_bar), 0, abort_ptr, p.status);
+        bool alive = mbar_wait_warp(smem_u32(&scale_bar), 0, abort_ptr, p.status);
         for (int kb = 0; kb < n_kb && alive; ++kb) {
             const int s = kb % kFewStages;
-            alive = mbar_wait(smem_u32(&full_bar[s]), (kb / kFewStages) & 1u, abort_ptr, p.status);
+            alive = mbar_wait_warp(smem_u32(&full_bar[s]), (kb / kFewStages) & 1u, abort_ptr, p.status);
             if (!alive) break;
             tc_fence_after();
             const uint32_t byte = kb & 3, scales = tmem + kFewScaleCol + (kb >> 2) * kFewScaleCols;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kFewThreads, 3) few_rows_kernel(const __grid_c
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&scale_bar));
-        if (mbar_wait(smem_u32(&acc_bar), 0, abort_ptr, p.status)) {
+        if (mbar_wait_warp(smem_u32(&acc_bar), 0, abort_ptr, p.status)) {
             tc_fence_after();
             uint32_t v[16];
             asm volatile(
@@ -379,10 +379,10 @@ __global__ void __launch_bounds__(kSomeThreads) some_rows_kernel(const __grid_co
             }
         }
     } else if (warp == 1) {
-        bool alive = mbar_wait(smem_u32(&scale_bar), 0, abort_ptr, p.status);
+        bool alive = mbar_wait_warp(smem_u32(&scale_bar), 0, abort_ptr, p.status);
         for (int kb = 0; kb < n_kb && alive; ++kb) {
             const int s = kb % p.stages;
-            alive = mbar_wait(smem_u32(&full_bar[s]), (kb / p.stages) & 1u, abort_ptr, p.status);
+            alive = mbar_wait_warp(smem_u32(&full_bar[s]), (kb / p.stages) & 1u, abort_ptr, p.status);
             if (!alive) break;
             tc_fence_after();
             const uint32_t byte = kb & 3, scales = tmem + p.cols_most + (kb >> 2) * kFewScaleCols;
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kSomeThreads) some_rows_kernel(const __grid_co
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&scale_bar));
-        if (mbar_wait(smem_u32(&acc_bar), 0, abort_ptr, p.status)) {
+        if (mbar_wait_warp(smem_u32(&acc_bar), 0, abort_ptr, p.status)) {
             tc_fence_after();
             float* const part = reinterpret_cast<float*>(base);  // [rows of x][128 weight rows], over the drained ring
             const int n = (warp & 3) * 32 + lane;

@@ -292,15 +292,15 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
                 F8PairTile t;
                 if (!f8_decode(p, tile, a_ntiles, 0, t) || t.expert < 0) continue;
                 // the epilogues have read the columns that this accumulator shares with the previous one
-                if (n_done > 0 && !mbar_wait(smem_u32(&acc_empty_bar), (n_done - 1) & 1u, abort_ptr, p.status)) break;
+                if (n_done > 0 && !mbar_wait_warp(smem_u32(&acc_empty_bar), (n_done - 1) & 1u, abort_ptr, p.status)) break;
                 tc_fence_after();
                 const uint32_t acc = tmem_base + (n_done & 1u) * F8_ACC1_COL;
                 for (int kb = 0; kb < p.k_blocks; kb += F8_STAGE_KB) {
-                    if ((kb & 3) == 0 && !mbar_wait(smem_u32(&scale_full_bar[sbuf]), sphase, abort_ptr, p.status)) {
+                    if ((kb & 3) == 0 && !mbar_wait_warp(smem_u32(&scale_full_bar[sbuf]), sphase, abort_ptr, p.status)) {
                         alive = false;
                         break;
                     }
-                    if (!mbar_wait(smem_u32(&full_bar[stage]), phase, abort_ptr, p.status)) {
+                    if (!mbar_wait_warp(smem_u32(&full_bar[stage]), phase, abort_ptr, p.status)) {
                         alive = false;
                         break;
                     }
@@ -351,7 +351,7 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
             // the 32 columns of the overlap come first: the last ones of accumulator 0, the first ones of 1
             const bool backwards = half == 1 && (n_done & 1u) == 0;
             if (t.expert >= 0) {
-                if (!mbar_wait(smem_u32(&acc_full_bar[n_done & 1u]), (n_done >> 1) & 1u, abort_ptr, p.status)) break;
+                if (!mbar_wait_warp(smem_u32(&acc_full_bar[n_done & 1u]), (n_done >> 1) & 1u, abort_ptr, p.status)) break;
                 tc_fence_after();
             }
             const int col = t.w0 + static_cast<int>(rank) * 128 + quad * 32 + (lane & 3) * 8;
@@ -452,7 +452,7 @@ gemm_fp8_kernel(const __grid_constant__ GemmFp8Params p) {
                 }
                 if (ends[buf] > 0) {
                     const uint32_t last = ends[buf] - 1;
-                    if (!mbar_wait(smem_u32(&empty_bar[last % F8_STAGES]), (last / F8_STAGES) & 1u, abort_ptr, p.status)) {
+                    if (!mbar_wait_warp(smem_u32(&empty_bar[last % F8_STAGES]), (last / F8_STAGES) & 1u, abort_ptr, p.status)) {
                         alive = false;
                         break;
                     }

@@ -66,6 +66,10 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
         }
     }
 }
+// With one answer for a whole converged warp (see mbar_wait_warp).
+__device__ __forceinline__ bool mbar_wait_cluster_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
+    return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, abort_flag, status));
+}
 // TMA load into this CTA's shared memory whose completion bytes are counted on the LEADER's mbarrier.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t leader_bar, int c0, int c1) {
     asm volatile(

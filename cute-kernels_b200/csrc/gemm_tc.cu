@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(64 + 32 * EPI_WARPS, 1) gemm_tc_kernel(const _
         int sslot = 0;
         uint32_t sphase = 0;
         while (true) {
-            if (!mbar_wait(smem_u32(&sched_full_bar[sslot]), sphase, abort_ptr, p.status)) break;
+            if (!mbar_wait_warp(smem_u32(&sched_full_bar[sslot]), sphase, abort_ptr, p.status)) break;
             const int tile = sched_tile[sslot];
             const int e_cur = sched_expert[sslot];
             __syncwarp();
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(64 + 32 * EPI_WARPS, 1) gemm_tc_kernel(const _
                 decode_segment(p, t, s, a_k0, b_k0, len);
                 any_k |= len > 0;
             }
-            if (!mbar_wait(smem_u32(&acc_full_bar[buf]), acc_phase, abort_ptr, p.status)) break;
+            if (!mbar_wait_warp(smem_u32(&acc_full_bar[buf]), acc_phase, abort_ptr, p.status)) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + buf * BN + (static_cast<uint32_t>(quad * 32) << 16);
             const bool row_ok = row_in_tile < t.rows_valid;

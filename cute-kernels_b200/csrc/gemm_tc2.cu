@@ -405,7 +405,7 @@ gemm_tc2_kernel(const __grid_constant__ GemmParams p) {
         int sslot = 0;
         uint32_t sphase = 0;
         while (true) {
-            if (!mbar_wait_cluster(smem_u32(&sched_full_bar[sslot]), sphase, abort_ptr, p.status)) break;
+            if (!mbar_wait_cluster_warp(smem_u32(&sched_full_bar[sslot]), sphase, abort_ptr, p.status)) break;
             const int tile = sched_tile[sslot];
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&sched_empty_bar[sslot]), 0));
@@ -438,7 +438,7 @@ gemm_tc2_kernel(const __grid_constant__ GemmParams p) {
             for (int h = 0; h < HALVES; ++h) {
             const int hs = h;  // tensor-memory half
             const uint32_t phs = acc_phase;
-            if (!mbar_wait(smem_u32(&acc_full_bar[hs]), phs, abort_ptr, p.status)) {
+            if (!mbar_wait_warp(smem_u32(&acc_full_bar[hs]), phs, abort_ptr, p.status)) {
                 alive = false;
                 break;
             }

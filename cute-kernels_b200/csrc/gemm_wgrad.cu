@@ -178,7 +178,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
             for (int tile = pair_id; tile < total_tiles && alive; tile += n_pairs) {
                 const WgradTile t = wgrad_decode(p, tile);
                 if (t.halves == 0) continue;
-                if (n_done >= 2 && !mbar_wait(smem_u32(&acc_empty_bar[n_done & 1u]), ((n_done >> 1) - 1) & 1u, abort_ptr, p.status)) break;
+                if (n_done >= 2 && !mbar_wait_warp(smem_u32(&acc_empty_bar[n_done & 1u]), ((n_done >> 1) - 1) & 1u, abort_ptr, p.status)) break;
                 tc_fence_after();
                 const uint32_t acc = tmem_base + (n_done & 1u) * 256;
                 for (int h0 = 0; h0 < t.halves && alive; h0 += 2) {
@@ -187,7 +187,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (h0 + h >= t.halves || !alive) continue;
-                        alive = mbar_wait(smem_u32(&full_bar[stage][h]), (phases[h] >> stage) & 1u, abort_ptr, p.status);
+                        alive = mbar_wait_warp(smem_u32(&full_bar[stage][h]), (phases[h] >> stage) & 1u, abort_ptr, p.status);
                         if (!alive) continue;
                         phases[h] ^= 1u << stage;
                         tc_fence_after();
@@ -216,7 +216,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WG_THREADS, 1) linea
             const WgradTile t = wgrad_decode(p, tile);
             const uint32_t acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + (n_done & 1u) * 256;
             if (t.halves > 0) {
-                if (!mbar_wait(smem_u32(&acc_full_bar[n_done & 1u]), (n_done >> 1) & 1u, abort_ptr, p.status)) break;
+                if (!mbar_wait_warp(smem_u32(&acc_full_bar[n_done & 1u]), (n_done >> 1) & 1u, abort_ptr, p.status)) break;
                 tc_fence_after();
             }
             const int first_row = t.m0 + static_cast<int>(rank) * 128 + quad * 32;
