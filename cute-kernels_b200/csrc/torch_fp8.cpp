@@ -38,6 +38,10 @@ std::string name_of(at::ScalarType t) {  // as Python prints it
 void require_cuda(const Tensor& t) {
     TORCH_CHECK(!t.defined() || t.is_cuda(), "this op runs on CUDA tensors only (no CPU fallback exists)");
 }
+// There is no forward-mode derivative, and a dual tensor need not require a gradient: without this its tangent would be lost.
+void refuse_tangent(const char* name, const Tensor& t) {
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), name, ": forward-mode derivatives are not available");
+}
 // The kernels leave no graph behind: a second derivative would come out as none.
 void once_differentiable() { TORCH_CHECK(!at::GradMode::is_enabled(), "the 8-bit operators can be differentiated once only (create_graph=False)"); }
 void check_cols(const char* name, int64_t cols) {
@@ -305,6 +309,8 @@ Tensor linear(const char* name, const Tensor& x, const py::object& weight, const
     }
     Tensor counts = counts_in;
     const at::IntArrayRef shape = parameter.defined() ? parameter.sizes() : at::IntArrayRef(held->shape);
+    refuse_tangent(name, x);
+    refuse_tangent(name, parameter);
     require_cuda(x);
     require_cuda(parameter);
     require_cuda(counts);
@@ -421,6 +427,8 @@ struct SwigluCheckpoint : torch::autograd::Function<SwigluCheckpoint> {
 Tensor swiglu_fp8_checkpoint(const Tensor& gate, const Tensor& up) {
     TORCH_CHECK(gate.sizes() == up.sizes() && gate.scalar_type() == up.scalar_type() && gate.device() == up.device(),
                 "swiglu_fp8_checkpoint: gate and up must have the same shape, dtype and device");
+    refuse_tangent("swiglu_fp8_checkpoint", gate);
+    refuse_tangent("swiglu_fp8_checkpoint", up);
     require_cuda(gate);
     dtype_code(gate.scalar_type());
     TORCH_CHECK(gate.dim() > 0, "swiglu_fp8_checkpoint: gate needs at least one dimension");
@@ -478,6 +486,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             }));
     for (const char* name : {"Fp8Blocks", "Fp8Weight"}) m.attr(name).attr("__module__") = "fma_b200";  // where pickle finds them
     m.def("few", &few, "Whether this many rows take the one-launch product (rows, experts, N, K).");
+    m.def(
+        "refuse_tangents", [](const char* name, const std::vector<Tensor>& tensors) { for (const Tensor& t : tensors) refuse_tangent(name, t); },
+        "Raises if one of the tensors carries a forward-mode tangent.");
     m.def("quantize_fp8", &quantize_fp8);
     m.def("quantize_fp8_weight", &quantize_fp8_weight);
     m.def("linear_fp8", &linear_fp8);

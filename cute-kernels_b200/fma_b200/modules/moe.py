@@ -431,9 +431,10 @@ class MoE(nn.Module):
         if hidden_states.dtype not in (torch.bfloat16, torch.float16) or self.c_fc.weight.dtype != hidden_states.dtype:
             raise RuntimeError(f"fp8_experts runs bfloat16 and float16 layers, got {hidden_states.dtype} tokens and "
                                f"{self.c_fc.weight.dtype} weights")  # fmt: skip
+        inputs = (hidden_states, router_weights, self.c_fc.weight, self.c_proj.weight)
+        _native.binding().refuse_tangents("fp8_experts", inputs)
         T = hidden_states.size(0)
-        graph = torch.is_grad_enabled() and any(
-            t.requires_grad for t in (hidden_states, router_weights, self.c_fc.weight, self.c_proj.weight))  # fmt: skip
+        graph = torch.is_grad_enabled() and any(t.requires_grad for t in inputs)
         held = None
         if not graph and self._held_experts is not None:
             if self._held_experts[2] != self._expert_weights_seen():

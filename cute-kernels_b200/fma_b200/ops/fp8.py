@@ -11,7 +11,8 @@ sums over tokens, where 1 x 128 blocks do not help: it is the 16-bit product of 
 that the 8-bit activations stand for.  The 8-bit activations are all that the forward pass keeps.
 
 The checks, the memory and the autograd nodes are in csrc/torch_fp8.cpp; the kernels are launched on the current stream of
-the arguments' device, and none of the calls waits for the device.  The gradients can be taken once (no create_graph).
+the arguments' device, and none of the calls waits for the device.  The gradients can be taken once (no create_graph); there are
+no forward-mode derivatives.  What is held in 8 bits by `quantize_fp8` or `quantize_fp8_weight` is a constant to autograd.
 """
 
 from __future__ import annotations

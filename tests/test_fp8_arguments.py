@@ -126,3 +126,27 @@ def test_definition_against_torchs_conversion(tall):
                     e += 1
             want = (part * 2.0**-e).to(torch.float8_e4m3fn).double() * 2.0**e
             assert torch.equal(held[r : r + tall, c : c + 128], want)
+
+
+def test_tangents_are_refused():
+    """A dual tensor need not require a gradient; its tangent must not get lost on the way without an autograd node."""
+    import torch.autograd.forward_ad as fwd
+
+    import fma_b200 as fma
+
+    x, w = torch.zeros(4, 16, dtype=torch.bfloat16), torch.zeros(8, 16, dtype=torch.bfloat16)
+    moe = fma.MoE(2, 1, 16, 8, fma.swiglu_packed, True, False, 0.02).bfloat16()
+    moe.fp8_experts = True
+    with fwd.dual_level():
+        dx, dw = (fwd.make_dual(t, torch.ones_like(t)) for t in (x, w))
+        for call in (lambda: fma.linear_fp8(dx, w), lambda: fma.linear_fp8(x, dw),
+                     lambda: fma.grouped_linear_fp8(dx, w[None], torch.tensor([4])),
+                     lambda: fma.grouped_linear_fp8(x, dw[None], torch.tensor([4])),
+                     lambda: fma.swiglu_fp8_checkpoint(dx, x), lambda: fma.swiglu_fp8_checkpoint(x, dx),
+                     lambda: moe._compute_experts(dx, torch.ones(4, 1).bfloat16(), torch.zeros(4, 1, dtype=torch.int64))):  # fmt: skip
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        for call in (lambda: fma.linear_fp8(x, w), lambda: fma.swiglu_fp8_checkpoint(x, x)):
+            with pytest.raises(RuntimeError, match="CUDA"):  # without a tangent the call goes on
+                call()
