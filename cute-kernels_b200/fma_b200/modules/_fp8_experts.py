@@ -113,6 +113,8 @@ class Fp8SwigluExperts(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        if torch.is_grad_enabled():  # what follows leaves no graph: the experts' part of a second derivative would be lost
+            raise RuntimeError("fp8_experts: the experts can be differentiated once only (create_graph=False)")
         x8, up8, gate8, act8, out, weights, fc, proj = ctx.saved_tensors
         fc, proj = ((b.data_ptr(), b.data_ptr() + at) for b, at in zip((fc, proj), ctx.scales_at))
         maps, (T, H, I), dtype, dev = ctx.maps, ctx.sizes, ctx.dtype, dy.device

@@ -150,3 +150,10 @@ def test_tangents_are_refused():
         for call in (lambda: fma.linear_fp8(x, w), lambda: fma.swiglu_fp8_checkpoint(x, x)):
             with pytest.raises(RuntimeError, match="CUDA"):  # without a tangent the call goes on
                 call()
+
+
+def test_second_derivatives_of_the_experts_are_refused():
+    from fma_b200.modules._fp8_experts import Fp8SwigluExperts
+
+    with torch.enable_grad(), pytest.raises(RuntimeError, match="once"):  # how the engine calls it under create_graph=True
+        Fp8SwigluExperts.backward(None, torch.zeros(1))

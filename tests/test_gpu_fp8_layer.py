@@ -186,3 +186,14 @@ def test_refusals():
     biased.fp8_experts = True
     with pytest.raises(RuntimeError, match="without bias"):
         biased(x)
+
+
+def test_second_derivatives_are_refused():
+    x = randn((300, 64), torch.bfloat16, 16).to(DEV).requires_grad_()
+    moe = _layer(4, 2, 64, 32, torch.bfloat16)
+    y, _ = moe(x)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    y, _ = moe(x)
+    (d_x,) = torch.autograd.grad(y.sum(), x)
+    assert bool(torch.isfinite(d_x).all()) and not d_x.requires_grad
