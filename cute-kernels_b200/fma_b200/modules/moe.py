@@ -203,6 +203,11 @@ def _is_swiglu_packed(fn: Callable) -> bool:
     return bool(getattr(fn, "_fma_b200_is_swiglu_packed", False))
 
 
+def _version(w: torch.Tensor) -> int | None:
+    """The count of writes to w; tensors made in inference mode have none."""
+    return None if w.is_inference() else w._version
+
+
 class Experts(nn.Module):
     def __init__(
         self, num_experts: int, in_features: int, out_features: int, add_bias: bool = True, std: float | None = None
@@ -255,7 +260,7 @@ class MoE(nn.Module):
     # Set to True to run the SwiGLU experts on 8-bit operands (bfloat16 / float16 layers): the products take e4m3 operands
     # with a scale per block of 128, and the backward pass works from 8-bit activations (modules/_fp8_experts.py).
     fp8_experts = False
-    _held_experts = None  # what quantize_experts() made
+    _held_experts = None  # what quantize_experts() made, and of what; empty once the weights are others
 
     def __init__(
         self,
@@ -414,16 +419,39 @@ class MoE(nn.Module):
     def _experts_in_8_bits(self):
         return tuple(quantize_fp8_weight(w) for w in (self.c_fc.weight, self.c_proj.weight))
 
-    def _expert_weights_seen(self):
-        return tuple((w._version, w.data_ptr(), w.dtype, w.device) for w in (self.c_fc.weight, self.c_proj.weight))
-
     @torch.no_grad()
     def quantize_experts(self) -> None:
         """For serving with fp8_experts: quantises the expert weights once, for all later forward passes without gradients
         (otherwise, and whenever gradients are recorded, every forward quantises the weights it finds).  After the
-        weights have changed, call it again; until then such a forward raises an error."""
+        weights have changed, call it again.  Until then such a forward raises an error where the change can be seen: writes to
+        the parameters that count in their version (optimizers, load_state_dict, in-place operations), other parameters or
+        other memory in their place.  Writes through `.data`, or from outside of torch, cannot be seen, nor can any to
+        parameters that were made in inference mode: without another call the layer goes on with the old weights."""
         with torch.cuda.device(self.c_fc.weight.device):
-            self._held_experts = (*self._experts_in_8_bits(), self._expert_weights_seen())
+            held = self._experts_in_8_bits()
+        # the aliases keep the memory, so that no other weights can come to lie at its address
+        self._held_experts = (held, tuple((w.detach(), _version(w)) for w in (self.c_fc.weight, self.c_proj.weight)))
+
+    def _quantized_experts(self):
+        """What quantize_experts() made, None if it was not called; raises if the weights are others now."""
+        if self._held_experts is None:
+            return None
+        if self._held_experts and not all(
+            w.data_ptr() == was.data_ptr() and w.dtype == was.dtype and w.device == was.device and _version(w) == version
+            for w, (was, version) in zip((self.c_fc.weight, self.c_proj.weight), self._held_experts[1])
+        ):
+            self._held_experts = ()
+        if not self._held_experts:
+            raise RuntimeError("the expert weights have changed since quantize_experts(): call it again")
+        return self._held_experts[0]
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        try:
+            self._quantized_experts()  # lets go of the old weights' memory if they moved
+        except RuntimeError:
+            pass
+        return self
 
     def _compute_experts_fp8(self, hidden_states, router_weights, selected_experts):
         if not (self.is_glu and _is_swiglu_packed(self.act) and self.c_fc.bias is None and self.c_proj.bias is None):
@@ -435,13 +463,7 @@ class MoE(nn.Module):
         _native.binding().refuse_tangents("fp8_experts", inputs)
         T = hidden_states.size(0)
         graph = torch.is_grad_enabled() and any(t.requires_grad for t in inputs)
-        held = None
-        if not graph and self._held_experts is not None:
-            if self._held_experts[2] != self._expert_weights_seen():
-                raise RuntimeError("the expert weights have changed since quantize_experts(): call it again")
-            held = self._held_experts[:2]
-        if held is None:
-            held = self._experts_in_8_bits()
+        held = (None if graph else self._quantized_experts()) or self._experts_in_8_bits()
         if not graph and _fp8_experts.few(T * self.top_k, held[1]):
             maps = self._sort_selected(selected_experts, row_align=1)
             self.last_row_maps = maps

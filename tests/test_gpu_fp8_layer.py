@@ -197,3 +197,83 @@ def test_second_derivatives_are_refused():
     y, _ = moe(x)
     (d_x,) = torch.autograd.grad(y.sum(), x)
     assert bool(torch.isfinite(d_x).all()) and not d_x.requires_grad
+
+
+def _refuses_until_quantized_again(moe, x):
+    with torch.no_grad():
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match="have changed"):
+                moe(x)
+        moe.quantize_experts()
+        held, _ = moe(x)
+        moe._held_experts = None
+        assert torch.equal(held, moe(x)[0])
+        moe.quantize_experts()
+
+
+def test_experts_quantized_once_follow_the_weights_or_refuse():
+    x = randn((5, 64), torch.bfloat16, 15).to(DEV)
+    moe, other = _layer(4, 2, 64, 32, torch.bfloat16), _layer(4, 2, 64, 32, torch.bfloat16, seed=7)
+    moe.quantize_experts()
+    with torch.no_grad():
+        first, _ = moe(x)
+    # writes that the parameters count
+    moe.load_state_dict(other.state_dict())
+    _refuses_until_quantized_again(moe, x)
+    optimizer = torch.optim.SGD(moe.parameters(), lr=0.1)
+    moe(x)[0].sum().backward()
+    optimizer.step()
+    _refuses_until_quantized_again(moe, x)
+    # other parameters: of three sets one after the other the third may get the memory of the first
+    shape = moe.c_fc.weight.shape
+    first_set = torch.zeros(shape, dtype=torch.bfloat16, device=DEV)
+    moe.c_fc.weight = torch.nn.Parameter(first_set)
+    moe.quantize_experts()
+    del first_set
+    for fill in (1.0, 2.0):
+        moe.c_fc.weight = torch.nn.Parameter(torch.full(shape, fill, dtype=torch.bfloat16, device=DEV))
+    _refuses_until_quantized_again(moe, x)
+    # moved away and back
+    moe.cpu()
+    moe.cuda()
+    _refuses_until_quantized_again(moe, x)
+    # a copy has the same weights, whatever it holds, and follows its own
+    twin = copy.deepcopy(moe)
+    with torch.no_grad():
+        twin.c_proj.weight.mul_(2)
+        moe(x)
+    _refuses_until_quantized_again(twin, x)
+    assert first.shape == x.shape
+
+
+def test_writes_through_data_are_seen_after_the_next_call():
+    """What the documentation of quantize_experts says of writes that torch does not count."""
+    x = randn((5, 64), torch.bfloat16, 15).to(DEV)
+    moe = _layer(4, 2, 64, 32, torch.bfloat16)
+    moe.quantize_experts()
+    with torch.no_grad():
+        before, _ = moe(x)
+        moe.c_proj.weight.data.mul_(2)
+        assert torch.equal(moe(x)[0], before)
+        moe.quantize_experts()
+        assert torch.equal(moe(x)[0], 2 * before)  # a power of two: every rounding is the same
+
+
+def test_parameters_made_in_inference_mode():
+    x = randn((5, 64), torch.bfloat16, 15).to(DEV)
+    with torch.inference_mode():
+        moe = _layer(4, 2, 64, 32, torch.bfloat16)
+        assert moe.c_fc.weight.is_inference()
+        want, _ = moe(x)
+        moe.quantize_experts()
+        assert torch.equal(moe(x)[0], want)
+
+
+def test_old_weights_are_let_go_when_the_layer_moves():
+    moe = _layer(4, 2, 512, 512, torch.bfloat16)
+    moe.quantize_experts()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    moe.cpu()
+    gone = before - torch.cuda.memory_allocated()
+    assert gone >= 3 * 4 * 512 * 512 * (2 + 1)  # in 16 bits and in 8
