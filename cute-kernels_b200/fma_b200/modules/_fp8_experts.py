@@ -90,14 +90,14 @@ def _weight_gradient(d_rows: torch.Tensor, a: _Held, maps: K.RowMaps) -> torch.T
 
 class Fp8SwigluExperts(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weights, w_fc, w_proj, held_fc, held_proj, maps: K.RowMaps):
+    def forward(ctx, x, weights, w_fc, w_proj, held_fc, held_proj, maps: K.RowMaps, keep: bool):
+        """keep: a backward pass may follow (ctx.needs_input_grad says True under torch.no_grad as well)."""
         x, weights = x.contiguous(), weights.contiguous()
         T, H = x.shape
         I, dev, cap = held_proj.shape[-1], x.device, maps.rows_cap
         x8 = _quantize_scatter(x, maps)
         fc, proj = held_fc.addresses, held_proj.addresses
         pre = _product(x8, *fc, 2 * I, x.dtype, maps)
-        keep = any(ctx.needs_input_grad)
         act8, up8, gate8 = _Held(cap, I, dev), *((_Held(cap, I, dev) if keep else None) for _ in range(2))
         at = (gate8.values, gate8.scales, up8.values, up8.scales) if keep else (None,) * 4
         call("fma_b200_swiglu_fp8_forward", pre.data_ptr() + I * pre.element_size(), 2 * I, ptr(pre), 2 * I, None, I,
@@ -141,7 +141,7 @@ class Fp8SwigluExperts(torch.autograd.Function):
                 if need_x:
                     d_xg = _product(d_pre8 or _quantize_rows(d_pre, used), *fc, H, dtype, maps, dgrad=True)
                     d_x = K.scatter_backward(d_xg, maps, T)
-        return d_x, d_w, d_w_fc, d_w_proj, None, None, None
+        return d_x, d_w, d_w_fc, d_w_proj, None, None, None, None
 
 
 def few(rows: int, held_proj) -> bool:

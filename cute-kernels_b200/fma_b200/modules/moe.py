@@ -471,4 +471,4 @@ class MoE(nn.Module):
         maps = self._sort_selected(selected_experts)
         self.last_row_maps = maps
         return _fp8_experts.Fp8SwigluExperts.apply(hidden_states, router_weights, self.c_fc.weight, self.c_proj.weight,
-                                                   *held, maps)  # fmt: skip
+                                                   *held, maps, graph)  # fmt: skip

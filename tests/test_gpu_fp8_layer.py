@@ -277,3 +277,26 @@ def test_old_weights_are_let_go_when_the_layer_moves():
     moe.cpu()
     gone = before - torch.cuda.memory_allocated()
     assert gone >= 3 * 4 * 512 * 512 * (2 + 1)  # in 16 bits and in 8
+
+
+def test_serving_keeps_nothing_for_a_backward_pass(monkeypatch):
+    from fma_b200.modules import _fp8_experts
+
+    calls = []
+
+    def record(name, *args):
+        if name == "fma_b200_swiglu_fp8_forward":
+            calls.append([a is not None for a in args[10:14]])  # gate and up in 8 bits, and their scales
+        return call(name, *args)
+
+    call = _fp8_experts.call
+    monkeypatch.setattr(_fp8_experts, "call", record)
+    x = randn((300, 64), torch.bfloat16, 17).to(DEV)
+    moe = _layer(4, 2, 64, 32, torch.bfloat16)
+    with torch.no_grad():
+        served, _ = moe(x)
+    trained, _ = moe(x)
+    moe.requires_grad_(False)
+    frozen, _ = moe(x)
+    assert calls == [[False] * 4, [True] * 4, [False] * 4]
+    assert torch.equal(served, trained) and torch.equal(served, frozen)
