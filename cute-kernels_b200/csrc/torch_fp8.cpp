@@ -61,21 +61,10 @@ Tensor rows_2d(const Tensor& x) {
                (t.size(0) == 1 || (t.stride(0) >= cols && t.stride(0) * size % 16 == 0));
     };
     if (fits(x)) return x;
-    if (x.dim() != 2) {
-        // leading dimensions that collapse onto one pitch are a view
-        int64_t expect = x.dim() > 1 ? x.stride(-2) * x.size(-2) : 0;
-        bool collapses = x.stride(-1) == 1;
-        for (int64_t d = x.dim() - 3; d >= 0 && collapses; --d) {
-            collapses = x.size(d) == 1 || x.stride(d) == expect;
-            expect *= x.size(d);
-        }
-        if (collapses) {
-            const int64_t rows = x.numel() / cols;
-            const Tensor t = x.as_strided({rows, cols}, {x.dim() > 1 && rows > 1 ? x.stride(-2) : cols, 1});
-            if (fits(t)) return t;
-        }
-    }
-    return x.reshape({-1, cols}).clone(at::MemoryFormat::Contiguous);
+    // Leading dimensions that collapse onto one pitch are a view, whose derivative is a view too (that of as_strided fills
+    // and copies a tensor as large as x's memory).
+    const Tensor t = x.reshape({-1, cols});
+    return fits(t) ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 int64_t pitch_of_rows(const Tensor& x) { return x.size(0) == 1 ? x.size(1) : x.stride(0); }
 
