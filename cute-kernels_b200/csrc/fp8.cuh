@@ -102,6 +102,15 @@ static int launch_kernel(const char* what, void (*kernel)(Params...), dim3 grid,
     return FMA_B200_OK;
 }
 
+// Rows of expert e, at most `rows`; none for a negative count.  index_bytes: 8 and 4 for signed integers, -4 for unsigned ones.
+__device__ __forceinline__ int32_t fp8_count(const void* counts, int32_t index_bytes, int e, int64_t rows) {
+    const long long c = index_bytes == 8   ? static_cast<const long long*>(counts)[e]
+                        : index_bytes == 4 ? static_cast<long long>(static_cast<const int32_t*>(counts)[e])
+                                           : static_cast<long long>(static_cast<const uint32_t*>(counts)[e]);
+    return static_cast<int32_t>(c < 0 ? 0 : (c > rows ? rows : c));
+}
+inline bool known_index_bytes(int32_t n) { return n == 4 || n == 8 || n == -4; }
+
 // Row access: a warp takes 512 columns of a row (one scale word); 8 lanes share a block of 128 columns, so the block
 // maximum is three shuffles and every load instruction of the 8 lanes covers 128 contiguous bytes.
 template <typename T>

@@ -73,11 +73,7 @@ __device__ __forceinline__ bool few_locate(const FewRows& p, int chunk, int& exp
         return rows > 0;
     }
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-        long long c = 0;
-        if (e0 + lane < p.E)
-            c = p.index_bytes == 8 ? static_cast<const long long*>(p.counts)[e0 + lane]
-                                   : static_cast<long long>(static_cast<const int32_t*>(p.counts)[e0 + lane]);
-        int end = static_cast<int>(c < 0 ? 0 : (c > p.rows ? p.rows : c));
+        int end = e0 + lane < p.E ? fp8_count(p.counts, p.index_bytes, e0 + lane, p.rows) : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {  // running sum, cut off at p.rows
             const int v = __shfl_up_sync(0xffffffffu, end, o);
@@ -584,7 +580,7 @@ int fma_b200_fp8_few_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t
     FMAB_REQUIRE(static_cast<int64_t>(E) * N < (1LL << 31) - 1024, FMA_B200_ERR_BAD_ARG, "E*N overflows");
     FMAB_REQUIRE(x_pitch >= K && x_pitch % 8 == 0, FMA_B200_ERR_BAD_ARG, "x: row pitch %lld", (long long)x_pitch);
     FMAB_REQUIRE(E == 1 || counts != nullptr, FMA_B200_ERR_BAD_ARG, "several experts need their counts");
-    FMAB_REQUIRE(counts == nullptr || index_bytes == 4 || index_bytes == 8, FMA_B200_ERR_UNSUPPORTED, "index_bytes=%d", index_bytes);
+    FMAB_REQUIRE(counts == nullptr || known_index_bytes(index_bytes), FMA_B200_ERR_UNSUPPORTED, "index_bytes=%d", index_bytes);
     if (rows == 0) return FMA_B200_OK;
     FMAB_REQUIRE(x && w && w_scales && out, FMA_B200_ERR_BAD_ARG, "NULL pointer");
     FMAB_REQUIRE(aligned16(x) && aligned16(w) && aligned16(w_scales) && aligned16(out), FMA_B200_ERR_BAD_ARG,

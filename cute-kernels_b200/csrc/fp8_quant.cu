@@ -513,13 +513,8 @@ __global__ void __launch_bounds__(kMapThreads) group_maps_kernel(const GroupMaps
     __shared__ uint32_t warp_sums[2][32];
     const int t = threadIdx.x;
     const int n = p.E;  // groups 0..n-1 are experts, group n the rows of no expert
-    long long c = 0;
-    if (t < n) {
-        c = p.index_bytes == 8 ? static_cast<const long long*>(p.counts)[t]
-                               : static_cast<long long>(static_cast<const int32_t*>(p.counts)[t]);
-        c = c < 0 ? 0 : (c > p.rows ? p.rows : c);
-    }
-    const uint32_t end = running_sum(static_cast<uint32_t>(c), static_cast<uint32_t>(p.rows), warp_sums[0]);
+    const uint32_t c = t < n ? static_cast<uint32_t>(fp8_count(p.counts, p.index_bytes, t, p.rows)) : 0;
+    const uint32_t end = running_sum(c, static_cast<uint32_t>(p.rows), warp_sums[0]);
     if (t < n) off[t + 1] = static_cast<int32_t>(end);
     if (t == 0) off[0] = 0;
     __syncthreads();
@@ -744,7 +739,7 @@ int fma_b200_fp8_group_maps(const void* counts, int32_t index_bytes, int32_t E, 
                             int32_t* offsets, int32_t* pad_offsets, int32_t* group_rows, int32_t* tile_expert,
                             int32_t* tile_row, int32_t* tile_rows, void* stream) {
     using namespace fmab;
-    FMAB_REQUIRE(index_bytes == 4 || index_bytes == 8, FMA_B200_ERR_UNSUPPORTED, "index_bytes=%d", index_bytes);
+    FMAB_REQUIRE(known_index_bytes(index_bytes), FMA_B200_ERR_UNSUPPORTED, "index_bytes=%d", index_bytes);
     FMAB_REQUIRE(E >= 1 && E <= kMapThreads, FMA_B200_ERR_BAD_ARG, "E=%d not in [1,1024]", E);
     FMAB_REQUIRE(rows >= 0 && layout_rows % 256 == 0 && layout_rows < (1LL << 31) &&
                      layout_rows >= (rows + 255) / 256 * 256 + 256LL * (E < rows ? E : rows),

@@ -181,10 +181,11 @@ struct GroupMaps {
     int32_t* tile_row() const { return at(3 * E + 3 + tiles()); }
     int32_t* tile_rows() const { return at(3 * E + 3 + 2 * tiles()); }
 };
+int32_t index_bytes(const Tensor& counts) { return counts.scalar_type() == at::kUInt32 ? -4 : static_cast<int32_t>(counts.element_size()); }
 GroupMaps make_maps(const Tensor& counts, int64_t rows) {
     const int64_t E = counts.numel();
     GroupMaps m(at::empty({3 * E + 3 + 3 * (GroupMaps::layout_of(E, rows) / 128)}, counts.options().dtype(at::kInt)), E, rows);
-    check(fma_b200_fp8_group_maps(counts.data_ptr(), static_cast<int32_t>(counts.element_size()), static_cast<int32_t>(E), rows, m.layout_rows,
+    check(fma_b200_fp8_group_maps(counts.data_ptr(), index_bytes(counts), static_cast<int32_t>(E), rows, m.layout_rows,
                                   m.offsets(), m.pad_offsets(), m.group_rows(), m.tile_expert(), m.tile_row(), m.tile_rows(), stream_of(counts)),
           "fma_b200_fp8_group_maps");
     return m;
@@ -225,7 +226,7 @@ Tensor few_rows(const Tensor& x, const Weight& w, const Tensor& counts) {
     check(fma_b200_fp8_few_rows(x.data_ptr(), pitch_of_rows(x), dtype_code(x.scalar_type()), x.size(0), w.values(), w.scales(),
                                 static_cast<int32_t>(w.E), static_cast<int32_t>(w.N), static_cast<int32_t>(w.K),
                                 counts.defined() ? counts.data_ptr() : nullptr,
-                                counts.defined() ? static_cast<int32_t>(counts.element_size()) : 4, out.data_ptr(), stream_of(x)),
+                                counts.defined() ? index_bytes(counts) : 4, out.data_ptr(), stream_of(x)),
           "fma_b200_fp8_few_rows");
     return out;
 }

@@ -445,8 +445,8 @@ int fma_b200_fp8_quantize_weight(const void* w, int32_t dtype, int32_t E, int32_
 int fma_b200_fp8_dequantize(const void* values, const void* scales, int32_t batch, int64_t rows, int64_t cols,
                             const int32_t* rows_used, void* out, int32_t dtype, void* stream);
 /*
- * Maps for rows grouped by expert without alignment: counts [E] (4- or 8-byte integers on the device) rows per
- * expert, rows = rows there are.  Writes offsets[E+1] (running sums, cut off at `rows`), pad_offsets[E+2] (first row of
+ * Maps for rows grouped by expert without alignment: counts [E] (on the device; index_bytes 4 or 8 for signed integers,
+ * of which negative ones count as 0, -4 for unsigned ones of 4 bytes) rows per expert, rows = rows there are.  Writes offsets[E+1] (running sums, cut off at `rows`), pad_offsets[E+2] (first row of
  * each expert in a layout aligned to 256 rows; entry E+1 is the end with the rows of no expert), group_rows[E] (the
  * counts after the cut), and for every 128-row tile of the layout its expert (-1 unused, -2 rows behind the last expert's), first source row and number
  * of source rows.  layout_rows is a multiple of 256, at least round_up(rows, 256) + 256 * min(E, rows).
@@ -478,7 +478,7 @@ int fma_b200_fp8_gemm_dgrad(const void* dy, const void* dy_scales, int64_t layou
                             const int32_t* rows_used, const int32_t* row_offsets, const int32_t* row_counts, void* stream);
 /*
  * The same product for a few rows, in one launch: x [rows, K] in bfloat16 or half is quantised on the way in; counts
- * [E] (4- or 8-byte integers on the device, NULL: one expert) consecutive rows per expert, rows behind the last
+ * [E] (on the device, index_bytes as for group_maps, NULL: one expert) consecutive rows per expert, rows behind the last
  * expert's give zeros.  For any number of rows, but meant for up to about 16 per expert: an expert's weights are read
  * once per 16 of its rows.
  */

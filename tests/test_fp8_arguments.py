@@ -157,3 +157,16 @@ def test_second_derivatives_of_the_experts_are_refused():
 
     with torch.enable_grad(), pytest.raises(RuntimeError, match="once"):  # how the engine calls it under create_graph=True
         Fp8SwigluExperts.backward(None, torch.zeros(1))
+
+
+def test_kinds_of_counts():
+    from fma_b200 import _native
+
+    lib = _native.lib()
+    null, at, odd = ctypes.c_void_p(None), ctypes.c_void_p(16), ctypes.c_void_p(24)
+    for index_bytes in (0, 2, -2, -8):
+        assert lib.fma_b200_fp8_group_maps(at, index_bytes, 4, 100, 2048, at, at, at, at, at, at, null) == 2
+        assert lib.fma_b200_fp8_few_rows(at, 16, 1, 4, at, at, 3, 16, 16, at, index_bytes, at, null) == 2
+    for index_bytes in (4, 8, -4):  # accepted: what is refused is the next argument
+        assert lib.fma_b200_fp8_group_maps(at, index_bytes, 4, 100, 1024, at, at, at, at, at, at, null) == 1
+        assert lib.fma_b200_fp8_few_rows(odd, 16, 1, 4, at, at, 3, 16, 16, at, index_bytes, at, null) == 1
