@@ -5,8 +5,8 @@
 // TMA streams it without any thread touching it.  A cluster of up to eight CTAs shares a tile, each with its part of the
 // reduction (whole groups of 512 columns): 4096 weight rows are only 32 tiles, and every SM has to load for the memory
 // to run at its rate.  The parts are added through distributed shared memory in the order of the ranks.
-// (With mma.sync and weights from global memory into registers one row of 14336 x 4096 took 17 to 23 us, this way 14: the
-// 8-bit mma.sync costs several times the instructions of the loads.)
+// (With mma.sync and weights from global memory into registers one row of 14336 x 4096 took 17 to 23 us, this way 14 from a
+// captured graph, 16.5 call by call: the 8-bit mma.sync costs several times the instructions of the loads.)
 #include "fp8.cuh"
 #include "gemm_pair.cuh"
 
@@ -470,16 +470,20 @@ __global__ void __launch_bounds__(kSomeThreads) some_rows_kernel(const __grid_co
     }
 }
 
-// CTAs per tile, in whole groups of 512 columns: until nearly every SM has one, and on while a CTA would read more than
-// 256 KB and there is room for all of them (three per SM).  Measured, one row: 14336 x 4096 (112 tiles) 16.1 / 14.1 / 17.0 us
-// with 1 / 2 / 4 CTAs per tile, 4096 x 4096 (32 tiles) 7.8 / 6.5 / 7.6 with 2 / 4 / 8, 4096 x 14336 16.9 / 14.6 with 4 / 8,
-// 8 rows of 8 experts of 1536 x 2048 (96 tiles) 9.5 / 10.9 with 2 / 4.
+// CTAs per tile, in whole groups of 512 columns: until nearly every SM has one, on while a CTA would read four groups (256 KB)
+// or more and there is room for all of them (three per SM), and on while its part is too long: longer than what fits into tensor
+// memory, or in the product that quantises x itself than what leaves room for a second CTA on the SM.  Measured from captured
+// graphs, weights not in L2: one row of 14336 x 4096 (112 tiles) 15.6 / 13.9 / 17.5 us with 1 / 2 / 4 CTAs per tile, 8192 x 4096 (64)
+// 12.3 / 10.5 / 14.2 with 2 / 4 / 8, 4096 x 4096 (32) 10.2 / 8.8 / 8.2, 4096 x 14336 (32) 16.7 / 14.3 with 4 / 8; eight rows of eight
+// experts, 5 of them hit, of 1536 x 2048 10.0 / 9.0 / 9.2 with 1 / 2 / 4, 4096 x 4096 27.7 / 23.8 / 25.8, 8192 x 8192 82.7 / 80.9 / 69.0;
+// 64 rows, tiles of up to 128, quantising included, 8192 x 4096 17.6 / 15.6 / 22.9 with 2 / 4 / 8, 4096 x 4096 15.8 / 12.5 / 13.8.
 constexpr int FEW_QUADS_MOST = 18;  // rows of x in 8 bits that fit into shared memory beside the ring
+constexpr int FEW_QUADS_TWO = 5;    // and that leave room for a second CTA on the SM
 static int few_split(int64_t items, int quads, int quads_fit) {
     const int64_t sms = sm_count();
     int split = 1;
     while (split < 8 && 2 * split <= quads &&
-           (100 * items * split < 85 * sms || (quads > 4 * split && 2 * items * split <= 3 * sms) || quads > quads_fit * split))
+           (100 * items * split < 85 * sms || (quads >= 4 * split && 2 * items * split <= 3 * sms) || quads > quads_fit * split))
         split *= 2;
     return split;
 }
@@ -490,6 +494,11 @@ static int64_t few_chunks(int64_t rows, int32_t E, bool counts) {  // at most
     if (!counts) return (rows + kFewRows - 1) / kFewRows;
     const int64_t groups = E + 1 < rows ? E + 1 : rows, n = rows / kFewRows + groups;
     return n < rows ? n : rows;
+}
+
+static int64_t few_chunks_even(int64_t rows, int32_t E) {  // if the rows are spread evenly
+    const int64_t n = (rows + kFewRows - 1) / kFewRows, hit = rows < E ? rows : E;
+    return n > hit ? n : hit;
 }
 
 // Opts a kernel into large dynamic shared memory, once per kernel and device.
@@ -604,7 +613,7 @@ int fma_b200_fp8_few_rows(const void* x, int64_t x_pitch, int32_t dtype, int64_t
     p.tiles = static_cast<int32_t>(fp8_row_tiles(N));
     p.b_tiles = E * p.tiles;
     const int64_t items = few_chunks(rows, E, counts != nullptr) * p.tiles;
-    p.split = few_split(items, p.quads, FEW_QUADS_MOST);
+    p.split = few_split(few_chunks_even(rows, E) * p.tiles, p.quads, FEW_QUADS_TWO);
     p.quads_most = (p.quads + p.split - 1) / p.split;
     p.tmem_cols = 32;
     while (p.tmem_cols < static_cast<uint32_t>(kFewScaleCol + kFewScaleCols * p.quads_most)) p.tmem_cols *= 2;

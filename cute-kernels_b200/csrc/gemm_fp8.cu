@@ -509,15 +509,17 @@ static int rows_per_tile(int64_t rows, int N) {
 }
 
 // Whether tiles of 128 weight rows and up to 128 rows of x, spread over clusters along k, are the faster way: with few
-// rows, where the pair tiles leave at least half of the pairs without work.  Measured (this way / pair tiles): one matrix
-// of 4096 x 4096 (16 tiles), 16 / 32 / 48 rows 7.9 / 8.7 / 9.1 us against 12.9 / 13.0 / 13.3, 4096 x 14336 (16) 20.5 / 21.3 /
-// 22.2 against 33.9 to 34.5, two experts of 4096 x 4096 (32) 13.4 / 14.1 / 14.9 against 13.9 / 14.3 / 14.5, of 4096 x 14336
-// 27.7 / 28.7 / 29.5 against 36.4 to 37.3; but 14336 x 4096 (56) 16.4 / 17.3 / 18.3 against 16.0 / 16.2 / 16.5, eight
-// experts of 4096 x 4096 (128) 31 to 32 against 30 to 31, 128 of 1536 x 2048 80 / 84 / 89 against 76 / 77 / 79.
+// rows, where the pair tiles leave at least half of the pairs without work, and up to 128 rows of a matrix, or per expert, if
+// there is much to share along k.  Measured from captured graphs, quantising x included, this way / pair tiles, us: 4096 x 4096 (16
+// pair tiles) with 17 / 64 / 128 rows 10.8 / 12.5 / 15.0 against 17.2 to 17.8, 4096 x 14336 18.5 / 21.0 / 25.7 against 39.4 to 40.3,
+// 8192 x 4096 (32) 24 / 96 rows 14.0 / 17.0 against 17.9 / 18.5; but 2048 x 768 48 / 64 rows 8.8 / 9.5 against 9.3 / 9.0, and
+// 14336 x 4096 (56) 24 / 64 / 128 rows 19.5 / 21.0 / 24.7 against 19.4 / 19.7 / 20.7.  Two experts of 4096 x 4096 (32) with 48 / 96
+// rows each 22.0 / 25.5 against 22.4 / 24.6, of 4096 x 14336 with 64 rows 48.8 against 58.4, of 1024 x 14336 33 against 53, four of
+// 1024 x 4096 with 96 rows 21.3 against 23.7; but eight of 14336 x 4096 101 against 97, 128 of 1536 x 2048 91 to 106 against 90 to 97.
 static bool some_rows_suit(int64_t layout_rows, int64_t out_rows, int32_t E, int32_t N, int32_t K, bool experts, bool tile_rows) {
     if (!fp8_some_rows_fits(K) || E * ((N + 255LL) / 256) * 2 > sm_count() / 2) return false;
-    if (!experts) return layout_rows <= 64 || (layout_rows <= 96 && K >= N) || (layout_rows <= 128 && K >= 2LL * N);
-    return tile_rows && out_rows <= 48LL * E;  // without tile_rows the rows of a layout are not known here
+    if (!experts) return layout_rows <= 48 || (layout_rows <= 128 && K >= 1536);
+    return tile_rows && out_rows <= (K >= 2LL * N ? 128LL : 48LL) * E;  // without tile_rows the rows of a layout are not known here
 }
 
 template <bool TURNED>

@@ -6,6 +6,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <utility>
+#include <vector>
+
 #include "../../include/fma_b200.h"
 
 namespace {
@@ -210,15 +214,36 @@ Tensor product(const Held& a, const Weight& w, bool turned, at::ScalarType dtype
     return out;
 }
 
-// Whether the product that reads x itself, in one launch, is the faster way.  Above, x is quantised by a launch of its own.
-// Measured with weights of 4096 x 4096: 8.3 us against 9.7 for one row, 9.8 / 10.1 for 16, 12.1 / 10.5 for 24; of 14336 x 4096:
-// 14.7 / 19.3, 18.9 / 19.5, 31.1 / 19.6; 128 experts of 1536 x 2048: 83 / 90 for 8 rows each, 92 / 91 for 12, 102 / 93 for 16;
-// eight of 4096 x 4096: 36 / 40 for 4, 42 / 39 for 12.  Every tile of the weights quantises x again, which counts where there
-// are several experts with many tiles or long rows: eight of 4096 x 14336 86 / 102 for one row each, 106 / 103 for two, 127 /
-// 107 for eight; of 14336 x 4096 80 / 75, 92 / 86, 110 / 97.
-bool few(int64_t rows, int64_t E, int64_t N, int64_t K) {
-    if (K > (1 << 16)) return false;
-    return rows <= (E == 1 ? 16 : (N * K <= (1 << 25) ? 12 * E : E));
+// Whether the product that reads x itself, in one launch, is the faster way; otherwise x is quantised by a launch of its own
+// (with experts also their row maps are made) and the tiles are those of fma_b200_fp8_gemm.  The one launch loses by its CTAs:
+// each starts cold, and quantises again the rows that its tile shares with the others of the same rows.  So they are counted: one per
+// 128 weight rows and part of the reduction (as few_split deals it, five groups of 512 columns at most; twice where a part is
+// longer and an SM has room for one only) for each expert that may be hit, and three for every 16 rows.  The other way costs
+// more with experts.  Measured from captured graphs, weights not in L2, this way / the other, us:
+//   one matrix  14336 x 4096: 1 row 14.6 / 19.0, 16 rows 18.6 / 19.3, 24 rows 27.3 / 19.4;  28672 x 4096: 8 rows 30.3 / 31.1,
+//               16 rows 35.1 / 31.3;  32768 x 8192: 1 row 53.4 / 54.8, 8 rows 58.2 / 55.2;  8192 x 28672: 1 row 73 / 47
+//   2 experts   14336 x 4096: 4 rows 28.6 / 38.3, 24 rows 34.6 / 37.7, 48 rows 50.3 / 37.4
+//   8 experts   14336 x 4096: 8 rows 59.5 / 63.4, 32 rows 99.3 / 97.6, 128 rows 130 / 98;  4096 x 4096: 64 rows 33.8 / 39.0,
+//               128 rows 44.3 / 38.8
+//   32 experts  8192 x 4096: 16 rows 84 / 88, 64 rows 183 / 169, 384 rows 246 / 186;  1536 x 2048: 384 rows 28.2 / 33.4
+//   128 experts 1536 x 2048: 8 rows 11.5 / 18.9, 512 rows 73 / 89, 1536 rows 91.1 / 90.6;  2048 x 768: 64 rows 24.7 / 30.2, 512 rows
+//               58.9 / 52.1;  4096 x 4096: 8 rows 32 / 40, 64 rows 173 / 152
+// Over 1276 such cases (1 to 256 experts, 17 shapes, rows spread at random) the faster way is missed by 1.2 % on average.
+// Rows that pile up on few experts are not known here; they go 16 at a time all the same.
+// In the layer both products go one way, and the other way has more work around them: E = 128, k = 8, H = 2048, I = 768 with 64 /
+// 96 / 192 tokens 179 / 190 / 215 against 207 / 209 / 210, E = 8, k = 2, H = 4096, I = 14336 with 4 / 8 / 16 tokens 237 / 288 / 326
+// against 254 / 287 / 312.
+bool few(int64_t rows, int64_t E, const std::vector<std::pair<int64_t, int64_t>>& shapes) {
+    if (rows > 16 * E) return false;
+    int64_t ctas = 0;
+    for (const auto& [N, K] : shapes) {
+        if (K > (1 << 16)) return false;
+        const int64_t tiles = (N + 127) / 128, groups = (K + 511) / 512;
+        int64_t parts = 1;
+        while (parts < 8 && groups > 5 * parts) parts *= 2;
+        ctas += tiles * parts * (groups > 5 * parts ? 2 : 1);
+    }
+    return (16 * std::min(E, rows) + 3 * rows) * ctas <= 16 * (E == 1 ? 1220 : (shapes.size() == 1 ? 3300 : 4000)) * static_cast<int64_t>(shapes.size());
 }
 
 Tensor few_rows(const Tensor& x, const Weight& w, const Tensor& counts) {
@@ -343,7 +368,7 @@ Tensor linear(const char* name, const Tensor& x, const py::object& weight, const
     if (want_x || want_w) {
         using Maybe = std::optional<Tensor>;
         out = Linear::apply(x2, parameter.defined() ? Maybe(parameter) : Maybe(), held, grouped ? Maybe(counts) : Maybe(), want_x, want_w);
-    } else if (few(rows, held->E, N, K)) {
+    } else if (few(rows, held->E, {{N, K}})) {
         out = few_rows(x2, *held, counts);
     } else {
         GroupMaps maps;
@@ -475,7 +500,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                                        t[5].cast<int64_t>()});
             }));
     for (const char* name : {"Fp8Blocks", "Fp8Weight"}) m.attr(name).attr("__module__") = "fma_b200";  // where pickle finds them
-    m.def("few", &few, "Whether this many rows take the one-launch product (rows, experts, N, K).");
+    m.def("few", &few, "Whether this many rows take the one-launch products (rows, experts, [(N, K) of each product]).");
     m.def(
         "refuse_tangents", [](const char* name, const std::vector<Tensor>& tensors) { for (const Tensor& t : tensors) refuse_tangent(name, t); },
         "Raises if one of the tensors carries a forward-mode tangent.");

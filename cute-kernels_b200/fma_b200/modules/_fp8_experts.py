@@ -147,8 +147,7 @@ class Fp8SwigluExperts(torch.autograd.Function):
 def few(rows: int, held_proj) -> bool:
     """Whether `few_tokens` is the faster way for this many routed rows."""
     E, H, I = held_proj.shape
-    one = _native.binding().few
-    return rows > 0 and one(rows, E, 2 * I, H) and one(rows, E, H, I)
+    return rows > 0 and _native.binding().few(rows, E, [(2 * I, H), (H, I)])
 
 
 def few_tokens(x, weights, held_fc, held_proj, maps: K.RowMaps) -> torch.Tensor:

@@ -170,3 +170,29 @@ def test_kinds_of_counts():
     for index_bytes in (4, 8, -4):  # accepted: what is refused is the next argument
         assert lib.fma_b200_fp8_group_maps(at, index_bytes, 4, 100, 1024, at, at, at, at, at, at, null) == 1
         assert lib.fma_b200_fp8_few_rows(odd, 16, 1, 4, at, at, 3, 16, 16, at, index_bytes, at, null) == 1
+
+
+# (experts, N, K, rows, us of the product in one launch, us with a launch that quantises): what the rule's comment quotes
+FEW = [(1, 14336, 4096, 1, 14.6, 19.0), (1, 14336, 4096, 16, 18.6, 19.3), (1, 14336, 4096, 24, 27.3, 19.4), (1, 28672, 4096, 8, 30.3, 31.1),
+       (1, 28672, 4096, 16, 35.1, 31.3), (1, 32768, 8192, 1, 53.4, 54.8), (1, 32768, 8192, 8, 58.2, 55.2), (1, 8192, 28672, 1, 73, 47),
+       (2, 14336, 4096, 4, 28.6, 38.3), (2, 14336, 4096, 24, 34.6, 37.7), (2, 14336, 4096, 48, 50.3, 37.4), (8, 14336, 4096, 8, 59.5, 63.4),
+       (8, 14336, 4096, 128, 130, 98), (8, 4096, 4096, 64, 33.8, 39.0), (32, 8192, 4096, 64, 183, 169), (32, 8192, 4096, 384, 246, 186),
+       (32, 1536, 2048, 384, 28.2, 33.4), (128, 1536, 2048, 8, 11.5, 18.9), (128, 1536, 2048, 512, 73, 89), (128, 2048, 768, 64, 24.7, 30.2),
+       (128, 2048, 768, 512, 58.9, 52.1), (128, 4096, 4096, 8, 32, 40), (128, 4096, 4096, 64, 173, 152)]  # fmt: skip
+
+
+@pytest.mark.parametrize("E,N,K,rows,one,two", FEW)
+def test_the_faster_product_is_taken(E, N, K, rows, one, two):
+    from fma_b200 import _native
+
+    assert _native.binding().few(rows, E, [(N, K)]) == (one < two)
+
+
+def test_both_products_of_the_layer_go_one_way():
+    from fma_b200 import _native
+
+    few = _native.binding().few
+    fine, wide = [(1536, 2048), (2048, 768)], [(28672, 4096), (4096, 14336)]
+    assert [few(8 * tokens, 128, fine) for tokens in (1, 64, 96, 192)] == [True, True, True, False]
+    assert [few(2 * tokens, 8, wide) for tokens in (1, 4, 16, 64)] == [True, True, False, False]
+    assert not few(17 * 4, 4, [(8, 8)]) and not few(1, 1, [(8, (1 << 16) + 8)])

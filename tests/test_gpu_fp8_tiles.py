@@ -124,3 +124,34 @@ def test_layer_on_few_pairs(sms):
     for g, f in zip(got, free):
         assert bool(torch.isfinite(g).all()) and torch.equal(g, f)
     check_device_status()
+
+
+# reductions of 1 to 128 groups of 512 columns, shared by one to eight CTAs, the last group short; tiles of 128 weight rows
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("K,N", [(520, 40), (1032, 4104), (2056, 264), (4104, 1800), (4104, 8200), (8200, 136), (14336, 264), (20488, 136), (65536, 24)])
+@pytest.mark.parametrize("rows", [1, 16, 49, 100])
+def test_few_rows_share_the_reduction(dtype, K, N, rows):
+    import fma_b200 as fma
+
+    x, w = randn((rows, K), dtype, 30).to(DEV), randn((N, K), dtype, 31, scale=0.02).to(DEV)
+    want, size = R.hold(x) @ R.hold_weight(w).T, R.hold(x).abs() @ R.hold_weight(w).abs().T
+    held = fma.quantize_fp8_weight(w)
+    got = fma.linear_fp8(x, held)
+    R.check_product(got, want, size, K)
+    assert torch.equal(got, fma.linear_fp8(x, held))
+    check_device_status()
+
+
+@pytest.mark.parametrize("K,N,E,rows", [(4104, 1032, 8, 8), (4104, 264, 8, 100), (8200, 264, 5, 30), (20488, 72, 3, 6), (2056, 776, 40, 64), (14344, 136, 2, 200), (1032, 264, 100, 700)])
+def test_few_rows_of_experts_share_the_reduction(K, N, E, rows):
+    import fma_b200 as fma
+
+    g = torch.Generator().manual_seed(K + rows)
+    counts = torch.bincount(torch.randint(0, E, (rows - 1,), generator=g), minlength=E).tolist()
+    x, w = randn((rows, K), torch.bfloat16, 32).to(DEV), randn((E, N, K), torch.bfloat16, 33, scale=0.02).to(DEV)
+    values, sizes = R.grouped(x, w, counts, torch.zeros(rows, N, device=DEV))
+    held, count = fma.quantize_fp8_weight(w), torch.tensor(counts, device=DEV)
+    got = fma.grouped_linear_fp8(x, held, count)
+    R.check_product(got, values[0], sizes[0], K)
+    assert torch.equal(got, fma.grouped_linear_fp8(x, held, count))
+    check_device_status()
