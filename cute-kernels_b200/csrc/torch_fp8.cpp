@@ -243,7 +243,7 @@ bool few(int64_t rows, int64_t E, const std::vector<std::pair<int64_t, int64_t>>
         while (parts < 8 && groups > 5 * parts) parts *= 2;
         ctas += tiles * parts * (groups > 5 * parts ? 2 : 1);
     }
-    return (16 * std::min(E, rows) + 3 * rows) * ctas <= 16 * (E == 1 ? 1220 : (shapes.size() == 1 ? 3300 : 4000)) * static_cast<int64_t>(shapes.size());
+    return (16 * std::min(E, rows) + 3 * rows) * ctas <= 16 * (E == 1 ? 1150 : (shapes.size() == 1 ? 3300 : 4000)) * static_cast<int64_t>(shapes.size());
 }
 
 Tensor few_rows(const Tensor& x, const Weight& w, const Tensor& counts) {
