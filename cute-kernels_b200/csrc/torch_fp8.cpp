@@ -114,6 +114,7 @@ struct Blocks {
         return held.buffer.narrow(0, 0, held.rows * pitch_of(held.cols)).view(at::kFloat8_e4m3fn).view({held.rows, pitch_of(held.cols)}).narrow(1, 0, held.cols);
     }
     Tensor dequantized(const py::object& to) const {
+        require_cuda(held.buffer);
         const c10::cuda::CUDAGuard guard(held.buffer.device());
         return dequantize(held.values(), held.scales(), 1, held.rows, shape, scalar_type_or(to, dtype), held.buffer, nullptr);
     }
@@ -142,6 +143,7 @@ struct Weight {
     Tensor values_tensor() const { return buffer.narrow(0, 0, value_bytes()).view(at::kFloat8_e4m3fn).view({E, N, pitch_of(K)}); }
     Tensor scales_tensor() const { return buffer.narrow(0, value_bytes(), scale_bytes()); }
     Tensor dequantized(const py::object& to) const {
+        require_cuda(buffer);
         const c10::cuda::CUDAGuard guard(buffer.device());
         return dequantize(values(), scales(), E, N, shape, scalar_type_or(to, dtype), buffer, nullptr);
     }

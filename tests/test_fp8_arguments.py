@@ -197,3 +197,16 @@ def test_both_products_of_the_layer_go_one_way():
     assert [few(8 * tokens, 128, fine) for tokens in (1, 64, 96, 192)] == [True, True, True, False]
     assert [few(2 * tokens, 8, wide) for tokens in (1, 4, 16, 64)] == [True, True, False, False]
     assert not few(17 * 4, 4, [(8, 8)]) and not few(1, 1, [(8, (1 << 16) + 8)])
+
+
+def test_what_was_loaded_to_the_cpu_stays_there():
+    import fma_b200 as fma
+
+    held = fma.Fp8Blocks.__new__(fma.Fp8Blocks)  # as unpickling makes it
+    held.__setstate__((torch.zeros(16 * 16 + 512, dtype=torch.uint8), 16, 16, [16, 16], 15))
+    assert held.device.type == "cpu" and held.shape == (16, 16) and held.dtype == torch.bfloat16 and held.nbytes == 768
+    weight = fma.Fp8Weight.__new__(fma.Fp8Weight)
+    weight.__setstate__((torch.zeros(16 * 16 + 512, dtype=torch.uint8), [16, 16], 15, 1, 16, 16))
+    for other in (held, weight):
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            other.dequantize()
