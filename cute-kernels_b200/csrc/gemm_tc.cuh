@@ -130,7 +130,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 // The same for all lanes of a converged warp, with one answer for all of them.  Each lane polls for itself, so when the
 // limit runs out just as the phase completes some see the one and some the other; lanes that went on alone would stand
-// in the next elect.sync, warp barrier or tcgen05 instruction of the whole warp for good.
+// in the next elect.sync, warp barrier or tcgen05 instruction of the whole warp for good.  The vote costs 0.6 % of a long 8-bit
+// product (8192 x 4096 x 14336 354.8 -> 357.0 us) and 1 % of one with short sums (128 experts of 1536 x 2048, 65536 rows, 209.2 ->
+// 211.2; input gradient 218.0 -> 220.7); the weight gradients show nothing.
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status));
 }
